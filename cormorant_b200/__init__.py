@@ -8,7 +8,9 @@ batch-sharded multi-GPU driver (``sharding``).
 """
 from ._lib import CormorantError, lib  # noqa: F401
 from .kernels import (  # noqa: F401
-    OP_ADD, OP_DIV, OP_MUL, OP_RELU, OP_RELU6, OP_SUB, POOL_AVG, POOL_LP, POOL_MAX,
-    ConvKernel, ConvKernelFused, MatmulKernel, MatmulKernelFused, PoolingKernel, VectorOPKernel, init,
+    F8_E4M3, F8_E5M2, OP_ADD, OP_DIV, OP_MUL, OP_RELU, OP_RELU6, OP_SUB, POOL_AVG, POOL_LP, POOL_MAX,
+    T_BF16, T_F16, T_F32, T_Q88,
+    ConvKernel, ConvKernelFused, MatmulKernel, MatmulKernelFp8, MatmulKernelFp8Grouped, MatmulKernelFused,
+    PoolingKernel, QuantKernelFp8, RmsNormKernelFp8, VectorOPKernel, init,
     launch_count, release, synchronize,
 )

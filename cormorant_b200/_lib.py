@@ -20,6 +20,7 @@ CM_ENOINIT = -6
 
 _p = C.c_void_p
 _u = C.c_uint
+_l = C.c_uint64
 
 # name -> (restype, argtypes); every function declared in include/cormorant_cuda.h
 SIGNATURES: dict[str, tuple] = {
@@ -75,6 +76,14 @@ SIGNATURES: dict[str, tuple] = {
     "cm_conv_weights_destroy": (None, [_p]),
     "cm_conv_prepared": (C.c_int, [_p] * 5 + [_u, _p, _p]),
     "cm_conv_prepared_async": (C.c_int, [_p] * 5 + [_u, _p, _p, _p]),
+    "cm_quant_fp8": (C.c_int, [_p, _u, _p, _p] + [_u] * 3 + [_l] * 6 + [_u] * 2),
+    "cm_quant_fp8_async": (C.c_int, [_p, _u, _p, _p] + [_u] * 3 + [_l] * 6 + [_u] * 2 + [_p]),
+    "cm_rmsnorm_fp8": (C.c_int, [_p] * 7 + [_u] * 2 + [_l] * 6 + [_u] * 2 + [C.c_float, _u]),
+    "cm_rmsnorm_fp8_async": (C.c_int, [_p] * 7 + [_u] * 2 + [_l] * 6 + [_u] * 2 + [C.c_float, _u, _p]),
+    "cm_matmul_fp8": (C.c_int, [_p] * 5 + [_u] * 3 + [_l] * 5 + [_u] * 3),
+    "cm_matmul_fp8_async": (C.c_int, [_p] * 5 + [_u] * 3 + [_l] * 5 + [_u] * 3 + [_p]),
+    "cm_matmul_fp8_grouped": (C.c_int, [_p] * 6 + [_u] * 4 + [_l] * 7 + [_u] * 3),
+    "cm_matmul_fp8_grouped_async": (C.c_int, [_p] * 6 + [_u] * 4 + [_l] * 7 + [_u] * 3 + [_p]),
     "cm_calls_supported": (C.c_int, [_p, _u]),
     "cm_calls": (C.c_int, [_p, _u]),
     "cm_calls_async": (C.c_int, [_p, _u, _p]),

@@ -63,7 +63,8 @@ int finish_sync(cm_stream_t stream) {
 }
 
 // ---- profiling --------------------------------------------------------------
-static const char* kProfNames[PK_COUNT] = {"gemm_q88", "split", "vectorop", "pool", "conv_aux"};
+static const char* kProfNames[PK_COUNT] = {"gemm_q88", "split", "vectorop", "pool", "conv_aux", "fp8_gemm",
+                                            "fp8_quant"};
 struct ProfPair { int kind; cudaEvent_t a, b; };
 static std::mutex g_prof_mu;
 static bool g_prof_on = false;

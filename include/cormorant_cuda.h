@@ -117,7 +117,7 @@ int cm_int8_mma_rate(unsigned pairs, unsigned iters, double* tops, double* ms, d
  * Between cm_profile_begin and cm_profile_end every kernel launch is bracketed
  * by CUDA events on its own stream.  cm_profile_read waits for those events
  * and returns the summed device time and launch count of one kernel family:
- * "gemm_q88", "split", "vectorop", "pool" or "conv_aux". */
+ * "gemm_q88", "split", "vectorop", "pool", "conv_aux", "fp8_gemm" or "fp8_quant". */
 int cm_profile_begin(void);
 int cm_profile_end(void);
 int cm_profile_read(const char* kernel, double* total_ms, uint64_t* launches);
@@ -376,6 +376,79 @@ int cm_matmul_prepared(const cm_matmul_weights_t* w, const int16_t* a, int16_t* 
 int cm_matmul_prepared_async(const cm_matmul_weights_t* w, const int16_t* a, int16_t* c, unsigned n, unsigned batch,
                              unsigned a_batch_stride, unsigned c_batch_stride, unsigned epilogue, const int16_t* bias,
                              cm_stream_t stream);
+
+/* ---- Block-scaled 8-bit floating point (no reference counterpart) ---------------------
+ * Serving a transformer's projections, norms and experts beside the Q8.8 kernels.  A block of
+ * 128 values x is held as q = round(x * (F / A)), A = max(max|x|, 2^-100), with the fp32 scale
+ * A / F; F is the format's largest finite value (CM_F8_E4M3: 448, CM_F8_E5M2: 57344), rounding
+ * is to nearest even.  A NaN in a block makes its scale and all its q NaN; an infinity makes
+ * the scale infinite, the finite values 0 and the infinite ones NaN.
+ *   activations  one scale for each row and 128 columns: scale[cb * lds + row], cb < ceil(cols/128)
+ *   weights      one scale for each 128 x 128 block:     scale[rb * lds + cb],  rb < ceil(rows/128)
+ * (the last blocks may be partial).  Row pitches (ld*) and strides are in elements and 64-bit,
+ * at least the row's length; CM_T_* name the type of an untyped buffer, aligned to its elements.
+ * Tensors may lie at any such alignment; rows of 8-bit operands that start on 16-byte boundaries
+ * (base and pitch) are read in place by the matrix products, others are first copied into such
+ * rows (stream-ordered scratch).  Inputs and outputs of one call must not overlap, except where
+ * an entry says so.  Calls are recorded into a stream capture like the other *_async entries. */
+#define CM_T_Q88    0u       /* int16 words, value = raw / 256 */
+#define CM_T_F32    1u
+#define CM_T_F16    2u
+#define CM_T_BF16   3u
+#define CM_F8_E4M3  0u
+#define CM_F8_E5M2  1u
+/* x [batch][rows][cols] -> q and its scales; block_rows 1 (activations) or 128 (weights).
+ * scale pitch lds >= rows (block_rows 1) or >= ceil(cols/128) (128).  x_batch_stride may be 0. */
+int cm_quant_fp8(const void* x, unsigned x_type, uint8_t* q, float* scale, unsigned rows, unsigned cols,
+                 unsigned batch, uint64_t ldx, uint64_t ldq, uint64_t lds, uint64_t x_batch_stride,
+                 uint64_t q_batch_stride, uint64_t scale_batch_stride, unsigned format, unsigned block_rows);
+int cm_quant_fp8_async(const void* x, unsigned x_type, uint8_t* q, float* scale, unsigned rows, unsigned cols,
+                       unsigned batch, uint64_t ldx, uint64_t ldq, uint64_t lds, uint64_t x_batch_stride,
+                       uint64_t q_batch_stride, uint64_t scale_batch_stride, unsigned format, unsigned block_rows,
+                       cm_stream_t stream);
+/* RMS norm with the residual's addition and an 8-bit output:
+ *   h = x + resid (fp32);  resid_out = h;  y = h / sqrt(mean(h^2) + eps) * weight;
+ *   q, scale = the blocks of y (activations, 1 x 128; scale pitch lds >= rows).
+ * resid (null: h = x), resid_out (needs resid), weight [cols] (null: 1), y, and q with scale may
+ * be null, but not y and q both.  x, resid, resid_out and y are of `type` (CM_T_F32 / F16 /
+ * BF16), weight of weight_type (one of the same).  y is rounded from fp32 and q from the fp32 y;
+ * the norm takes h unrounded.  resid_out may be resid or x itself (the same address and pitch),
+ * and so may y be x.  At most 32768 columns (CM_EUNSUPPORTED); eps finite and >= 0. */
+int cm_rmsnorm_fp8(const void* x, const void* resid, const void* weight, void* resid_out, void* y, uint8_t* q,
+                   float* scale, unsigned rows, unsigned cols, uint64_t ldx, uint64_t ldr, uint64_t ldo, uint64_t ldy,
+                   uint64_t ldq, uint64_t lds, unsigned type, unsigned weight_type, float eps, unsigned format);
+int cm_rmsnorm_fp8_async(const void* x, const void* resid, const void* weight, void* resid_out, void* y, uint8_t* q,
+                         float* scale, unsigned rows, unsigned cols, uint64_t ldx, uint64_t ldr, uint64_t ldo,
+                         uint64_t ldy, uint64_t ldq, uint64_t lds, unsigned type, unsigned weight_type, float eps,
+                         unsigned format, cm_stream_t stream);
+/* c[i][j] = sum over t < ceil(k/128) of a_scale[t*a_scale_ld + i] * b_scale[(j/128)*b_scale_ld + t]
+ *                                       * (sum of a[i][.] * b[j][.] over the block's columns),
+ * i < n, j < m: a [n][k] activations, b [m][k] weights (k contiguous in both: a . b transposed),
+ * each in its own format, c of c_type.  Sums are fp32 and are rounded once to c_type (CM_T_Q88:
+ * floor to 1/256, saturating, NaN = 0).  The product of a block's two scales has to be finite.
+ * k = 0 gives zeros.  Results do not depend on the stream or on other calls in flight. */
+int cm_matmul_fp8(const uint8_t* a, const float* a_scale, const uint8_t* b, const float* b_scale, void* c, unsigned n,
+                  unsigned k, unsigned m, uint64_t lda, uint64_t a_scale_ld, uint64_t ldb, uint64_t b_scale_ld,
+                  uint64_t ldc, unsigned a_format, unsigned b_format, unsigned c_type);
+int cm_matmul_fp8_async(const uint8_t* a, const float* a_scale, const uint8_t* b, const float* b_scale, void* c,
+                        unsigned n, unsigned k, unsigned m, uint64_t lda, uint64_t a_scale_ld, uint64_t ldb,
+                        uint64_t b_scale_ld, uint64_t ldc, unsigned a_format, unsigned b_format, unsigned c_type,
+                        cm_stream_t stream);
+/* The same product with the rows of a and c grouped by expert: rows offsets[g] .. offsets[g+1]-1
+ * use b + g*b_group_stride and b_scale + g*b_scale_group_stride.  offsets: groups + 1 int32 on the
+ * device, increasing, within 0..n (read by the kernel: no host synchronisation; values outside
+ * are held to that range and order).  Groups may be empty; rows before offsets[0] and from
+ * offsets[groups] on are left as they were.  At most 1024 groups (CM_EUNSUPPORTED). */
+int cm_matmul_fp8_grouped(const uint8_t* a, const float* a_scale, const uint8_t* b, const float* b_scale, void* c,
+                          const int32_t* offsets, unsigned groups, unsigned n, unsigned k, unsigned m, uint64_t lda,
+                          uint64_t a_scale_ld, uint64_t ldb, uint64_t b_scale_ld, uint64_t b_group_stride,
+                          uint64_t b_scale_group_stride, uint64_t ldc, unsigned a_format, unsigned b_format,
+                          unsigned c_type);
+int cm_matmul_fp8_grouped_async(const uint8_t* a, const float* a_scale, const uint8_t* b, const float* b_scale, void* c,
+                                const int32_t* offsets, unsigned groups, unsigned n, unsigned k, unsigned m,
+                                uint64_t lda, uint64_t a_scale_ld, uint64_t ldb, uint64_t b_scale_ld,
+                                uint64_t b_group_stride, uint64_t b_scale_group_stride, uint64_t ldc, unsigned a_format,
+                                unsigned b_format, unsigned c_type, cm_stream_t stream);
 
 /* ---- Small call lists in one launch (no reference counterpart) ----------------------
  * A list of small kernel calls -- a batch-1 network, bound by launch latency -- run as ONE
