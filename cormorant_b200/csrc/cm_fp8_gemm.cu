@@ -1,14 +1,28 @@
 // cm_fp8_gemm.cu -- matrix products of block-scaled 8-bit floating point operands:
 //   c[i][j] = sum over 128-deep blocks t of  a_scale[t][i] * b_scale[j / 128][t] * (a[i][t] . b[j][t])
 // dense (cm_matmul_fp8) and grouped by expert (cm_matmul_fp8_grouped: rows offsets[g] ..
-// offsets[g+1] - 1 of a and c use b[g]).  A block's products are summed in fp32, scaled, and the
-// scaled blocks are summed in fp32; one rounding to the output type.
+// offsets[g+1] - 1 of a and c use b[g]).
+//
+// The weights are the tensor cores' 128-row operand and the tokens their N operand:
+//   D[128 weight rows (TMEM lanes)][TN tokens (TMEM columns)] = one 128-deep block of K
+// so a tile's weight scale is one number a block (a tile is one weight-scale block high), a single
+// token costs a 16-column tile instead of a 128-row one, and an output column is 32 neighbouring
+// lanes: its stores are whole sectors.  A block's product is a fresh accumulator (4 MMAs, 32 deep);
+// epilogue warps take it out of TMEM and add it, times token scale * weight scale, to fp32 sums in
+// registers, two columns an instruction, while the next blocks' MMAs run into other TMEM buffers.
+//
+// Warps: 0 TMA producer, 1 MMA issuer (of the pair's leader), 2-3 token scales (global memory ->
+// times the weight scale -> a ring in shared memory), 4.. epilogue.  Every mbarrier wait is bounded
+// by %globaltimer, as in cm_gemm.cu.
 #include <algorithm>
 
 #include "cm_fp8.cuh"
+#include "cm_tcgen05.cuh"
 
 namespace cm {
 namespace {
+
+constexpr uint32_t kMaxGroups = 1024;
 
 struct Fp8Args {
     const uint8_t* a;
@@ -21,76 +35,550 @@ struct Fp8Args {
     uint64_t lda, a_lds, ldb, b_lds, b_gs, bs_gs, ldc;
 };
 
-__device__ __forceinline__ float fp8_f32(uint32_t format, uint8_t v) {
-    uint32_t h;
-    if (format == CM_F8_E4M3) asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)v));
-    else asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(h) : "h"((uint16_t)v));
-    return __half2float(__ushort_as_half((unsigned short)(h & 0xffffu)));
+// What the kernel needs beside its two tensor maps.
+struct KArgs {
+    const float* as;
+    const float* bs;
+    void* c;
+    const int32_t* offsets;
+    uint64_t a_lds, b_lds, bs_gs, ldc;
+    uint32_t groups, n, m, c_type, kb, ksteps, tiles_m, tiles_t, total, idesc, group_step;
+    FastDiv fd_m;
+    int* status;
+    uint64_t timeout_ns;
+};
+
+template <int TN, int CG>
+struct F8Cfg {
+    static constexpr int EPI_WARPS = TN >= 128 ? 8 : 4;
+    static constexpr int COLS = TN / (EPI_WARPS / 4);        // token columns of an epilogue warp
+    static constexpr int THREADS = 128 + 32 * EPI_WARPS;
+    static constexpr int A_TILE = 128 * 128, B_TILE = TN / CG * 128;
+    static constexpr int STAGE = A_TILE + B_TILE;
+    static constexpr int STAGES = TN >= 128 ? 6 : TN == 64 ? 8 : TN == 32 ? 9 : 10;
+    static constexpr int NBUF = TN == 256 ? 2 : 4;           // accumulators in TMEM
+    static constexpr int SLOTS = 8;                          // scale ring
+    static constexpr uint32_t TMEM_COLS = NBUF * TN;
+    static constexpr int TABLES = 2 * (kMaxGroups + 1) * 4;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + SLOTS * TN * 4 + 512 + TABLES;
+    static_assert(SMEM <= 232448 && 2 * SMEM > 232448, "one CTA an SM");
+    static_assert(TN * 512 <= STAGES * STAGE, "partial sums of a split tile fit the stages");
+};
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+// the same, completing on the pair leader's barrier (bar is a shared::cluster address)
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
 }
 
-__device__ __forceinline__ void store_c(void* c, uint32_t type, uint64_t i, float v) {
-    switch (type) {
-        case CM_T_Q88: from_f32(v, ((int16_t*)c)[i]); break;
-        case CM_T_F32: from_f32(v, ((float*)c)[i]); break;
-        case CM_T_F16: from_f32(v, ((__half*)c)[i]); break;
-        default: from_f32(v, ((__nv_bfloat16*)c)[i]); break;
-    }
+template <int CG>
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
 }
 
-constexpr uint32_t ST = 64, SK = 32;
+// 16 accumulator columns of this warp's 32 lanes, complete on return: the wait carries the
+// registers, so nothing that reads them can move above it.
+#define CM_O(i) "=r"(r[i])
+#define CM_IO(i) "+r"(r[i])
+#define CM_16(X) X(0), X(1), X(2), X(3), X(4), X(5), X(6), X(7), X(8), X(9), X(10), X(11), X(12), X(13), X(14), X(15)
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : CM_16(CM_O)
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : CM_16(CM_IO)::"memory");
+}
+#undef CM_O
+#undef CM_IO
+#undef CM_16
 
-__global__ void __launch_bounds__(256) fp8_simple_kernel(Fp8Args g) {
-    griddep_wait();
-    __shared__ float as[ST][SK + 1], bs[ST][SK + 1];
-    uint32_t row0 = blockIdx.y * ST, row1 = g.n, group = 0;
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+// two fp32 multiply-adds in one instruction
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+struct TileF8 {
+    uint32_t m0;             // first weight row (of this CTA)
+    uint32_t row0, row1;     // token rows row0 .. row1 - 1, at most TN of them used
+    uint32_t group;
+};
+
+// Tile t: groups in order; within a group, bands of kBand token tiles are walked weight tile by
+// weight tile, so that the tiles in flight share a few operand panels in L2.
+constexpr uint32_t kBand = 8;
+
+template <int TN, int CG>
+__device__ __forceinline__ TileF8 decode_tile(const KArgs& g, const uint32_t* first, const uint32_t* ends, uint32_t t, uint32_t rank) {
+    uint32_t local = t, tt = g.tiles_t, row0 = 0, row1 = g.n, group = 0;
     if (g.offsets) {
-        // this CTA's token tile: groups in order, each in whole tiles; offsets are held to 0..n and
-        // to increasing order, so that no value of theirs can reach outside a and c
-        uint32_t left = blockIdx.y, lo = (uint32_t)min(max(g.offsets[0], 0), (int)g.n);
-        for (;; ++group) {
-            if (group == g.groups) return;
-            const uint32_t hi = max(lo, (uint32_t)min(max(g.offsets[group + 1], 0), (int)g.n));
-            const uint32_t tiles = (hi - lo + ST - 1) / ST;
-            if (left < tiles) { row0 = lo + left * ST; row1 = hi; break; }
-            left -= tiles;
-            lo = hi;
+        const uint32_t q = g.fd_m.div(t);                     // token tile over all groups
+        uint32_t lo = 0, hi = g.groups;                        // the last group with first[] <= q
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (first[mid] <= q) lo = mid;
+            else hi = mid;
         }
+        group = lo;
+        tt = first[lo + 1] - first[lo];
+        local = t - first[lo] * g.tiles_m;
+        row0 = ends[lo];
+        row1 = ends[lo + 1];
     }
-    const uint32_t col0 = blockIdx.x * ST;
-    const uint8_t* b = g.b + group * g.b_gs;
-    const float* bsc = g.bs + group * g.bs_gs;
-    const uint32_t tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    float acc[4][4] = {}, part[4][4] = {};
-    for (uint32_t k0 = 0; k0 < g.k; k0 += SK) {
-        for (uint32_t e = threadIdx.x; e < ST * SK; e += 256) {
-            const uint32_t r = e / SK, kk = e % SK;
-            as[r][kk] = row0 + r < row1 && k0 + kk < g.k ? fp8_f32(g.a_format, g.a[(row0 + r) * g.lda + k0 + kk]) : 0.0f;
-            bs[r][kk] = col0 + r < g.m && k0 + kk < g.k ? fp8_f32(g.b_format, b[(col0 + r) * g.ldb + k0 + kk]) : 0.0f;
-        }
-        __syncthreads();
-        for (uint32_t kk = 0; kk < SK; ++kk)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) part[i][j] = fmaf(as[ty + 16 * i][kk], bs[tx + 16 * j][kk], part[i][j]);
-        __syncthreads();
-        if ((k0 + SK) % kFp8Block == 0 || k0 + SK >= g.k) {
-            const uint32_t kb = k0 / kFp8Block;
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t r = row0 + ty + 16 * i, cc = col0 + tx + 16 * j;
-                    const float s = r < row1 && cc < g.m ? g.as[kb * g.a_lds + r] * bsc[(cc / kFp8Block) * g.b_lds + kb] : 0.0f;
-                    acc[i][j] = fmaf(part[i][j], s, acc[i][j]);
-                    part[i][j] = 0.0f;
-                }
-        }
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t r = row0 + ty + 16 * i, cc = col0 + tx + 16 * j;
-            if (r < row1 && cc < g.m) store_c(g.c, g.c_type, r * g.ldc + cc, acc[i][j]);
-        }
+    const uint32_t per = kBand * g.tiles_m, band = local / per, r = local - band * per;
+    const uint32_t size = min(kBand, tt - band * kBand), mt = r / size;
+    TileF8 c;
+    c.m0 = (mt * CG + rank) * 128;
+    c.row0 = row0 + (band * kBand + r - mt * size) * TN;
+    c.row1 = row1;
+    c.group = group;
+    return c;
 }
 
-constexpr uint32_t kMaxGroups = 1024;
+template <typename T, int COLS>
+__device__ __forceinline__ void store_cols(const KArgs& g, const TileF8& tc, uint32_t col0, uint32_t mrow, const uint64_t (&acc)[COLS / 2]) {
+    if (mrow >= g.m) return;
+    const uint32_t tok = tc.row0 + col0;
+    T* p = (T*)g.c + (uint64_t)tok * g.ldc + mrow;
+    const uint32_t live = tc.row1 > tok ? tc.row1 - tok : 0u;
+#pragma unroll
+    for (uint32_t j = 0; j < COLS / 2; ++j) {
+        float lo, hi;
+        unpack2(acc[j], lo, hi);
+        if (2 * j < live) from_f32(lo, *p);
+        p += g.ldc;
+        if (2 * j + 1 < live) from_f32(hi, *p);
+        p += g.ldc;
+    }
+}
+
+__device__ __forceinline__ void store_one(const KArgs& g, uint64_t i, float v) {
+    switch (g.c_type) {
+        case CM_T_Q88: from_f32(v, ((int16_t*)g.c)[i]); break;
+        case CM_T_F32: from_f32(v, ((float*)g.c)[i]); break;
+        case CM_T_F16: from_f32(v, ((__half*)g.c)[i]); break;
+        default: from_f32(v, ((__nv_bfloat16*)g.c)[i]); break;
+    }
+}
+
+// The token scales of one (tile, K block), as a scale warp holds them on their way from global
+// memory: the loads are issued two blocks of this warp (four of the CTA) ahead of their use.
+template <int TN>
+struct ScaleRegs {
+    float v[TN < 32 ? 1 : TN / 32];
+    float sb;
+};
+
+// KS: the CTAs of a cluster share one tile, each a contiguous part of its K blocks, and add their
+// sums through distributed shared memory, in the order of their ranks.
+template <int TN, int CG, bool KS>
+__global__ void __launch_bounds__(F8Cfg<TN, CG>::THREADS, 1)
+    gemm_f8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT, const KArgs g) {
+    using C = F8Cfg<TN, CG>;
+    static_assert(CG == 1 || !KS, "a pair does not split K");
+    griddep_wait();
+    griddep_launch_dependents();   // all CTAs are resident
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float* ring = (float*)(smem + C::STAGES * C::STAGE);
+    uint64_t* bars = (uint64_t*)(ring + C::SLOTS * TN);
+    uint64_t* full_b = bars;
+    uint64_t* empty_b = full_b + C::STAGES;
+    uint64_t* accf_b = empty_b + C::STAGES;
+    uint64_t* acce_b = accf_b + C::NBUF;
+    uint64_t* sfull_b = acce_b + C::NBUF;
+    uint64_t* sempty_b = sfull_b + C::SLOTS;
+    uint64_t* done_b = sempty_b + C::SLOTS;
+    volatile uint32_t* tmem_slot = (volatile uint32_t*)(done_b + 1);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    uint32_t* first = (uint32_t*)((uint8_t*)bars + 512);      // grouped: first token tile of each group
+    uint32_t* ends = first + kMaxGroups + 1;                   // grouped: offsets, held to 0..n and in order
+
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t crank = CG == 2 || KS ? cluster_rank() : 0u;
+    uint32_t csize = 1;
+    if (KS) asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
+    const uint32_t rank = CG == 2 ? crank : 0u;
+    const bool leader = rank == 0;
+    const uint32_t per_tile = CG == 2 ? 2u : csize;            // CTAs of a tile
+    const uint32_t cid = blockIdx.x / per_tile, ncl = gridDim.x / per_tile;
+    const uint32_t kb0 = KS ? (uint32_t)((uint64_t)g.kb * crank / csize) : 0u;
+    const uint32_t kb1 = KS ? (uint32_t)((uint64_t)g.kb * (crank + 1) / csize) : g.kb;
+    constexpr uint16_t kPairMask = 0x3;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(smem_u32(&full_b[s]), 1);
+            mbar_init(smem_u32(&empty_b[s]), 1);
+        }
+        for (int b = 0; b < C::NBUF; ++b) {
+            mbar_init(smem_u32(&accf_b[b]), 1);
+            mbar_init(smem_u32(&acce_b[b]), C::EPI_WARPS * CG);
+        }
+        for (int s = 0; s < C::SLOTS; ++s) {
+            mbar_init(smem_u32(&sfull_b[s]), 1);
+            mbar_init(smem_u32(&sempty_b[s]), C::EPI_WARPS);
+        }
+        mbar_init(smem_u32(done_b), 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        if (CG == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)),
+                         "r"(C::TMEM_COLS)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)),
+                         "r"(C::TMEM_COLS)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+        tc_fence_before();
+    }
+    if (g.offsets && warp == 2) {
+        // running maximum of the offsets held to 0..n, then running sum of the groups' token tiles:
+        // whatever the offsets hold, no row outside 0..n-1 is reached
+        uint32_t high = 0, tiles = 0;
+        for (uint32_t base = 0; base <= g.groups; base += 32) {
+            const uint32_t i = base + lane;
+            uint32_t e = i <= g.groups ? (uint32_t)min(max(g.offsets[i], 0), (int)g.n) : 0u;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const uint32_t p = __shfl_up_sync(0xffffffffu, e, o);
+                if (lane >= (uint32_t)o) e = max(e, p);
+            }
+            e = max(e, high);
+            uint32_t before = __shfl_up_sync(0xffffffffu, e, 1);
+            if (lane == 0) before = high;
+            // tiles of the group that ends at offset i (none ends at offset 0)
+            uint32_t cnt = i > 0 ? (e - before + TN - 1) / TN : 0u;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const uint32_t p = __shfl_up_sync(0xffffffffu, cnt, o);
+                if (lane >= (uint32_t)o) cnt += p;
+            }
+            if (i <= g.groups) {
+                ends[i] = e;
+                first[i] = tiles + cnt;
+            }
+            high = __shfl_sync(0xffffffffu, e, 31);
+            tiles += __shfl_sync(0xffffffffu, cnt, 31);
+        }
+    }
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();      // both CTAs' barriers exist before any remote arrival
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t total = g.offsets ? first[g.groups] * g.tiles_m : g.total;
+    const WaitCtl wc{abort_flag, g.status, g.timeout_ns};
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t s = 0, phase = 1, it = 0;
+            bool ok = true;
+            for (uint32_t t = cid; ok && t < total; t += ncl) {
+                const TileF8 tc = decode_tile<TN, CG>(g, first, ends, t, rank);
+                for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
+                    if (!mbar_wait(smem_u32(&empty_b[s]), phase, wc)) { ok = false; break; }
+                    const uint32_t st = smem_u32(smem + s * C::STAGE);
+                    if (CG == 2) {
+                        const uint32_t full = map_to_rank(smem_u32(&full_b[s]), 0);
+                        if (leader) mbar_expect_tx(smem_u32(&full_b[s]), 2 * C::STAGE);
+                        tma_load_3d_pair(st, &tmW, full, (int)(kb * 128), (int)tc.m0, (int)(tc.group * g.group_step));
+                        tma_load_2d_pair(st + C::A_TILE, &tmT, full, (int)(kb * 128), (int)(tc.row0 + rank * (TN / 2)));
+                    } else {
+                        const uint32_t full = smem_u32(&full_b[s]);
+                        mbar_expect_tx(full, C::STAGE);
+                        tma_load_3d(st, &tmW, full, (int)(kb * 128), (int)tc.m0, (int)(tc.group * g.group_step));
+                        tma_load_2d(st + C::A_TILE, &tmT, full, (int)(kb * 128), (int)tc.row0);
+                    }
+                    if (++s == C::STAGES) { s = 0; phase ^= 1; }
+                }
+            }
+            if (*abort_flag && leader) {
+                // let copies already in flight land before the CTA exits
+                const uint32_t from = it > C::STAGES ? it - C::STAGES : 0u;
+                volatile int never = 0;
+                WaitCtl drain{&never, g.status, g.timeout_ns};
+                for (uint32_t k = from; k < it; ++k) mbar_wait(smem_u32(&full_b[k % C::STAGES]), (k / C::STAGES) & 1u, drain);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            uint32_t s = 0, phase = 0, buf = 0, bphase = 1;
+            bool ok = true;
+            for (uint32_t t = cid; ok && t < total; t += ncl) {
+                for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait(smem_u32(&acce_b[buf]), bphase, wc) || !mbar_wait(smem_u32(&full_b[s]), phase, wc)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t da = sdesc(smem_u32(smem + s * C::STAGE)), db = sdesc(smem_u32(smem + s * C::STAGE + C::A_TILE));
+                    const uint32_t d = tmem + buf * TN;
+                    const uint32_t steps = g.ksteps - kb * 4;        // 32-deep steps with any column below k
+#pragma unroll
+                    for (uint32_t kk = 0; kk < 4; ++kk)
+                        if (kk < steps) umma_f8<CG>(d, da + 2 * kk, db + 2 * kk, g.idesc, kk != 0);
+                    if (CG == 2) {
+                        umma_commit_pair(smem_u32(&empty_b[s]), kPairMask);
+                        umma_commit_pair(smem_u32(&accf_b[buf]), kPairMask);
+                    } else {
+                        umma_commit(smem_u32(&empty_b[s]));
+                        umma_commit(smem_u32(&accf_b[buf]));
+                    }
+                    if (++s == C::STAGES) { s = 0; phase ^= 1; }
+                    if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
+                }
+            }
+            // every MMA issued by this thread has completed once `done` fires
+            if (CG == 2) umma_commit_pair(smem_u32(done_b), 0x1);
+            else umma_commit(smem_u32(done_b));
+            volatile int never = 0;
+            WaitCtl drain{&never, g.status, g.timeout_ns};
+            mbar_wait(smem_u32(done_b), 0, drain);
+        }
+    } else if (warp < 4) {
+        // Scale warps: 2 takes the even (tile, K block) items of this CTA, 3 the odd ones.
+        constexpr uint32_t AHEAD = 2;
+        ScaleRegs<TN> regs[AHEAD];
+        uint32_t t = cid, kb = kb0;
+        TileF8 tc{};
+        const float* sbp = nullptr;
+        bool fresh = true;
+        auto advance = [&](uint32_t by) {
+            for (uint32_t i = 0; i < by; ++i)
+                if (++kb == kb1) { kb = kb0; t += ncl; fresh = true; }
+        };
+        auto load = [&](ScaleRegs<TN>& r) {
+            if (fresh) {
+                tc = decode_tile<TN, CG>(g, first, ends, t, rank);
+                sbp = tc.m0 < g.m ? g.bs + tc.group * g.bs_gs + (uint64_t)(tc.m0 / 128) * g.b_lds : nullptr;
+                fresh = false;
+            }
+            r.sb = sbp ? __ldg(sbp + kb) : 0.0f;
+            const float* p = g.as + (uint64_t)kb * g.a_lds + tc.row0;
+#pragma unroll
+            for (uint32_t i = 0; i < sizeof(r.v) / 4; ++i) {
+                const uint32_t j = lane + 32 * i;
+                r.v[i] = j < TN && tc.row0 + j < tc.row1 ? __ldg(p + j) : 0.0f;
+            }
+        };
+        uint32_t item = warp - 2;
+        advance(item);
+        bool have[AHEAD];
+#pragma unroll
+        for (uint32_t p = 0; p < AHEAD; ++p) {
+            have[p] = t < total;
+            if (have[p]) { load(regs[p]); advance(2); }
+        }
+        bool ok = true;
+        while (ok && have[0]) {
+#pragma unroll
+            for (uint32_t p = 0; p < AHEAD; ++p) {
+                if (ok && have[p]) {
+                    const uint32_t slot = item % C::SLOTS, use = item / C::SLOTS;
+                    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sempty_b[slot]), (use & 1u) ^ 1u, wc));
+                    if (ok) {
+#pragma unroll
+                        for (uint32_t i = 0; i < sizeof(regs[p].v) / 4; ++i) {
+                            const uint32_t j = lane + 32 * i;
+                            if (j < TN) ring[slot * TN + j] = regs[p].v[i] * regs[p].sb;
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&sfull_b[slot]));
+                        item += 2;
+                        have[p] = t < total;
+                        if (have[p]) { load(regs[p]); advance(2); }
+                    }
+                }
+            }
+        }
+    } else {
+        const uint32_t quarter = warp & 3u, col0 = (warp - 4) / 4 * C::COLS;
+        uint32_t buf = 0, bphase = 0, slot = 0, sphase = 0;
+        bool ok = true;
+        const uint32_t acce0 = CG == 2 ? map_to_rank(smem_u32(&acce_b[0]), 0) : smem_u32(&acce_b[0]);
+        for (uint32_t t = cid; ok && t < total; t += ncl) {
+            const TileF8 tc = decode_tile<TN, CG>(g, first, ends, t, rank);
+            uint64_t acc[C::COLS / 2];
+#pragma unroll
+            for (int j = 0; j < C::COLS / 2; ++j) acc[j] = 0;      // two positive zeros
+            for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sfull_b[slot]), sphase, wc) &&
+                                                 mbar_wait(smem_u32(&accf_b[buf]), bphase, wc));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t d = tmem + buf * TN + col0 + (quarter << 21);
+                const float* sc = ring + slot * TN + col0;
+#pragma unroll
+                for (int c0 = 0; c0 < C::COLS; c0 += 16) {
+                    uint32_t r[16];
+                    tmem_ld16(d + c0, r);
+                    tmem_ld_done(r);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const ulonglong2 s2 = *reinterpret_cast<const ulonglong2*>(sc + c0 + j);
+                        acc[(c0 + j) / 2] = fma2(pack2(r[j], r[j + 1]), s2.x, acc[(c0 + j) / 2]);
+                        acc[(c0 + j) / 2 + 1] = fma2(pack2(r[j + 2], r[j + 3]), s2.y, acc[(c0 + j) / 2 + 1]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CG == 2) mbar_arrive_cluster(acce0 + 8 * buf);
+                    else mbar_arrive(smem_u32(&acce_b[buf]));
+                    mbar_arrive(smem_u32(&sempty_b[slot]));
+                }
+                if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
+                if (++slot == C::SLOTS) { slot = 0; sphase ^= 1; }
+            }
+            if (KS) {
+                // this CTA's part, [column][weight row], over the stages: their copies have landed and
+                // the MMAs that read them are complete (this tile is the CTA's only one)
+                float* part = (float*)smem + quarter * 32 + lane;
+#pragma unroll
+                for (int j = 0; j < C::COLS / 2; ++j) {
+                    float lo, hi;
+                    unpack2(acc[j], lo, hi);
+                    part[(col0 + 2 * j) * 128] = lo;
+                    part[(col0 + 2 * j + 1) * 128] = hi;
+                }
+            } else if (ok) {
+                const uint32_t mrow = tc.m0 + quarter * 32 + lane;
+                switch (g.c_type) {
+                    case CM_T_Q88: store_cols<int16_t, C::COLS>(g, tc, col0, mrow, acc); break;
+                    case CM_T_F32: store_cols<float, C::COLS>(g, tc, col0, mrow, acc); break;
+                    case CM_T_F16: store_cols<__half, C::COLS>(g, tc, col0, mrow, acc); break;
+                    default: store_cols<__nv_bfloat16, C::COLS>(g, tc, col0, mrow, acc); break;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (KS) {
+        __syncwarp();
+        cluster_sync_all();                 // every CTA's part is written
+        if (cid < total) {
+            const TileF8 tc = decode_tile<TN, CG>(g, first, ends, cid, rank);
+            const uint32_t lo = TN * crank / csize, hi = TN * (crank + 1) / csize;
+            const uint32_t base = smem_u32(smem);
+            for (uint32_t e = threadIdx.x; e < (hi - lo) * 128; e += C::THREADS) {
+                const uint32_t col = lo + e / 128, r = e % 128;
+                if (tc.row0 + col >= tc.row1 || tc.m0 + r >= g.m) continue;
+                float v = 0.0f;
+                for (uint32_t p = 0; p < csize; ++p) {
+                    float x;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(map_to_rank(base + (col * 128 + r) * 4, p)) : "memory");
+                    v += x;
+                }
+                store_one(g, (uint64_t)(tc.row0 + col) * g.ldc + tc.m0 + r, v);
+            }
+        }
+    }
+    // CTAs of a cluster use each other's shared memory and barriers until here
+    if (CG == 2 || KS) {
+        __syncwarp();
+        cluster_sync_all();
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        if (CG == 2)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");
+    }
+}
+
+// Rows of 8-bit values that do not start on 16-byte boundaries, copied to rows that do.  Each
+// thread makes 16 bytes from the five aligned words that hold them (words without a byte of the
+// row are not read).
+__global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* __restrict__ src, uint64_t ld, uint64_t gs, uint32_t rows,
+                                                         uint32_t cols, uint8_t* __restrict__ dst, uint64_t dst_ld, uint64_t total) {
+    griddep_wait();
+    const uint32_t chunks = (uint32_t)(dst_ld / 16);
+    for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (uint64_t)gridDim.x * 256) {
+        const uint64_t row = e / chunks;
+        const uint32_t c0 = (uint32_t)(e - row * chunks) * 16;
+        const uint64_t z = row / rows, r = row - z * rows;
+        const uint8_t* p = src + z * gs + r * ld + c0;
+        const uint32_t n = min(16u, cols - c0), shift = (uint32_t)((uintptr_t)p & 3u);
+        const uint32_t* w = (const uint32_t*)(p - shift);
+        uint32_t v[5];
+#pragma unroll
+        for (uint32_t i = 0; i < 5; ++i) v[i] = 4 * i < n + shift ? w[i] : 0u;
+        uint4 o;
+        o.x = __funnelshift_r(v[0], v[1], 8 * shift);
+        o.y = __funnelshift_r(v[1], v[2], 8 * shift);
+        o.z = __funnelshift_r(v[2], v[3], 8 * shift);
+        o.w = __funnelshift_r(v[3], v[4], 8 * shift);
+        *(uint4*)(dst + row * dst_ld + c0) = o;
+    }
+}
+
+// c = 0 (k = 0): the rows of the groups, or all of them.
+__global__ void __launch_bounds__(256) zero_rows_kernel(const KArgs g, uint64_t total) {
+    griddep_wait();
+    uint32_t lo = 0, hi = g.n;
+    if (g.offsets) {
+        // the running maximum ends at the largest offset; the first one opens the range
+        lo = (uint32_t)min(max(g.offsets[0], 0), (int)g.n);
+        hi = lo;
+        for (uint32_t i = 1; i <= g.groups; ++i) hi = max(hi, (uint32_t)min(max(g.offsets[i], 0), (int)g.n));
+    }
+    for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (uint64_t)gridDim.x * 256) {
+        const uint64_t row = e / g.m;
+        if (row >= lo && row < hi) store_one(g, row * g.ldc + (e - row * g.m), 0.0f);
+    }
+}
 
 int fp8_check(const char* who, const Fp8Args& g) {
     const unsigned size = type_size(g.c_type);
@@ -111,14 +599,152 @@ int fp8_check(const char* who, const Fp8Args& g) {
     return CM_OK;
 }
 
-int fp8_launch(const char* who, const Context* cx, const Fp8Args& g, cudaStream_t s) {
-    (void)cx;
-    const dim3 grid((g.m + ST - 1) / ST, (unsigned)(g.offsets ? (uint64_t)g.n / ST + g.groups : (g.n + ST - 1) / ST));
+int make_map(CUtensorMap* map, const uint8_t* base, uint32_t k, uint64_t ld, uint32_t rows, uint32_t groups, uint64_t gs, uint32_t box_rows,
+             uint32_t dims) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return set_error(CM_ECUDA, "cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t size[3] = {k, rows, groups};
+    const cuuint64_t strides[2] = {ld, gs};
+    const cuuint32_t box[3] = {128, box_rows, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, dims, (void*)base, size, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? CM_OK : set_error(CM_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+}
+
+// Clusters of `size` CTAs of this kernel that the GPU holds at once.
+template <int TN, int CG, bool KS>
+int resident_clusters(const Context* cx, uint32_t size, int* out) {
+    static int known[16][9] = {};        // by device and size (function attributes are a device's own)
+    const int dev = cx->device < 16 ? cx->device : 15;
+    if (!known[dev][size] || dev == 15) {
+        const auto kern = gemm_f8_kernel<TN, CG, KS>;
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F8Cfg<TN, CG>::SMEM);
+        if (e != cudaSuccess) return cuda_error(e, "cudaFuncSetAttribute(gemm_f8)");
+        int n = cx->sm_count / (int)size;
+        if (size > 1) {
+            cudaLaunchConfig_t q{};
+            q.gridDim = dim3(size * n);
+            q.blockDim = dim3(F8Cfg<TN, CG>::THREADS);
+            q.dynamicSmemBytes = F8Cfg<TN, CG>::SMEM;
+            cudaLaunchAttribute at{};
+            at.id = cudaLaunchAttributeClusterDimension;
+            at.val.clusterDim.x = size; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+            q.attrs = &at; q.numAttrs = 1;
+            int r = 0;
+            if (cudaOccupancyMaxActiveClusters(&r, kern, &q) == cudaSuccess && r > 0) n = std::min(n, r);
+            cudaGetLastError();
+        }
+        known[dev][size] = n;
+    }
+    *out = known[dev][size];
+    return CM_OK;
+}
+
+template <int TN, int CG, bool KS>
+int launch_tiles(const Context* cx, const CUtensorMap& tw, const CUtensorMap& tt, const KArgs& g, uint32_t size, uint64_t most, cudaStream_t s) {
+    int resident = 0;
+    int rc = resident_clusters<TN, CG, KS>(cx, size, &resident);
+    if (rc) return rc;
+    const unsigned clusters = (unsigned)std::min<uint64_t>(most, KS ? most : (uint64_t)resident);
+    cudaLaunchConfig_t q{};
+    q.gridDim = dim3(size * clusters);
+    q.blockDim = dim3(F8Cfg<TN, CG>::THREADS);
+    q.dynamicSmemBytes = F8Cfg<TN, CG>::SMEM;
+    q.stream = s;
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = g_pdl ? 1 : 0;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = size; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    q.attrs = at; q.numAttrs = size > 1 ? 2 : 1;
+    cudaError_t e;
     {
         ProfScope ps_(PK_FP8_GEMM, s);
-        launch_k(fp8_simple_kernel, grid, 256, 0, s, g);
+        e = cudaLaunchKernelEx(&q, gemm_f8_kernel<TN, CG, KS>, tw, tt, g);
     }
     count_launch();
+    return e == cudaSuccess ? CM_OK : cuda_error(e, "gemm_f8 launch");
+}
+
+template <int TN, int CG>
+int run_tiles(const Context* cx, const uint8_t* a, uint64_t lda, const uint8_t* b, uint64_t ldb, uint64_t b_gs, const Fp8Args& f, KArgs g,
+              cudaStream_t s) {
+    g.tiles_m = (f.m + 128 * CG - 1) / (128 * CG);
+    g.tiles_t = (f.n + TN - 1) / TN;
+    // a group's last tile may be partial, so grouped rows make at most n / TN + groups tiles
+    const uint64_t token_tiles = f.offsets ? std::min<uint64_t>((uint64_t)f.n / TN + f.groups, f.n) : g.tiles_t;
+    const uint64_t most = token_tiles * g.tiles_m;
+    if (most >= (1ull << 31)) return set_error(CM_EUNSUPPORTED, "cm_matmul_fp8: more than 2^31 tiles");
+    g.total = (uint32_t)most;
+    g.fd_m = FastDiv(g.tiles_m);
+    // D fp32; A = weights, B = tokens, both K-major; M = 128 a CTA, N = TN
+    g.idesc = (1u << 4) | (f.b_format << 7) | (f.a_format << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(CG * 128 >> 4) << 24);
+    const uint32_t stored_groups = f.offsets && b_gs ? f.groups : 1u;
+    g.group_step = stored_groups > 1 ? 1u : 0u;
+    CUtensorMap tw, tt;
+    int rc = make_map(&tw, b, f.k, ldb, f.m, stored_groups, stored_groups > 1 ? b_gs : (uint64_t)f.m * ldb, 128, 3);
+    if (!rc) rc = make_map(&tt, a, f.k, lda, f.n, 1, 0, TN / CG, 2);
+    if (rc) return rc;
+    if constexpr (CG == 1) {
+        // few tiles: the largest cluster whose CTAs each take at least one K block of one tile and
+        // are all resident
+        for (uint32_t size = 8; size >= 2; size /= 2) {
+            int resident = 0;
+            if (size > g.kb || most * size > (uint64_t)cx->sm_count) continue;
+            rc = resident_clusters<TN, CG, true>(cx, size, &resident);
+            if (rc) return rc;
+            if (most <= (uint64_t)resident) return launch_tiles<TN, CG, true>(cx, tw, tt, g, size, most, s);
+        }
+    }
+    return launch_tiles<TN, CG, false>(cx, tw, tt, g, CG, most, s);
+}
+
+int fp8_launch(const char* who, const Context* cx, const Fp8Args& f, cudaStream_t s) {
+    KArgs g{};
+    g.as = f.as; g.bs = f.bs; g.c = f.c; g.offsets = f.offsets;
+    g.a_lds = f.a_lds; g.b_lds = f.b_lds; g.bs_gs = f.bs_gs; g.ldc = f.ldc;
+    g.groups = f.groups; g.n = f.n; g.m = f.m; g.c_type = f.c_type;
+    g.kb = (f.k + 127) / 128; g.ksteps = (f.k + 31) / 32;
+    g.status = cx->status; g.timeout_ns = cx->timeout_ns;
+    if (f.k == 0) {
+        const uint64_t total = (uint64_t)f.n * f.m;
+        launch_k(zero_rows_kernel, grid_for(cx, total, 256, 8), 256, 0, s, g, total);
+        count_launch();
+        cudaError_t e = cudaGetLastError();
+        return e == cudaSuccess ? CM_OK : cuda_error(e, who);
+    }
+    // TMA reads rows that start on 16-byte boundaries (pitches below 2^40); others are copied first
+    const uint64_t k16 = (f.k + 15ull) & ~15ull;
+    const uint64_t lda = f.n > 1 ? f.lda : k16, ldb = f.m > 1 ? f.ldb : k16;
+    const bool one = !f.offsets || f.groups == 1 || f.b_gs == 0;
+    const bool a_ok = (uintptr_t)f.a % 16 == 0 && lda % 16 == 0 && lda < (1ull << 40);
+    const bool b_ok = (uintptr_t)f.b % 16 == 0 && ldb % 16 == 0 && ldb < (1ull << 40) && (one || (f.b_gs % 16 == 0 && f.b_gs < (1ull << 40)));
+    const uint64_t b_count = one ? 1 : f.groups;
+    const uint64_t a_bytes = a_ok ? 0 : f.n * k16, b_bytes = b_ok ? 0 : b_count * f.m * k16;
+    uint8_t* scratch = nullptr;
+    int rc = scratch_alloc((void**)&scratch, a_bytes + b_bytes, s);
+    if (rc) return rc;
+    auto align_rows = [&](const uint8_t* src, uint64_t ld, uint64_t gs, uint32_t rows, uint64_t count, uint8_t* dst) {
+        const uint64_t total = count * rows * (k16 / 16);
+        ProfScope ps_(PK_FP8_QUANT, s);
+        launch_k(align_rows_kernel, grid_for(cx, total, 256, 8), 256, 0, s, src, ld, gs, rows, f.k, dst, k16, total);
+        count_launch();
+    };
+    if (a_bytes) align_rows(f.a, lda, 0, f.n, 1, scratch);
+    if (b_bytes) align_rows(f.b, ldb, one ? 0 : f.b_gs, f.m, b_count, scratch + a_bytes);
+    const uint8_t* a = a_bytes ? scratch : f.a;
+    const uint8_t* b = b_bytes ? scratch + a_bytes : f.b;
+    const uint64_t pa = a_bytes ? k16 : lda, pb = b_bytes ? k16 : ldb, gsb = one ? 0 : b_bytes ? f.m * k16 : f.b_gs;
+    // rows a weight tile meets at once: the smallest tile that holds a group's (mean) rows
+    const uint64_t rows = f.offsets ? (f.n + (uint64_t)f.groups - 1) / f.groups : f.n;
+    if (rows <= 16) rc = run_tiles<16, 1>(cx, a, pa, b, pb, gsb, f, g, s);
+    else if (rows <= 32) rc = run_tiles<32, 1>(cx, a, pa, b, pb, gsb, f, g, s);
+    else if (rows <= 64) rc = run_tiles<64, 1>(cx, a, pa, b, pb, gsb, f, g, s);
+    else if (rows <= 128) rc = run_tiles<128, 1>(cx, a, pa, b, pb, gsb, f, g, s);
+    else rc = run_tiles<256, 2>(cx, a, pa, b, pb, gsb, f, g, s);
+    scratch_free(scratch, s);
+    if (rc) return rc;
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? CM_OK : cuda_error(e, who);
 }
