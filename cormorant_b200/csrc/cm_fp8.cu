@@ -2,11 +2,15 @@
 // output of an RMS norm with the residual's addition (cm_rmsnorm_fp8).
 //
 // Both are HBM-bound: every input is read once and every output written once, all arithmetic in
-// fp32 registers.  A row's 128-column block is the work of 16 neighbouring lanes of 8 values each
-// (one 16-byte load of a 2-byte type), so the block's maximum is four shuffles inside a half warp
-// and the 8-bit values leave as one 8-byte store a lane.  Rows whose pitch or base is not a
-// multiple of those sizes run the same kernel with one-element accesses in which 16 neighbouring
-// lanes touch 16 neighbouring elements.
+// fp32 registers.  What stands in the way of the bandwidth is the issue rate, so the work that a
+// block needs once (the reduction of its maximum, the divisions) is spread over as few lanes as
+// the loads allow: a row's 128-column block belongs to 4 neighbouring lanes of 32 values each.
+// Chunk i of lane l is the 8 columns from 8 * (4 * i + l): the 4 lanes of a block read 64
+// neighbouring bytes of a 2-byte type with one load and write one 32-byte sector with one store;
+// the maximum is two shuffles, and of the two quotients lane 0 takes A / F and the others F / A.
+// (With 16 lanes a block and 8 values each, 8192 x 4096 bf16 took 30.9 us instead of 20.3.)
+// Rows whose pitch or base is not a multiple of the vector sizes run the same kernel with
+// one-element accesses, column l + 4 * j of the block.
 #include <cmath>
 
 #include "cm_fp8.cuh"
@@ -14,79 +18,120 @@
 namespace cm {
 namespace {
 
-// ---- eight values of a 128-column block held by lane l (0..15) of a half warp ------------------
-// VEC: columns col0 + 8*l .. +7;  else columns col0 + l + 16*j, j < 8.
-template <typename T>
-__device__ __forceinline__ void unpack8(const uint4 (&w)[sizeof(T) / 2], float (&v)[8]) {
-    const T* t = reinterpret_cast<const T*>(w);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f32(t[j]);
-}
+constexpr uint32_t kLanes = 4;                       // lanes of a block
+constexpr uint32_t kVals = kFp8Block / kLanes;       // values of a lane
+constexpr uint32_t kChunks = kVals / 8;
 
 template <bool VEC>
 __device__ __forceinline__ uint32_t column(uint32_t col0, uint32_t l, uint32_t j) {
-    return VEC ? col0 + 8 * l + j : col0 + l + 16 * j;
+    return VEC ? col0 + 8 * (kLanes * (j / 8) + l) + j % 8 : col0 + l + kLanes * j;
 }
 
+// 32 values of a lane, 0 past the row's end
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, uint32_t col0, uint32_t l, uint32_t cols, float (&v)[8]) {
-    if (VEC && col0 + 8 * l + 8 <= cols) {
-        uint4 w[sizeof(T) / 2];
+__device__ __forceinline__ void load32(const T* row, uint32_t col0, uint32_t l, uint32_t cols, float (&v)[kVals]) {
+    if (VEC && col0 + kFp8Block <= cols) {
+        uint4 w[kChunks][sizeof(T) / 2];
 #pragma unroll
-        for (uint32_t i = 0; i < sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(row + col0 + 8 * l)[i];
-        unpack8<T>(w, v);
+        for (uint32_t i = 0; i < kChunks; ++i)
+#pragma unroll
+            for (uint32_t k = 0; k < sizeof(T) / 2; ++k)
+                w[i][k] = reinterpret_cast<const uint4*>(row + col0 + 8 * (kLanes * i + l))[k];
+#pragma unroll
+        for (uint32_t i = 0; i < kChunks; ++i) {
+            const T* t = reinterpret_cast<const T*>(w[i]);
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) v[8 * i + j] = to_f32(t[j]);
+        }
         return;
     }
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-        const uint32_t c = column<VEC>(col0, l, j);
-        v[j] = c < cols ? to_f32(row[c]) : 0.0f;
+    for (uint32_t i = 0; i < kChunks; ++i) {
+        if (VEC && column<VEC>(col0, l, 8 * i) + 8 <= cols) {    // a whole chunk of the last, partial block
+            uint4 w[sizeof(T) / 2];
+#pragma unroll
+            for (uint32_t k = 0; k < sizeof(T) / 2; ++k) w[k] = reinterpret_cast<const uint4*>(row + column<VEC>(col0, l, 8 * i))[k];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) v[8 * i + j] = to_f32(reinterpret_cast<const T*>(w)[j]);
+            continue;
+        }
+#pragma unroll
+        for (uint32_t j = 8 * i; j < 8 * i + 8; ++j) {
+            const uint32_t c = column<VEC>(col0, l, j);
+            v[j] = c < cols ? to_f32(row[c]) : 0.0f;
+        }
     }
 }
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* row, uint32_t col0, uint32_t l, uint32_t cols, const float (&v)[8]) {
-    if (VEC && col0 + 8 * l + 8 <= cols) {
-        uint4 w[sizeof(T) / 2];
-        T* t = reinterpret_cast<T*>(w);
+__device__ __forceinline__ void store32(T* row, uint32_t col0, uint32_t l, uint32_t cols, const float (&v)[kVals]) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) from_f32(v[j], t[j]);
+    for (uint32_t i = 0; i < kChunks; ++i) {
+        if (VEC && column<VEC>(col0, l, 8 * i) + 8 <= cols) {
+            uint4 w[sizeof(T) / 2];
+            T* t = reinterpret_cast<T*>(w);
 #pragma unroll
-        for (uint32_t i = 0; i < sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(row + col0 + 8 * l)[i] = w[i];
-        return;
-    }
+            for (uint32_t j = 0; j < 8; ++j) from_f32(v[8 * i + j], t[j]);
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-        const uint32_t c = column<VEC>(col0, l, j);
-        if (c < cols) from_f32(v[j], row[c]);
+            for (uint32_t k = 0; k < sizeof(T) / 2; ++k) reinterpret_cast<uint4*>(row + column<VEC>(col0, l, 8 * i))[k] = w[k];
+            continue;
+        }
+#pragma unroll
+        for (uint32_t j = 8 * i; j < 8 * i + 8; ++j) {
+            const uint32_t c = column<VEC>(col0, l, j);
+            if (c < cols) from_f32(v[j], row[c]);
+        }
     }
 }
 
-// Bits of the largest magnitude: IEEE magnitudes order as integers, infinities above every finite
-// value and NaN above infinity, so a NaN of the block reaches its scale.
-__device__ __forceinline__ uint32_t max_bits(const float (&v)[8], uint32_t m) {
+// max(|v|) and a floor; a NaN among them is the result, so that it reaches the block's scale
+__device__ __forceinline__ float max_abs(const float (&v)[kVals], float m) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+    for (uint32_t j = 0; j < kVals; j += 2)
+        asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v[j]), "f"(v[j + 1]));
+    return m;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
     return m;
 }
 
-constexpr uint32_t kTinyBits = (127u - 100u) << 23;   // 2^-100
+constexpr float kTiny = 7.888609052210118e-31f;   // 2^-100
 
 template <bool VEC>
-__device__ __forceinline__ void store_q8(uint8_t* row, uint32_t col0, uint32_t l, uint32_t cols, uint32_t format,
-                                         float inv, const float (&v)[8]) {
-    uint32_t p[4];
+__device__ __forceinline__ void store_q32(uint8_t* row, uint32_t col0, uint32_t l, uint32_t cols, uint32_t format, float inv,
+                                          const float (&v)[kVals]) {
+    uint32_t p[kVals / 2];
+    if (format == CM_F8_E4M3) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = cvt_fp8x2(format, v[2 * j] * inv, v[2 * j + 1] * inv);
-    if (VEC && col0 + 8 * l + 8 <= cols) {
-        *reinterpret_cast<uint2*>(row + col0 + 8 * l) = make_uint2(p[0] | (p[1] << 16), p[2] | (p[3] << 16));
-        return;
+        for (uint32_t j = 0; j < kVals / 2; ++j) p[j] = cvt_fp8x2(CM_F8_E4M3, v[2 * j] * inv, v[2 * j + 1] * inv);
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < kVals / 2; ++j) p[j] = cvt_fp8x2(CM_F8_E5M2, v[2 * j] * inv, v[2 * j + 1] * inv);
     }
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-        const uint32_t c = column<VEC>(col0, l, j);
-        if (c < cols) row[c] = (uint8_t)(p[j / 2] >> (8 * (j & 1)));
+    for (uint32_t i = 0; i < kChunks; ++i) {
+        if (VEC && column<VEC>(col0, l, 8 * i) + 8 <= cols) {
+            *reinterpret_cast<uint2*>(row + column<VEC>(col0, l, 8 * i)) =
+                make_uint2(p[4 * i] | (p[4 * i + 1] << 16), p[4 * i + 2] | (p[4 * i + 3] << 16));
+            continue;
+        }
+#pragma unroll
+        for (uint32_t j = 8 * i; j < 8 * i + 8; ++j) {
+            const uint32_t c = column<VEC>(col0, l, j);
+            if (c < cols) row[c] = (uint8_t)(p[j / 2] >> (8 * (j & 1)));
+        }
     }
+}
+
+// From a lane's max(|v|): F / A of its block in every lane, and A / F in lane 0.
+__device__ __forceinline__ float block_scale(float m, uint32_t l, float F, float& scale) {
+#pragma unroll
+    for (uint32_t o = kLanes / 2; o; o /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float r = (l == 0 ? m : F) / (l == 0 ? F : m);
+    scale = r;
+    return __shfl_sync(0xffffffffu, r, 1, kLanes);
 }
 
 // ---- cm_quant_fp8, one scale per row and 128 columns -------------------------------------------
@@ -99,82 +144,60 @@ struct QuantArgs {
     uint32_t row_tiles, col_tiles;   // tiles per matrix
 };
 
-// A CTA takes 8 rows x 4 column blocks: each row piece is 1 KB of a 2-byte type (whole DRAM
-// bursts), and the 8 scales of a column block, which lie side by side, fill one 32-byte sector.
-constexpr uint32_t kQRows = 8, kQCols = 4;
+// A warp takes 8 rows of a column block -- their scales lie side by side and fill one 32-byte
+// sector --, a CTA 8 rows x 8 column blocks, 2 KB of a row of a 2-byte type.
+constexpr uint32_t kQRows = 8, kQCols = 8;
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quant_rows_kernel(QuantArgs g) {
     griddep_wait();
     const uint32_t ct = blockIdx.x % g.col_tiles, rest = blockIdx.x / g.col_tiles;
     const uint32_t rt = rest % g.row_tiles, z = rest / g.row_tiles;
-    const uint32_t hw = threadIdx.x / 16, l = threadIdx.x % 16;
-    const T* x = (const T*)g.x + (uint64_t)z * g.x_bs;
-    constexpr uint32_t N = kQRows * kQCols / 16;
-    float v[N][8];
-    uint32_t row[N], cb[N];
+    const uint32_t lane = threadIdx.x % 32, l = lane % kLanes;
+    const uint32_t row = rt * kQRows + lane / kLanes, cb = ct * kQCols + threadIdx.x / 32, col0 = cb * kFp8Block;
+    if (col0 >= g.cols) return;                        // the whole warp
+    const bool live = row < g.rows;
+    float v[kVals];
+    if (live) {
+        load32<T, VEC>((const T*)g.x + (uint64_t)z * g.x_bs + row * g.ldx, col0, l, g.cols, v);
+    } else {
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) {
-        const uint32_t item = hw + 16 * i;
-        row[i] = rt * kQRows + item / kQCols;
-        cb[i] = ct * kQCols + item % kQCols;
-        if (row[i] < g.rows && cb[i] * kFp8Block < g.cols) {
-            load8<T, VEC>(x + row[i] * g.ldx, cb[i] * kFp8Block, l, g.cols, v[i]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-        }
+        for (uint32_t j = 0; j < kVals; ++j) v[j] = 0.0f;
     }
-    const float F = fp8_largest(g.format);
-#pragma unroll
-    for (uint32_t i = 0; i < N; ++i) {
-        uint32_t m = max_bits(v[i], kTinyBits);
-#pragma unroll
-        for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (row[i] >= g.rows || cb[i] * kFp8Block >= g.cols) continue;
-        const float A = __uint_as_float(m);
-        store_q8<VEC>(g.q + (uint64_t)z * g.q_bs + row[i] * g.ldq, cb[i] * kFp8Block, l, g.cols, g.format, F / A, v[i]);
-        if (l == 0) g.scale[(uint64_t)z * g.s_bs + cb[i] * g.lds + row[i]] = A / F;
-    }
+    float scale;
+    const float inv = block_scale(max_abs(v, kTiny), l, fp8_largest(g.format), scale);
+    if (!live) return;
+    store_q32<VEC>(g.q + (uint64_t)z * g.q_bs + row * g.ldq, col0, l, g.cols, g.format, inv, v);
+    if (l == 0) g.scale[(uint64_t)z * g.s_bs + cb * g.lds + row] = scale;
 }
 
 // ---- cm_quant_fp8, one scale per 128 x 128 block -----------------------------------------------
-// A CTA holds its whole block in registers (64 values a thread), so it is read once.
+// A CTA of 512 threads holds its whole block in registers (32 values a thread), so it is read once.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) quant_blocks_kernel(QuantArgs g) {
+__global__ void __launch_bounds__(512) quant_blocks_kernel(QuantArgs g) {
     griddep_wait();
-    __shared__ uint32_t top[8];
+    __shared__ float top[16];
     const uint32_t cb = blockIdx.x % g.col_tiles, rest = blockIdx.x / g.col_tiles;
     const uint32_t rb = rest % g.row_tiles, z = rest / g.row_tiles;
-    const uint32_t hw = threadIdx.x / 16, l = threadIdx.x % 16;
-    const T* x = (const T*)g.x + (uint64_t)z * g.x_bs;
-    float v[8][8];
-    uint32_t m = kTinyBits;
+    const uint32_t l = threadIdx.x % kLanes, row = rb * kFp8Block + threadIdx.x / kLanes, col0 = cb * kFp8Block;
+    const bool live = row < g.rows;
+    float v[kVals];
+    if (live) {
+        load32<T, VEC>((const T*)g.x + (uint64_t)z * g.x_bs + row * g.ldx, col0, l, g.cols, v);
+    } else {
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        const uint32_t row = rb * kFp8Block + hw + 16 * i;
-        if (row < g.rows) {
-            load8<T, VEC>(x + row * g.ldx, cb * kFp8Block, l, g.cols, v[i]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-        }
+        for (uint32_t j = 0; j < kVals; ++j) v[j] = 0.0f;
     }
+    float m = max_abs(v, kTiny);
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) m = max_bits(v[i], m);
-    m = __reduce_max_sync(0xffffffffu, m);
+    for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = m;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) m = max(m, top[w]);
-    const float F = fp8_largest(g.format), A = __uint_as_float(m), inv = F / A;
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        const uint32_t row = rb * kFp8Block + hw + 16 * i;
-        if (row < g.rows)
-            store_q8<VEC>(g.q + (uint64_t)z * g.q_bs + row * g.ldq, cb * kFp8Block, l, g.cols, g.format, inv, v[i]);
-    }
-    if (threadIdx.x == 0) g.scale[(uint64_t)z * g.s_bs + rb * g.lds + cb] = A / F;
+    for (int w = 0; w < 16; ++w) m = max_nan(m, top[w]);
+    const float F = fp8_largest(g.format);
+    if (live) store_q32<VEC>(g.q + (uint64_t)z * g.q_bs + row * g.ldq, col0, l, g.cols, g.format, F / m, v);
+    if (threadIdx.x == 0) g.scale[(uint64_t)z * g.s_bs + rb * g.lds + cb] = m / F;
 }
 
 // ---- cm_rmsnorm_fp8 ----------------------------------------------------------------------------
@@ -195,54 +218,40 @@ struct NormArgs {
 };
 
 template <bool VEC>
-__device__ __forceinline__ void load_weight8(const void* w, uint32_t type, uint32_t col0, uint32_t l, uint32_t cols, float (&v)[8]) {
-    if (type == CM_T_F32) load8<float, VEC>((const float*)w, col0, l, cols, v);
-    else if (type == CM_T_F16) load8<__half, VEC>((const __half*)w, col0, l, cols, v);
-    else load8<__nv_bfloat16, VEC>((const __nv_bfloat16*)w, col0, l, cols, v);
+__device__ __forceinline__ void load_weight(const void* w, uint32_t type, uint32_t col0, uint32_t l, uint32_t cols, float (&v)[kVals]) {
+    if (type == CM_T_F32) load32<float, VEC>((const float*)w, col0, l, cols, v);
+    else if (type == CM_T_F16) load32<__half, VEC>((const __half*)w, col0, l, cols, v);
+    else load32<__nv_bfloat16, VEC>((const __nv_bfloat16*)w, col0, l, cols, v);
 }
 
-// G threads share a row, which stays in their registers: at most NI chunks of 8 values each.
-constexpr uint32_t kNormChunks = 4;
-
+// G threads share a row, which stays in their registers, a block to 4 of them.
 template <typename T, uint32_t G, bool VEC>
 __global__ void __launch_bounds__(G < 128 ? 128 : G) rmsnorm_kernel(NormArgs g) {
     griddep_wait();
-    constexpr uint32_t NI = kNormChunks, ROWS = G < 128 ? 128 / G : 1;
+    constexpr uint32_t ROWS = G < 128 ? 128 / G : 1;
     __shared__ float part[32];
-    const uint32_t t = threadIdx.x % G;
+    const uint32_t t = threadIdx.x % G, l = t % kLanes, blk = t / kLanes, col0 = blk * kFp8Block;
     const uint32_t row = blockIdx.x * ROWS + threadIdx.x / G;
-    const bool live = row < g.rows;
-    const uint32_t l = t % 16;
-    const uint64_t r = live ? row : 0;
-    float h[NI][8];
+    const bool in = row < g.rows && col0 < g.cols;
+    const uint64_t r = row;
+    float h[kVals];
 #pragma unroll
-    for (uint32_t i = 0; i < NI; ++i) {
-        const uint32_t col0 = (t / 16 + i * (G / 16)) * kFp8Block;
-        if (live && col0 < g.cols) {
-            load8<T, VEC>((const T*)g.x + r * g.ldx, col0, l, g.cols, h[i]);
-        } else {
+    for (uint32_t j = 0; j < kVals; ++j) h[j] = 0.0f;
+    if (in) {
+        load32<T, VEC>((const T*)g.x + r * g.ldx, col0, l, g.cols, h);
+        if (g.resid) {
+            float v[kVals];
+            load32<T, VEC>((const T*)g.resid + r * g.ldr, col0, l, g.cols, v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] = 0.0f;
-        }
-    }
-    if (g.resid) {
-#pragma unroll
-        for (uint32_t i = 0; i < NI; ++i) {
-            const uint32_t col0 = (t / 16 + i * (G / 16)) * kFp8Block;
-            if (!live || col0 >= g.cols) continue;
-            float v[8];
-            load8<T, VEC>((const T*)g.resid + r * g.ldr, col0, l, g.cols, v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] += v[j];
+            for (uint32_t j = 0; j < kVals; ++j) h[j] += v[j];
         }
     }
     float ss = 0.0f;
+    {
+        float s[4] = {};
 #pragma unroll
-    for (uint32_t i = 0; i < NI; ++i) {
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s = fmaf(h[i][j], h[i][j], s);
-        ss += s;
+        for (uint32_t j = 0; j < kVals; ++j) s[j % 4] = fmaf(h[j], h[j], s[j % 4]);
+        ss = (s[0] + s[1]) + (s[2] + s[3]);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -254,36 +263,27 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) rmsnorm_kernel(NormArgs g) 
         for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     }
     const float rms = 1.0f / sqrtf(ss / (float)g.cols + g.eps);
-    const float F = fp8_largest(g.format);
+    if (in && g.resid_out) store32<T, VEC>((T*)g.resid_out + r * g.ldo, col0, l, g.cols, h);
 #pragma unroll
-    for (uint32_t i = 0; i < NI; ++i) {
-        const uint32_t blk = t / 16 + i * (G / 16), col0 = blk * kFp8Block;
-        const bool in = live && col0 < g.cols;
-        if (in && g.resid_out) store8<T, VEC>((T*)g.resid_out + r * g.ldo, col0, l, g.cols, h[i]);
-        float y[8];
+    for (uint32_t j = 0; j < kVals; ++j) h[j] *= rms;
+    if (in && g.weight) {
+        float w[kVals];
+        load_weight<VEC>(g.weight, g.weight_type, col0, l, g.cols, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = h[i][j] * rms;
-        if (in && g.weight) {
-            float w[8];
-            load_weight8<VEC>(g.weight, g.weight_type, col0, l, g.cols, w);
+        for (uint32_t j = 0; j < kVals; ++j) h[j] *= w[j];
+    }
+    if (in && g.y) store32<T, VEC>((T*)g.y + r * g.ldy, col0, l, g.cols, h);
+    if (g.q) {
+        if (col0 + kFp8Block > g.cols) {   // columns past the row's end hold no value (an infinite rms would make 0 * inf of them)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] *= w[j];
+            for (uint32_t j = 0; j < kVals; ++j)
+                if (column<VEC>(col0, l, j) >= g.cols) h[j] = 0.0f;
         }
-        if (in && g.y) store8<T, VEC>((T*)g.y + r * g.ldy, col0, l, g.cols, y);
-        if (g.q) {
-            if (!VEC || col0 + 8 * l + 8 > g.cols) {   // columns past the row's end hold no value (an infinite rms would make 0 * inf of them)
-#pragma unroll
-                for (uint32_t j = 0; j < 8; ++j)
-                    if (column<VEC>(col0, l, j) >= g.cols) y[j] = 0.0f;
-            }
-            uint32_t m = max_bits(y, kTinyBits);
-#pragma unroll
-            for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            if (in) {
-                const float A = __uint_as_float(m);
-                store_q8<VEC>(g.q + r * g.ldq, col0, l, g.cols, g.format, F / A, y);
-                if (l == 0) g.scale[blk * g.lds + r] = A / F;
-            }
+        float scale;
+        const float inv = block_scale(max_abs(h, kTiny), l, fp8_largest(g.format), scale);
+        if (in) {
+            store_q32<VEC>(g.q + r * g.ldq, col0, l, g.cols, g.format, inv, h);
+            if (l == 0) g.scale[blk * g.lds + r] = scale;
         }
     }
 }
@@ -295,7 +295,7 @@ template <bool VEC>
 void launch_quant(const QuantArgs& g, unsigned type, bool blocks, unsigned grid, cudaStream_t s) {
 #define CM_QUANT(T)                                                        \
     do {                                                                   \
-        if (blocks) launch_k(quant_blocks_kernel<T, VEC>, grid, 256, 0, s, g); \
+        if (blocks) launch_k(quant_blocks_kernel<T, VEC>, grid, 512, 0, s, g); \
         else launch_k(quant_rows_kernel<T, VEC>, grid, 256, 0, s, g);      \
     } while (0)
     switch (type) {
@@ -308,28 +308,25 @@ void launch_quant(const QuantArgs& g, unsigned type, bool blocks, unsigned grid,
 }
 
 template <typename T, bool VEC>
-void launch_norm(const Context* cx, const NormArgs& g, cudaStream_t s) {
-    // Threads a row: enough for the row to fit their registers (32 values each); rows that do not
-    // fill the GPU take one chunk a thread instead, so that a row's loads are all in flight at once.
-    const bool few = (uint64_t)g.rows < 4ull * cx->sm_count;
-    const uint32_t need = (g.cols + 7) / 8;             // chunks of 8 values
-    const uint32_t fit = few ? need : (need + kNormChunks - 1) / kNormChunks;
-    if (fit <= 32 && need <= 32 * kNormChunks) launch_k(rmsnorm_kernel<T, 32, VEC>, (g.rows + 3) / 4, 128, 0, s, g);
-    else if (fit <= 128 && need <= 128 * kNormChunks) launch_k(rmsnorm_kernel<T, 128, VEC>, g.rows, 128, 0, s, g);
-    else if (fit <= 512 && need <= 512 * kNormChunks) launch_k(rmsnorm_kernel<T, 512, VEC>, g.rows, 512, 0, s, g);
+void launch_norm(const NormArgs& g, cudaStream_t s) {
+    // threads a row: the fewest that hold it (32 values each)
+    if (g.cols <= 32 * kVals) launch_k(rmsnorm_kernel<T, 32, VEC>, (g.rows + 3) / 4, 128, 0, s, g);
+    else if (g.cols <= 128 * kVals) launch_k(rmsnorm_kernel<T, 128, VEC>, g.rows, 128, 0, s, g);
+    else if (g.cols <= 256 * kVals) launch_k(rmsnorm_kernel<T, 256, VEC>, g.rows, 256, 0, s, g);
+    else if (g.cols <= 512 * kVals) launch_k(rmsnorm_kernel<T, 512, VEC>, g.rows, 512, 0, s, g);
     else launch_k(rmsnorm_kernel<T, 1024, VEC>, g.rows, 1024, 0, s, g);
 }
 
 template <bool VEC>
-void launch_norm_type(const Context* cx, const NormArgs& g, unsigned type, cudaStream_t s) {
+void launch_norm_type(const NormArgs& g, unsigned type, cudaStream_t s) {
     switch (type) {
-        case CM_T_F32: launch_norm<float, VEC>(cx, g, s); break;
-        case CM_T_F16: launch_norm<__half, VEC>(cx, g, s); break;
-        default: launch_norm<__nv_bfloat16, VEC>(cx, g, s); break;
+        case CM_T_F32: launch_norm<float, VEC>(g, s); break;
+        case CM_T_F16: launch_norm<__half, VEC>(g, s); break;
+        default: launch_norm<__nv_bfloat16, VEC>(g, s); break;
     }
 }
 
-constexpr uint32_t kNormMaxCols = 1024 * 8 * kNormChunks;
+constexpr uint32_t kNormMaxCols = 1024 * kVals;
 
 }  // namespace
 }  // namespace cm
@@ -426,8 +423,8 @@ extern "C" int cm_rmsnorm_fp8_async(const void* x, const void* resid, const void
                      (!q || aligned(q, ldq, 8)) && (!weight || aligned(weight, 0, 16));
     {
         ProfScope ps_(PK_FP8_QUANT, s);
-        if (vec) launch_norm_type<true>(cx, g, type, s);
-        else launch_norm_type<false>(cx, g, type, s);
+        if (vec) launch_norm_type<true>(g, type, s);
+        else launch_norm_type<false>(g, type, s);
     }
     count_launch();
     cudaError_t e = cudaGetLastError();
