@@ -9,8 +9,11 @@
 // neighbouring bytes of a 2-byte type with one load and write one 32-byte sector with one store;
 // the maximum is two shuffles, and of the two quotients lane 0 takes A / F and the others F / A.
 // (With 16 lanes a block and 8 values each, 8192 x 4096 bf16 took 30.9 us instead of 20.3.)
+// Values stay in their own type until they are needed, fp32 works on pairs, and the next rows'
+// loads are issued before the current rows are worked on.
 // Rows whose pitch or base is not a multiple of the vector sizes run the same kernel with
 // one-element accesses, column l + 4 * j of the block.
+#include <algorithm>
 #include <cmath>
 
 #include "cm_fp8.cuh"
@@ -22,113 +25,190 @@ constexpr uint32_t kLanes = 4;                       // lanes of a block
 constexpr uint32_t kVals = kFp8Block / kLanes;       // values of a lane
 constexpr uint32_t kChunks = kVals / 8;
 
+// column of a lane's value j
 template <bool VEC>
 __device__ __forceinline__ uint32_t column(uint32_t col0, uint32_t l, uint32_t j) {
     return VEC ? col0 + 8 * (kLanes * (j / 8) + l) + j % 8 : col0 + l + kLanes * j;
 }
 
-// 32 values of a lane, 0 past the row's end
-template <typename T, bool VEC>
-__device__ __forceinline__ void load32(const T* row, uint32_t col0, uint32_t l, uint32_t cols, float (&v)[kVals]) {
-    if (VEC && col0 + kFp8Block <= cols) {
-        uint4 w[kChunks][sizeof(T) / 2];
+// A lane's 32 values as they lie in memory; 0 past the row's end.
+template <typename T>
+struct Raw {
+    static constexpr uint32_t W = sizeof(T) / 2;     // 16-byte words of a chunk
+    uint4 w[kChunks * W];
+
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (uint32_t i = 0; i < kChunks; ++i)
+        for (uint32_t i = 0; i < kChunks * W; ++i) w[i] = make_uint4(0, 0, 0, 0);
+    }
+    template <bool VEC>
+    __device__ __forceinline__ void load(const T* row, uint32_t col0, uint32_t l, uint32_t cols) {
+        if (VEC && col0 + kFp8Block <= cols) {
 #pragma unroll
-            for (uint32_t k = 0; k < sizeof(T) / 2; ++k)
-                w[i][k] = reinterpret_cast<const uint4*>(row + col0 + 8 * (kLanes * i + l))[k];
+            for (uint32_t i = 0; i < kChunks * W; ++i) w[i] = reinterpret_cast<const uint4*>(row + column<VEC>(col0, l, 8 * (i / W)))[i % W];
+            return;
+        }
 #pragma unroll
         for (uint32_t i = 0; i < kChunks; ++i) {
-            const T* t = reinterpret_cast<const T*>(w[i]);
+            if (VEC && column<VEC>(col0, l, 8 * i) + 8 <= cols) {      // a whole chunk of the last, partial block
 #pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) v[8 * i + j] = to_f32(t[j]);
-        }
-        return;
-    }
+                for (uint32_t k = 0; k < W; ++k) w[i * W + k] = reinterpret_cast<const uint4*>(row + column<VEC>(col0, l, 8 * i))[k];
+                continue;
+            }
+            union {
+                T t[8];
+                uint4 u[W];
+            } c;
 #pragma unroll
-    for (uint32_t i = 0; i < kChunks; ++i) {
-        if (VEC && column<VEC>(col0, l, 8 * i) + 8 <= cols) {    // a whole chunk of the last, partial block
-            uint4 w[sizeof(T) / 2];
+            for (uint32_t k = 0; k < W; ++k) c.u[k] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (uint32_t k = 0; k < sizeof(T) / 2; ++k) w[k] = reinterpret_cast<const uint4*>(row + column<VEC>(col0, l, 8 * i))[k];
+            for (uint32_t j = 0; j < 8; ++j)
+                if (column<VEC>(col0, l, 8 * i + j) < cols) c.t[j] = row[column<VEC>(col0, l, 8 * i + j)];
 #pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) v[8 * i + j] = to_f32(reinterpret_cast<const T*>(w)[j]);
-            continue;
-        }
-#pragma unroll
-        for (uint32_t j = 8 * i; j < 8 * i + 8; ++j) {
-            const uint32_t c = column<VEC>(col0, l, j);
-            v[j] = c < cols ? to_f32(row[c]) : 0.0f;
+            for (uint32_t k = 0; k < W; ++k) w[i * W + k] = c.u[k];
         }
     }
-}
+    __device__ __forceinline__ uint32_t word(uint32_t i) const {
+        const uint4& v = w[i / 4];
+        return i % 4 == 0 ? v.x : i % 4 == 1 ? v.y : i % 4 == 2 ? v.z : v.w;
+    }
+    // values 2 p and 2 p + 1 in fp32 (p a constant)
+    __device__ __forceinline__ uint64_t pair(uint32_t p) const;
+    // max(|v|) of the lane; a NaN among them is the result, so that it reaches the block's scale
+    __device__ __forceinline__ float max_abs() const;
+};
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store32(T* row, uint32_t col0, uint32_t l, uint32_t cols, const float (&v)[kVals]) {
-#pragma unroll
-    for (uint32_t i = 0; i < kChunks; ++i) {
-        if (VEC && column<VEC>(col0, l, 8 * i) + 8 <= cols) {
-            uint4 w[sizeof(T) / 2];
-            T* t = reinterpret_cast<T*>(w);
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) from_f32(v[8 * i + j], t[j]);
-#pragma unroll
-            for (uint32_t k = 0; k < sizeof(T) / 2; ++k) reinterpret_cast<uint4*>(row + column<VEC>(col0, l, 8 * i))[k] = w[k];
-            continue;
-        }
-#pragma unroll
-        for (uint32_t j = 8 * i; j < 8 * i + 8; ++j) {
-            const uint32_t c = column<VEC>(col0, l, j);
-            if (c < cols) from_f32(v[j], row[c]);
-        }
-    }
-}
-
-// max(|v|) and a floor; a NaN among them is the result, so that it reaches the block's scale
-__device__ __forceinline__ float max_abs(const float (&v)[kVals], float m) {
-#pragma unroll
-    for (uint32_t j = 0; j < kVals; j += 2)
-        asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v[j]), "f"(v[j + 1]));
-    return m;
-}
 __device__ __forceinline__ float max_nan(float a, float b) {
     float m;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
     return m;
 }
+__device__ __forceinline__ float max_abs3(float m, float a, float b) {
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(a), "f"(b));
+    return m;
+}
 
-constexpr float kTiny = 7.888609052210118e-31f;   // 2^-100
+template <> __device__ __forceinline__ uint64_t Raw<float>::pair(uint32_t p) const { return pack2(word(2 * p), word(2 * p + 1)); }
+template <> __device__ __forceinline__ uint64_t Raw<__nv_bfloat16>::pair(uint32_t p) const {
+    return pack2(word(p) << 16, word(p) & 0xffff0000u);        // bf16 is the upper half of fp32
+}
+template <> __device__ __forceinline__ uint64_t Raw<__half>::pair(uint32_t p) const {
+    const uint32_t u = word(p);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+    return pack2(f.x, f.y);
+}
+template <> __device__ __forceinline__ uint64_t Raw<int16_t>::pair(uint32_t p) const {
+    const uint32_t u = word(p);
+    return pack2(to_f32((int16_t)(u & 0xffffu)), to_f32((int16_t)(u >> 16)));
+}
 
-template <bool VEC>
-__device__ __forceinline__ void store_q32(uint8_t* row, uint32_t col0, uint32_t l, uint32_t cols, uint32_t format, float inv,
-                                          const float (&v)[kVals]) {
-    uint32_t p[kVals / 2];
-    if (format == CM_F8_E4M3) {
+template <> __device__ __forceinline__ float Raw<float>::max_abs() const {
+    float m = 0.0f;
 #pragma unroll
-        for (uint32_t j = 0; j < kVals / 2; ++j) p[j] = cvt_fp8x2(CM_F8_E4M3, v[2 * j] * inv, v[2 * j + 1] * inv);
-    } else {
+    for (uint32_t i = 0; i < kVals; i += 2) m = max_abs3(m, __uint_as_float(word(i)), __uint_as_float(word(i + 1)));
+    return m;
+}
+// magnitudes of 16-bit IEEE types order as integers, infinities above every finite value and NaN
+// above infinity, so two of them compare in one instruction
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t m;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+    return m;
+}
+template <> __device__ __forceinline__ float Raw<__nv_bfloat16>::max_abs() const {
+    uint32_t m = 0;
 #pragma unroll
-        for (uint32_t j = 0; j < kVals / 2; ++j) p[j] = cvt_fp8x2(CM_F8_E5M2, v[2 * j] * inv, v[2 * j + 1] * inv);
+    for (uint32_t i = 0; i < kVals / 2; ++i) m = max_u16x2(m, word(i) & 0x7fff7fffu);
+    return __uint_as_float(max(m & 0xffffu, m >> 16) << 16);
+}
+template <> __device__ __forceinline__ float Raw<__half>::max_abs() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kVals / 2; ++i) m = max_u16x2(m, word(i) & 0x7fff7fffu);
+    return __half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16)));
+}
+template <> __device__ __forceinline__ float Raw<int16_t>::max_abs() const {
+    float m = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < kVals / 2; ++i) {
+        float a, b;
+        unpack2(pair(i), a, b);
+        m = max_abs3(m, a, b);
     }
+    return m;
+}
+
+// a lane's 32 values in fp32 pairs -> row of T
+template <typename T>
+__device__ __forceinline__ uint32_t to_word(uint64_t v);
+template <> __device__ __forceinline__ uint32_t to_word<__nv_bfloat16>(uint64_t v) {
+    float lo, hi;
+    unpack2(v, lo, hi);
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&b);
+}
+template <> __device__ __forceinline__ uint32_t to_word<__half>(uint64_t v) {
+    float lo, hi;
+    unpack2(v, lo, hi);
+    const __half2 b = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void store32(T* row, uint32_t col0, uint32_t l, uint32_t cols, const uint64_t (&v)[kVals / 2]) {
 #pragma unroll
     for (uint32_t i = 0; i < kChunks; ++i) {
         if (VEC && column<VEC>(col0, l, 8 * i) + 8 <= cols) {
-            *reinterpret_cast<uint2*>(row + column<VEC>(col0, l, 8 * i)) =
-                make_uint2(p[4 * i] | (p[4 * i + 1] << 16), p[4 * i + 2] | (p[4 * i + 3] << 16));
+            uint4* d = reinterpret_cast<uint4*>(row + column<VEC>(col0, l, 8 * i));
+            if constexpr (sizeof(T) == 4) {
+                reinterpret_cast<ulonglong2*>(d)[0] = make_ulonglong2(v[4 * i], v[4 * i + 1]);
+                reinterpret_cast<ulonglong2*>(d)[1] = make_ulonglong2(v[4 * i + 2], v[4 * i + 3]);
+            } else {
+                *d = make_uint4(to_word<T>(v[4 * i]), to_word<T>(v[4 * i + 1]), to_word<T>(v[4 * i + 2]), to_word<T>(v[4 * i + 3]));
+            }
             continue;
         }
 #pragma unroll
-        for (uint32_t j = 8 * i; j < 8 * i + 8; ++j) {
-            const uint32_t c = column<VEC>(col0, l, j);
+        for (uint32_t j = 8 * i; j < 8 * i + 8; j += 2) {
+            float lo, hi;
+            unpack2(v[j / 2], lo, hi);
+            if (column<VEC>(col0, l, j) < cols) from_f32(lo, row[column<VEC>(col0, l, j)]);
+            if (column<VEC>(col0, l, j + 1) < cols) from_f32(hi, row[column<VEC>(col0, l, j + 1)]);
+        }
+    }
+}
+
+template <bool VEC, typename V>
+__device__ __forceinline__ void store_q32(uint8_t* row, uint32_t col0, uint32_t l, uint32_t cols, uint32_t format, float inv, V value) {
+    const uint64_t inv2 = pack2(inv, inv);
+#pragma unroll
+    for (uint32_t i = 0; i < kChunks; ++i) {
+        uint32_t p[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            float lo, hi;
+            unpack2(mul2(value(4 * i + j), inv2), lo, hi);
+            p[j] = cvt_fp8x2(format, lo, hi);
+        }
+        if (VEC && column<VEC>(col0, l, 8 * i) + 8 <= cols) {
+            *reinterpret_cast<uint2*>(row + column<VEC>(col0, l, 8 * i)) = make_uint2(p[0] | (p[1] << 16), p[2] | (p[3] << 16));
+            continue;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            const uint32_t c = column<VEC>(col0, l, 8 * i + j);
             if (c < cols) row[c] = (uint8_t)(p[j / 2] >> (8 * (j & 1)));
         }
     }
 }
 
+constexpr float kTiny = 7.888609052210118e-31f;   // 2^-100
+
 // From a lane's max(|v|): F / A of its block in every lane, and A / F in lane 0.
 __device__ __forceinline__ float block_scale(float m, uint32_t l, float F, float& scale) {
 #pragma unroll
     for (uint32_t o = kLanes / 2; o; o /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = max_nan(m, kTiny);
     const float r = (l == 0 ? m : F) / (l == 0 ? F : m);
     scale = r;
     return __shfl_sync(0xffffffffu, r, 1, kLanes);
@@ -139,64 +219,74 @@ struct QuantArgs {
     const void* x;
     uint8_t* q;
     float* scale;
-    uint32_t rows, cols, format;
+    uint32_t rows, cols;
     uint64_t ldx, ldq, lds, x_bs, q_bs, s_bs;
-    uint32_t row_tiles, col_tiles;   // tiles per matrix
+    uint32_t row_tiles, col_tiles, tiles, step;   // row tiles a matrix, column tiles, row tiles of the batch, row tiles a pass
+    FastDiv fd_row, fd_col;
 };
 
 // A warp takes 8 rows of a column block -- their scales lie side by side and fill one 32-byte
-// sector --, a CTA 8 rows x 8 column blocks, 2 KB of a row of a 2-byte type.
+// sector --, a CTA 8 rows x 8 column blocks, 2 KB of a row of a 2-byte type, and then the rows
+// `step` tiles on.
 constexpr uint32_t kQRows = 8, kQCols = 8;
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) quant_rows_kernel(QuantArgs g) {
+template <typename T>
+constexpr uint32_t quant_ctas() { return sizeof(T) == 4 ? 2 : 4; }     // resident an SM: two tiles' values are in registers
+
+template <typename T, bool VEC, uint32_t FMT>
+__global__ void __launch_bounds__(256, quant_ctas<T>()) quant_rows_kernel(const QuantArgs g) {
     griddep_wait();
-    const uint32_t ct = blockIdx.x % g.col_tiles, rest = blockIdx.x / g.col_tiles;
-    const uint32_t rt = rest % g.row_tiles, z = rest / g.row_tiles;
+    const uint32_t rt0 = g.fd_col.div(blockIdx.x), ct = blockIdx.x - rt0 * g.col_tiles;
     const uint32_t lane = threadIdx.x % 32, l = lane % kLanes;
-    const uint32_t row = rt * kQRows + lane / kLanes, cb = ct * kQCols + threadIdx.x / 32, col0 = cb * kFp8Block;
+    const uint32_t cb = ct * kQCols + threadIdx.x / 32, col0 = cb * kFp8Block;
     if (col0 >= g.cols) return;                        // the whole warp
-    const bool live = row < g.rows;
-    float v[kVals];
-    if (live) {
-        load32<T, VEC>((const T*)g.x + (uint64_t)z * g.x_bs + row * g.ldx, col0, l, g.cols, v);
-    } else {
-#pragma unroll
-        for (uint32_t j = 0; j < kVals; ++j) v[j] = 0.0f;
+    const float F = fp8_largest(FMT);
+    auto fetch = [&](uint32_t t, Raw<T>& v, uint32_t& z, uint32_t& row) {
+        z = g.fd_row.div(t);
+        row = (t - z * g.row_tiles) * kQRows + lane / kLanes;
+        if (row < g.rows) v.template load<VEC>((const T*)g.x + (uint64_t)z * g.x_bs + row * g.ldx, col0, l, g.cols);
+        else v.clear();
+    };
+    Raw<T> next;
+    uint32_t nz, nrow;
+    fetch(rt0, next, nz, nrow);
+    for (uint32_t t = rt0; t < g.tiles; t += g.step) {
+        const Raw<T> v = next;
+        const uint32_t z = nz, row = nrow;
+        if (t + g.step < g.tiles) fetch(t + g.step, next, nz, nrow);
+        float scale;
+        const float inv = block_scale(v.max_abs(), l, F, scale);
+        if (row < g.rows) {
+            store_q32<VEC>(g.q + (uint64_t)z * g.q_bs + row * g.ldq, col0, l, g.cols, FMT, inv, [&](uint32_t p) { return v.pair(p); });
+            if (l == 0) g.scale[(uint64_t)z * g.s_bs + cb * g.lds + row] = scale;
+        }
     }
-    float scale;
-    const float inv = block_scale(max_abs(v, kTiny), l, fp8_largest(g.format), scale);
-    if (!live) return;
-    store_q32<VEC>(g.q + (uint64_t)z * g.q_bs + row * g.ldq, col0, l, g.cols, g.format, inv, v);
-    if (l == 0) g.scale[(uint64_t)z * g.s_bs + cb * g.lds + row] = scale;
 }
 
 // ---- cm_quant_fp8, one scale per 128 x 128 block -----------------------------------------------
 // A CTA of 512 threads holds its whole block in registers (32 values a thread), so it is read once.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(512) quant_blocks_kernel(QuantArgs g) {
+template <typename T, bool VEC, uint32_t FMT>
+__global__ void __launch_bounds__(512) quant_blocks_kernel(const QuantArgs g) {
     griddep_wait();
     __shared__ float top[16];
-    const uint32_t cb = blockIdx.x % g.col_tiles, rest = blockIdx.x / g.col_tiles;
-    const uint32_t rb = rest % g.row_tiles, z = rest / g.row_tiles;
+    const uint32_t rbz = g.fd_col.div(blockIdx.x), cb = blockIdx.x - rbz * g.col_tiles;
+    const uint32_t z = g.fd_row.div(rbz), rb = rbz - z * g.row_tiles;
     const uint32_t l = threadIdx.x % kLanes, row = rb * kFp8Block + threadIdx.x / kLanes, col0 = cb * kFp8Block;
     const bool live = row < g.rows;
-    float v[kVals];
-    if (live) {
-        load32<T, VEC>((const T*)g.x + (uint64_t)z * g.x_bs + row * g.ldx, col0, l, g.cols, v);
-    } else {
-#pragma unroll
-        for (uint32_t j = 0; j < kVals; ++j) v[j] = 0.0f;
-    }
-    float m = max_abs(v, kTiny);
+    Raw<T> v;
+    if (live) v.template load<VEC>((const T*)g.x + (uint64_t)z * g.x_bs + row * g.ldx, col0, l, g.cols);
+    else v.clear();
+    float m = v.max_abs();
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = m;
     __syncthreads();
+    m = max_nan(top[threadIdx.x % 16], kTiny);
 #pragma unroll
-    for (int w = 0; w < 16; ++w) m = max_nan(m, top[w]);
-    const float F = fp8_largest(g.format);
-    if (live) store_q32<VEC>(g.q + (uint64_t)z * g.q_bs + row * g.ldq, col0, l, g.cols, g.format, F / m, v);
+    for (int o = 8; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float F = fp8_largest(FMT);
+    if (live)
+        store_q32<VEC>(g.q + (uint64_t)z * g.q_bs + row * g.ldq, col0, l, g.cols, FMT, F / m, [&](uint32_t p) { return v.pair(p); });
     if (threadIdx.x == 0) g.scale[(uint64_t)z * g.s_bs + rb * g.lds + cb] = m / F;
 }
 
@@ -217,73 +307,118 @@ struct NormArgs {
     float eps;
 };
 
-template <bool VEC>
-__device__ __forceinline__ void load_weight(const void* w, uint32_t type, uint32_t col0, uint32_t l, uint32_t cols, float (&v)[kVals]) {
-    if (type == CM_T_F32) load32<float, VEC>((const float*)w, col0, l, cols, v);
-    else if (type == CM_T_F16) load32<__half, VEC>((const __half*)w, col0, l, cols, v);
-    else load32<__nv_bfloat16, VEC>((const __nv_bfloat16*)w, col0, l, cols, v);
+// G threads share a row, which stays in their registers, a block to 4 of them, and then take the
+// row gridDim rows on.  The weight's values of a thread stay in its registers for all its rows: in
+// the tensors' own type where that is the weight's (WT = T), else in fp32.  Rows of more than 256
+// threads have no registers to spare for either: they are loaded, and so is the weight, row by row.
+template <typename T, typename WT>
+constexpr uint32_t norm_ctas(uint32_t g) {     // resident an SM
+    return g > 256 ? 1 : g == 256 ? 2 : sizeof(T) + sizeof(WT) == 4 ? 5 : 4 - sizeof(T) / 4;
 }
 
-// G threads share a row, which stays in their registers, a block to 4 of them.
-template <typename T, uint32_t G, bool VEC>
-__global__ void __launch_bounds__(G < 128 ? 128 : G) rmsnorm_kernel(NormArgs g) {
+template <typename T, typename WT, uint32_t G, bool VEC>
+__global__ void __launch_bounds__(G < 128 ? 128 : G, norm_ctas<T, WT>(G)) rmsnorm_kernel(const NormArgs g) {
     griddep_wait();
+    constexpr bool AHEAD = G <= 256;
     constexpr uint32_t ROWS = G < 128 ? 128 / G : 1;
-    __shared__ float part[32];
+    __shared__ float part[2][32];
     const uint32_t t = threadIdx.x % G, l = t % kLanes, blk = t / kLanes, col0 = blk * kFp8Block;
-    const uint32_t row = blockIdx.x * ROWS + threadIdx.x / G;
-    const bool in = row < g.rows && col0 < g.cols;
-    const uint64_t r = row;
-    float h[kVals];
+    const bool mine = col0 < g.cols;
+    uint32_t row = blockIdx.x * ROWS + threadIdx.x / G;
+    const uint32_t step = gridDim.x * ROWS;
+    Raw<T> x, r;
+    x.clear();
+    r.clear();
+    auto fetch = [&](uint64_t i) {
+        if (!mine || i >= g.rows) return;
+        x.template load<VEC>((const T*)g.x + i * g.ldx, col0, l, g.cols);
+        if (g.resid) r.template load<VEC>((const T*)g.resid + i * g.ldr, col0, l, g.cols);
+    };
+    if (AHEAD) fetch(row);
+    Raw<WT> w;
+    w.clear();
+    auto fetch_weight = [&]() {
+        if (!mine || !g.weight) return;
+        if constexpr (sizeof(WT) == sizeof(T)) {
+            w.template load<VEC>((const WT*)g.weight, col0, l, g.cols);
+        } else if (g.weight_type == CM_T_F32) {
+            w.template load<VEC>((const WT*)g.weight, col0, l, g.cols);
+        } else {
+            // the other 16-bit type: element by element, once a thread
 #pragma unroll
-    for (uint32_t j = 0; j < kVals; ++j) h[j] = 0.0f;
-    if (in) {
-        load32<T, VEC>((const T*)g.x + r * g.ldx, col0, l, g.cols, h);
-        if (g.resid) {
-            float v[kVals];
-            load32<T, VEC>((const T*)g.resid + r * g.ldr, col0, l, g.cols, v);
-#pragma unroll
-            for (uint32_t j = 0; j < kVals; ++j) h[j] += v[j];
+            for (uint32_t j = 0; j < kVals; ++j) {
+                const uint32_t c = column<VEC>(col0, l, j);
+                if (c < g.cols)
+                    reinterpret_cast<float*>(w.w)[j] = g.weight_type == CM_T_F16 ? to_f32(((const __half*)g.weight)[c])
+                                                                                 : to_f32(((const __nv_bfloat16*)g.weight)[c]);
+            }
         }
-    }
-    float ss = 0.0f;
-    {
-        float s[4] = {};
+    };
+    if (AHEAD) fetch_weight();
+    const float F = fp8_largest(g.format), inv_cols = 1.0f / (float)g.cols;
+    // every thread of a CTA makes the same number of passes: the barrier below is the CTA's
+    for (uint32_t first = blockIdx.x * ROWS, pass = 0; first < g.rows; first += step, row += step, pass ^= 1) {
+        const bool in = mine && row < g.rows;
+        uint64_t h[kVals / 2];
+        if (!AHEAD) fetch(row);
+        if (g.resid) {
 #pragma unroll
-        for (uint32_t j = 0; j < kVals; ++j) s[j % 4] = fmaf(h[j], h[j], s[j % 4]);
-        ss = (s[0] + s[1]) + (s[2] + s[3]);
-    }
+            for (uint32_t p = 0; p < kVals / 2; ++p) h[p] = add2(x.pair(p), r.pair(p));
+        } else {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (G > 32) {
-        if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = ss;
-        __syncthreads();
-        ss = threadIdx.x % 32 < G / 32 ? part[threadIdx.x % 32] : 0.0f;
+            for (uint32_t p = 0; p < kVals / 2; ++p) h[p] = x.pair(p);
+        }
+        if (AHEAD) fetch((uint64_t)row + step);
+        uint64_t s2[4] = {};
+#pragma unroll
+        for (uint32_t p = 0; p < kVals / 2; ++p) s2[p % 4] = fma2(h[p], h[p], s2[p % 4]);
+        float ss, other;
+        unpack2(add2(add2(s2[0], s2[1]), add2(s2[2], s2[3])), ss, other);
+        ss += other;
 #pragma unroll
         for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    }
-    const float rms = 1.0f / sqrtf(ss / (float)g.cols + g.eps);
-    if (in && g.resid_out) store32<T, VEC>((T*)g.resid_out + r * g.ldo, col0, l, g.cols, h);
+        if (G > 32) {
+            // two sets of partial sums in turn: one barrier a row is enough
+            if (threadIdx.x % 32 == 0) part[pass][threadIdx.x / 32] = ss;
+            __syncthreads();
+            ss = threadIdx.x % 32 < G / 32 ? part[pass][threadIdx.x % 32] : 0.0f;
 #pragma unroll
-    for (uint32_t j = 0; j < kVals; ++j) h[j] *= rms;
-    if (in && g.weight) {
-        float w[kVals];
-        load_weight<VEC>(g.weight, g.weight_type, col0, l, g.cols, w);
+            for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        }
+        const float rms = 1.0f / sqrtf(fmaf(ss, inv_cols, g.eps));
+        const uint64_t rms2 = pack2(rms, rms);
+        if (in && g.resid_out) store32<T, VEC>((T*)g.resid_out + (uint64_t)row * g.ldo, col0, l, g.cols, h);
 #pragma unroll
-        for (uint32_t j = 0; j < kVals; ++j) h[j] *= w[j];
-    }
-    if (in && g.y) store32<T, VEC>((T*)g.y + r * g.ldy, col0, l, g.cols, h);
-    if (g.q) {
+        for (uint32_t p = 0; p < kVals / 2; ++p) h[p] = mul2(h[p], rms2);
+        if (g.weight) {
+            if (!AHEAD) fetch_weight();
+#pragma unroll
+            for (uint32_t p = 0; p < kVals / 2; ++p) h[p] = mul2(h[p], w.pair(p));
+        }
+        if (in && g.y) store32<T, VEC>((T*)g.y + (uint64_t)row * g.ldy, col0, l, g.cols, h);
+        if (!g.q) continue;
         if (col0 + kFp8Block > g.cols) {   // columns past the row's end hold no value (an infinite rms would make 0 * inf of them)
 #pragma unroll
-            for (uint32_t j = 0; j < kVals; ++j)
-                if (column<VEC>(col0, l, j) >= g.cols) h[j] = 0.0f;
+            for (uint32_t j = 0; j < kVals; j += 2) {
+                float lo, hi;
+                unpack2(h[j / 2], lo, hi);
+                h[j / 2] = pack2(column<VEC>(col0, l, j) < g.cols ? lo : 0.0f, column<VEC>(col0, l, j + 1) < g.cols ? hi : 0.0f);
+            }
         }
-        float scale;
-        const float inv = block_scale(max_abs(h, kTiny), l, fp8_largest(g.format), scale);
+        float m = 0.0f, scale;
+#pragma unroll
+        for (uint32_t p = 0; p < kVals / 2; ++p) {
+            float lo, hi;
+            unpack2(h[p], lo, hi);
+            m = max_abs3(m, lo, hi);
+        }
+        const float inv = block_scale(m, l, F, scale);
         if (in) {
-            store_q32<VEC>(g.q + r * g.ldq, col0, l, g.cols, g.format, inv, h);
-            if (l == 0) g.scale[blk * g.lds + r] = scale;
+            uint8_t* q = g.q + (uint64_t)row * g.ldq;
+            auto value = [&](uint32_t p) { return h[p]; };
+            if (g.format == CM_F8_E4M3) store_q32<VEC>(q, col0, l, g.cols, CM_F8_E4M3, inv, value);
+            else store_q32<VEC>(q, col0, l, g.cols, CM_F8_E5M2, inv, value);
+            if (l == 0) g.scale[blk * g.lds + row] = scale;
         }
     }
 }
@@ -291,39 +426,37 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) rmsnorm_kernel(NormArgs g) 
 // ---- host ---------------------------------------------------------------------------------------
 bool aligned(const void* p, uint64_t pitch_bytes, unsigned to) { return ((uintptr_t)p % to) == 0 && pitch_bytes % to == 0; }
 
-template <bool VEC>
-void launch_quant(const QuantArgs& g, unsigned type, bool blocks, unsigned grid, cudaStream_t s) {
-#define CM_QUANT(T)                                                        \
-    do {                                                                   \
-        if (blocks) launch_k(quant_blocks_kernel<T, VEC>, grid, 512, 0, s, g); \
-        else launch_k(quant_rows_kernel<T, VEC>, grid, 256, 0, s, g);      \
-    } while (0)
-    switch (type) {
-        case CM_T_Q88: CM_QUANT(int16_t); break;
-        case CM_T_F32: CM_QUANT(float); break;
-        case CM_T_F16: CM_QUANT(__half); break;
-        default: CM_QUANT(__nv_bfloat16); break;
-    }
-#undef CM_QUANT
+template <typename T, bool VEC, uint32_t FMT>
+void launch_quant(const QuantArgs& g, bool blocks, unsigned grid, cudaStream_t s) {
+    if (blocks) launch_k(quant_blocks_kernel<T, VEC, FMT>, grid, 512, 0, s, g);
+    else launch_k(quant_rows_kernel<T, VEC, FMT>, grid, 256, 0, s, g);
 }
 
-template <typename T, bool VEC>
-void launch_norm(const NormArgs& g, cudaStream_t s) {
-    // threads a row: the fewest that hold it (32 values each)
-    if (g.cols <= 32 * kVals) launch_k(rmsnorm_kernel<T, 32, VEC>, (g.rows + 3) / 4, 128, 0, s, g);
-    else if (g.cols <= 128 * kVals) launch_k(rmsnorm_kernel<T, 128, VEC>, g.rows, 128, 0, s, g);
-    else if (g.cols <= 256 * kVals) launch_k(rmsnorm_kernel<T, 256, VEC>, g.rows, 256, 0, s, g);
-    else if (g.cols <= 512 * kVals) launch_k(rmsnorm_kernel<T, 512, VEC>, g.rows, 512, 0, s, g);
-    else launch_k(rmsnorm_kernel<T, 1024, VEC>, g.rows, 1024, 0, s, g);
+template <typename T>
+void launch_quant_type(const QuantArgs& g, bool blocks, bool vec, unsigned format, unsigned grid, cudaStream_t s) {
+    if (vec && format == CM_F8_E4M3) launch_quant<T, true, CM_F8_E4M3>(g, blocks, grid, s);
+    else if (vec) launch_quant<T, true, CM_F8_E5M2>(g, blocks, grid, s);
+    else if (format == CM_F8_E4M3) launch_quant<T, false, CM_F8_E4M3>(g, blocks, grid, s);
+    else launch_quant<T, false, CM_F8_E5M2>(g, blocks, grid, s);
 }
 
-template <bool VEC>
-void launch_norm_type(const NormArgs& g, unsigned type, cudaStream_t s) {
-    switch (type) {
-        case CM_T_F32: launch_norm<float, VEC>(g, s); break;
-        case CM_T_F16: launch_norm<__half, VEC>(g, s); break;
-        default: launch_norm<__nv_bfloat16, VEC>(g, s); break;
-    }
+template <typename T, typename WT, bool VEC>
+void launch_norm(const Context* cx, const NormArgs& g, cudaStream_t s) {
+    // threads a row: the fewest that hold it (32 values each); CTAs: what the SMs hold at once
+    auto ctas = [&](unsigned threads, uint32_t rows) { return std::min(rows, (uint32_t)cx->sm_count * norm_ctas<T, WT>(threads)); };
+    if (g.cols <= 32 * kVals) launch_k(rmsnorm_kernel<T, WT, 32, VEC>, ctas(128, (g.rows + 3) / 4), 128, 0, s, g);
+    else if (g.cols <= 128 * kVals) launch_k(rmsnorm_kernel<T, WT, 128, VEC>, ctas(128, g.rows), 128, 0, s, g);
+    else if (g.cols <= 256 * kVals) launch_k(rmsnorm_kernel<T, WT, 256, VEC>, ctas(256, g.rows), 256, 0, s, g);
+    else if (g.cols <= 512 * kVals) launch_k(rmsnorm_kernel<T, WT, 512, VEC>, ctas(512, g.rows), 512, 0, s, g);
+    else launch_k(rmsnorm_kernel<T, WT, 1024, VEC>, ctas(1024, g.rows), 1024, 0, s, g);
+}
+
+template <typename T>
+void launch_norm_type(const Context* cx, const NormArgs& g, bool vec, bool same, cudaStream_t s) {
+    if (vec && same) launch_norm<T, T, true>(cx, g, s);
+    else if (vec) launch_norm<T, float, true>(cx, g, s);
+    else if (same) launch_norm<T, T, false>(cx, g, s);
+    else launch_norm<T, float, false>(cx, g, s);
 }
 
 constexpr uint32_t kNormMaxCols = 1024 * kVals;
@@ -359,18 +492,29 @@ extern "C" int cm_quant_fp8_async(const void* x, unsigned x_type, uint8_t* q, fl
     int rc = enter(&cx);
     if (rc) return rc;
     if (rows == 0 || cols == 0 || batch == 0) return CM_OK;
-    QuantArgs g{x, q, scale, rows, cols, format, ldx, ldq, lds, x_batch_stride, q_batch_stride, scale_batch_stride, 0, 0};
+    QuantArgs g{x, q, scale, rows, cols, ldx, ldq, lds, x_batch_stride, q_batch_stride, scale_batch_stride};
     g.row_tiles = (uint32_t)(blocks ? rb : (rows + (uint64_t)kQRows - 1) / kQRows);
     g.col_tiles = (uint32_t)(blocks ? cb : (cb + kQCols - 1) / kQCols);
-    const unsigned __int128 grid = (unsigned __int128)g.row_tiles * g.col_tiles * batch;
-    if (grid >= (1u << 31)) return set_error(CM_EUNSUPPORTED, "cm_quant_fp8: more than 2^31 tiles");
+    const uint64_t tiles = (uint64_t)g.row_tiles * batch;
+    if (tiles >= (1u << 30) || tiles * g.col_tiles >= (1u << 31)) return set_error(CM_EUNSUPPORTED, "cm_quant_fp8: more than 2^31 tiles");
+    g.tiles = (uint32_t)tiles;
+    // blocks: one CTA each; rows: as many CTAs as the SMs hold, each walking down its column tile
+    const uint32_t hold = (x_type == CM_T_F32 ? quant_ctas<float>() : quant_ctas<__half>()) * cx->sm_count;
+    g.step = blocks ? g.tiles : std::min(g.tiles, std::max(1u, hold / g.col_tiles));
+    g.fd_row = FastDiv(g.row_tiles);
+    g.fd_col = FastDiv(g.col_tiles);
+    const unsigned grid = g.step * g.col_tiles;
     const cudaStream_t s = (cudaStream_t)stream;
     const bool vec = aligned(x, ldx * size, 16) && aligned(q, ldq, 8) &&
                      (batch == 1 || (x_batch_stride * size % 16 == 0 && q_batch_stride % 8 == 0));
     {
         ProfScope ps_(PK_FP8_QUANT, s);
-        if (vec) launch_quant<true>(g, x_type, blocks, (unsigned)grid, s);
-        else launch_quant<false>(g, x_type, blocks, (unsigned)grid, s);
+        switch (x_type) {
+            case CM_T_Q88: launch_quant_type<int16_t>(g, blocks, vec, format, grid, s); break;
+            case CM_T_F32: launch_quant_type<float>(g, blocks, vec, format, grid, s); break;
+            case CM_T_F16: launch_quant_type<__half>(g, blocks, vec, format, grid, s); break;
+            default: launch_quant_type<__nv_bfloat16>(g, blocks, vec, format, grid, s); break;
+        }
     }
     count_launch();
     cudaError_t e = cudaGetLastError();
@@ -423,8 +567,12 @@ extern "C" int cm_rmsnorm_fp8_async(const void* x, const void* resid, const void
                      (!q || aligned(q, ldq, 8)) && (!weight || aligned(weight, 0, 16));
     {
         ProfScope ps_(PK_FP8_QUANT, s);
-        if (vec) launch_norm_type<true>(g, type, s);
-        else launch_norm_type<false>(g, type, s);
+        const bool same = !weight || weight_type == type;
+        switch (type) {
+            case CM_T_F32: launch_norm_type<float>(cx, g, vec, same, s); break;
+            case CM_T_F16: launch_norm_type<__half>(cx, g, vec, same, s); break;
+            default: launch_norm_type<__nv_bfloat16>(cx, g, vec, same, s); break;
+        }
     }
     count_launch();
     cudaError_t e = cudaGetLastError();

@@ -128,21 +128,6 @@ __device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[16]) {
 #undef CM_IO
 #undef CM_16
 
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-    uint64_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
-    return v;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-// two fp32 multiply-adds in one instruction
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-
 struct TileF8 {
     uint32_t m0;             // first weight row (of this CTA)
     uint32_t row0, row1;     // token rows row0 .. row1 - 1, at most TN of them used
