@@ -48,19 +48,25 @@ struct KArgs {
     uint64_t timeout_ns;
 };
 
-template <int TN, int CG>
+template <int TN, int CG, bool TOK>
 struct F8Cfg {
+    static_assert(!TOK || (TN == 256 && CG == 2), "tokens are the M operand of 256 x 256 pair tiles");
     static constexpr int EPI_WARPS = TN >= 128 ? 8 : 4;
-    static constexpr int COLS = TN / (EPI_WARPS / 4);        // token columns of an epilogue warp
+    static constexpr int COLS = TN / (EPI_WARPS / 4);        // accumulator columns of an epilogue warp
     static constexpr int THREADS = 128 + 32 * EPI_WARPS;
+    static constexpr uint32_t TOKENS = TOK ? 128 * CG : TN;  // token rows of a tile
+    static constexpr uint32_t WEIGHTS = TOK ? TN : 128 * CG; // weight rows of a tile
+    static constexpr bool SPLIT_REGS = TN == 256;            // 128 sums a thread: registers move to the epilogue warps
     static constexpr int A_TILE = 128 * 128, B_TILE = TN / CG * 128;
     static constexpr int STAGE = A_TILE + B_TILE;
     static constexpr int STAGES = TN >= 128 ? 6 : TN == 64 ? 8 : TN == 32 ? 9 : 10;
     static constexpr int NBUF = TN == 256 ? 2 : 4;           // accumulators in TMEM
     static constexpr int SLOTS = 8;                          // scale ring
     static constexpr uint32_t TMEM_COLS = NBUF * TN;
-    static constexpr int TABLES = 2 * (kMaxGroups + 1) * 4;
-    static constexpr int SMEM = 1024 + STAGES * STAGE + SLOTS * TN * 4 + 512 + TABLES;
+    static constexpr int TABLES = (2 * (kMaxGroups + 1) * 4 + 15) / 16 * 16;
+    static_assert((STAGES * STAGE + SLOTS * TN * 4) % 16 == 0, "what follows the ring is 16-byte aligned");
+    static constexpr int OUT = TOK ? EPI_WARPS * 2048 : 0;   // output staging: 32 rows x 64 bytes a warp
+    static constexpr int SMEM = 1024 + STAGES * STAGE + SLOTS * TN * 4 + 512 + TABLES + OUT;
     static_assert(SMEM <= 232448 && 2 * SMEM > 232448, "one CTA an SM");
     static_assert(TN * 512 <= STAGES * STAGE, "partial sums of a split tile fit the stages");
 };
@@ -109,28 +115,39 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a, uint64_t b,
             : "memory");
 }
 
-// 16 accumulator columns of this warp's 32 lanes, complete on return: the wait carries the
-// registers, so nothing that reads them can move above it.
+// 16 or 32 accumulator columns of this warp's 32 lanes; they are there after tmem_ld_done, which
+// carries the registers, so that nothing that reads them can move above it.
 #define CM_O(i) "=r"(r[i])
 #define CM_IO(i) "+r"(r[i])
-#define CM_16(X) X(0), X(1), X(2), X(3), X(4), X(5), X(6), X(7), X(8), X(9), X(10), X(11), X(12), X(13), X(14), X(15)
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+#define CM_8(X, o) X(o), X(o + 1), X(o + 2), X(o + 3), X(o + 4), X(o + 5), X(o + 6), X(o + 7)
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : CM_16(CM_O)
+        : CM_8(CM_O, 0), CM_8(CM_O, 8)
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : CM_8(CM_O, 0), CM_8(CM_O, 8), CM_8(CM_O, 16), CM_8(CM_O, 24)
         : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : CM_16(CM_IO)::"memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : CM_8(CM_IO, 0), CM_8(CM_IO, 8)::"memory");
+}
+__device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : CM_8(CM_IO, 0), CM_8(CM_IO, 8), CM_8(CM_IO, 16), CM_8(CM_IO, 24)::"memory");
 }
 #undef CM_O
 #undef CM_IO
-#undef CM_16
+#undef CM_8
 
 struct TileF8 {
-    uint32_t m0;             // first weight row (of this CTA)
-    uint32_t row0, row1;     // token rows row0 .. row1 - 1, at most TN of them used
+    uint32_t m0;             // first weight row
+    uint32_t row0, row1;     // token rows row0 .. row1 - 1, at most a tile's used
     uint32_t group;
 };
 
@@ -138,8 +155,8 @@ struct TileF8 {
 // weight tile, so that the tiles in flight share a few operand panels in L2.
 constexpr uint32_t kBand = 8;
 
-template <int TN, int CG>
-__device__ __forceinline__ TileF8 decode_tile(const KArgs& g, const uint32_t* first, const uint32_t* ends, uint32_t t, uint32_t rank) {
+template <typename C>
+__device__ __forceinline__ TileF8 decode_tile(const KArgs& g, const uint32_t* first, const uint32_t* ends, uint32_t t) {
     uint32_t local = t, tt = g.tiles_t, row0 = 0, row1 = g.n, group = 0;
     if (g.offsets) {
         const uint32_t q = g.fd_m.div(t);                     // token tile over all groups
@@ -158,8 +175,8 @@ __device__ __forceinline__ TileF8 decode_tile(const KArgs& g, const uint32_t* fi
     const uint32_t per = kBand * g.tiles_m, band = local / per, r = local - band * per;
     const uint32_t size = min(kBand, tt - band * kBand), mt = r / size;
     TileF8 c;
-    c.m0 = (mt * CG + rank) * 128;
-    c.row0 = row0 + (band * kBand + r - mt * size) * TN;
+    c.m0 = mt * C::WEIGHTS;
+    c.row0 = row0 + (band * kBand + r - mt * size) * C::TOKENS;
     c.row1 = row1;
     c.group = group;
     return c;
@@ -182,6 +199,55 @@ __device__ __forceinline__ void store_cols(const KArgs& g, const TileF8& tc, uin
     }
 }
 
+// TOK: 32 token rows of 128 columns, a row a lane.  64 bytes of each row go through shared memory
+// at a time (16-byte pieces XOR-swizzled over the bank groups), so that a store covers whole
+// 64-byte runs of eight rows instead of 16 bytes of 32.
+template <typename T>
+__device__ __forceinline__ void store_rows(const KArgs& g, uint32_t row0, uint32_t row1, uint32_t mcol, uint8_t* stage, uint32_t lane,
+                                           const uint64_t (&acc)[64]) {
+    constexpr uint32_t W = 64 / sizeof(T);           // columns of a pass
+    const bool vec = (uintptr_t)g.c % 16 == 0 && g.ldc * sizeof(T) % 16 == 0;
+#pragma unroll
+    for (uint32_t c0 = 0; c0 < 128; c0 += W) {
+        if (mcol + c0 >= g.m) break;                  // the whole warp
+        __syncwarp();
+#pragma unroll
+        for (uint32_t p = 0; p < 4; ++p) {
+            union {
+                T t[W / 4];
+                uint4 u;
+            } o;
+#pragma unroll
+            for (uint32_t j = 0; j < W / 4; j += 2) {
+                float lo, hi;
+                unpack2(acc[(c0 + p * (W / 4) + j) / 2], lo, hi);
+                from_f32(lo, o.t[j]);
+                from_f32(hi, o.t[j + 1]);
+            }
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((p ^ (lane >> 1)) & 3) * 16) = o.u;
+        }
+        __syncwarp();
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t r = 8 * i + lane / 4, p = lane % 4, col = mcol + c0 + p * (W / 4);
+            union {
+                T t[W / 4];
+                uint4 u;
+            } o;
+            o.u = *reinterpret_cast<const uint4*>(stage + r * 64 + ((p ^ (r >> 1)) & 3) * 16);
+            if (row0 + r >= row1) continue;
+            T* d = (T*)g.c + (uint64_t)(row0 + r) * g.ldc + col;
+            if (vec && col + W / 4 <= g.m) {
+                *reinterpret_cast<uint4*>(d) = o.u;
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < W / 4; ++j)
+                    if (col + j < g.m) d[j] = o.t[j];
+            }
+        }
+    }
+}
+
 __device__ __forceinline__ void store_one(const KArgs& g, uint64_t i, float v) {
     switch (g.c_type) {
         case CM_T_Q88: from_f32(v, ((int16_t*)g.c)[i]); break;
@@ -191,20 +257,23 @@ __device__ __forceinline__ void store_one(const KArgs& g, uint64_t i, float v) {
     }
 }
 
+__device__ __forceinline__ void fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
+__device__ __forceinline__ void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
+
 // The token scales of one (tile, K block), as a scale warp holds them on their way from global
 // memory: the loads are issued two blocks of this warp (four of the CTA) ahead of their use.
-template <int TN>
+template <int TN, bool TOK>
 struct ScaleRegs {
-    float v[TN < 32 ? 1 : TN / 32];
-    float sb;
+    float v[TOK ? 4 : TN < 32 ? 1 : TN / 32];
+    float sb[TOK ? 2 : 1];
 };
 
 // KS: the CTAs of a cluster share one tile, each a contiguous part of its K blocks, and add their
 // sums through distributed shared memory, in the order of their ranks.
-template <int TN, int CG, bool KS>
-__global__ void __launch_bounds__(F8Cfg<TN, CG>::THREADS, 1)
+template <int TN, int CG, bool TOK, bool KS>
+__global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
     gemm_f8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT, const KArgs g) {
-    using C = F8Cfg<TN, CG>;
+    using C = F8Cfg<TN, CG, TOK>;
     static_assert(CG == 1 || !KS, "a pair does not split K");
     griddep_wait();
     griddep_launch_dependents();   // all CTAs are resident
@@ -284,7 +353,7 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG>::THREADS, 1)
             uint32_t before = __shfl_up_sync(0xffffffffu, e, 1);
             if (lane == 0) before = high;
             // tiles of the group that ends at offset i (none ends at offset 0)
-            uint32_t cnt = i > 0 ? (e - before + TN - 1) / TN : 0u;
+            uint32_t cnt = i > 0 ? (e - before + C::TOKENS - 1) / C::TOKENS : 0u;
 #pragma unroll
             for (int o = 1; o < 32; o *= 2) {
                 const uint32_t p = __shfl_up_sync(0xffffffffu, cnt, o);
@@ -305,20 +374,25 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG>::THREADS, 1)
     const uint32_t total = g.offsets ? first[g.groups] * g.tiles_m : g.total;
     const WaitCtl wc{abort_flag, g.status, g.timeout_ns};
 
+    // each role moves its registers: 168 a thread at launch, 128 x 56 + 256 x 224 = 384 x 168
     if (warp == 0) {
+        if constexpr (C::SPLIT_REGS) fewer_regs();
         if (lane == 0) {
             uint32_t s = 0, phase = 1, it = 0;
             bool ok = true;
             for (uint32_t t = cid; ok && t < total; t += ncl) {
-                const TileF8 tc = decode_tile<TN, CG>(g, first, ends, t, rank);
+                const TileF8 tc = decode_tile<C>(g, first, ends, t);
                 for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
                     if (!mbar_wait(smem_u32(&empty_b[s]), phase, wc)) { ok = false; break; }
                     const uint32_t st = smem_u32(smem + s * C::STAGE);
                     if (CG == 2) {
                         const uint32_t full = map_to_rank(smem_u32(&full_b[s]), 0);
                         if (leader) mbar_expect_tx(smem_u32(&full_b[s]), 2 * C::STAGE);
-                        tma_load_3d_pair(st, &tmW, full, (int)(kb * 128), (int)tc.m0, (int)(tc.group * g.group_step));
-                        tma_load_2d_pair(st + C::A_TILE, &tmT, full, (int)(kb * 128), (int)(tc.row0 + rank * (TN / 2)));
+                        // each CTA its 128 rows of the M operand and its half of the N operand
+                        const uint32_t w = TOK ? C::A_TILE : 0, x = TOK ? 0 : C::A_TILE;
+                        tma_load_3d_pair(st + w, &tmW, full, (int)(kb * 128), (int)(tc.m0 + rank * (C::WEIGHTS / 2)),
+                                         (int)(tc.group * g.group_step));
+                        tma_load_2d_pair(st + x, &tmT, full, (int)(kb * 128), (int)(tc.row0 + rank * (C::TOKENS / 2)));
                     } else {
                         const uint32_t full = smem_u32(&full_b[s]);
                         mbar_expect_tx(full, C::STAGE);
@@ -337,6 +411,7 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG>::THREADS, 1)
             }
         }
     } else if (warp == 1) {
+        if constexpr (C::SPLIT_REGS) fewer_regs();
         if (lane == 0 && leader) {
             uint32_t s = 0, phase = 0, buf = 0, bphase = 1;
             bool ok = true;
@@ -373,28 +448,34 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG>::THREADS, 1)
         }
     } else if (warp < 4) {
         // Scale warps: 2 takes the even (tile, K block) items of this CTA, 3 the odd ones.
+        if constexpr (C::SPLIT_REGS) fewer_regs();
         constexpr uint32_t AHEAD = 2;
-        ScaleRegs<TN> regs[AHEAD];
+        ScaleRegs<TN, TOK> regs[AHEAD];
         uint32_t t = cid, kb = kb0;
         TileF8 tc{};
         const float* sbp = nullptr;
+        uint32_t blocks = 0;                 // weight blocks of this CTA's part of the tile that exist
         bool fresh = true;
         auto advance = [&](uint32_t by) {
             for (uint32_t i = 0; i < by; ++i)
                 if (++kb == kb1) { kb = kb0; t += ncl; fresh = true; }
         };
-        auto load = [&](ScaleRegs<TN>& r) {
+        auto load = [&](ScaleRegs<TN, TOK>& r) {
             if (fresh) {
-                tc = decode_tile<TN, CG>(g, first, ends, t, rank);
-                sbp = tc.m0 < g.m ? g.bs + tc.group * g.bs_gs + (uint64_t)(tc.m0 / 128) * g.b_lds : nullptr;
+                tc = decode_tile<C>(g, first, ends, t);
+                if (TOK) tc.row0 += rank * 128;
+                else tc.m0 += rank * 128;
+                blocks = tc.m0 < g.m ? (g.m - tc.m0 + 127) / 128 : 0u;
+                sbp = g.bs + tc.group * g.bs_gs + (uint64_t)(tc.m0 / 128) * g.b_lds;
                 fresh = false;
             }
-            r.sb = sbp ? __ldg(sbp + kb) : 0.0f;
+#pragma unroll
+            for (uint32_t h = 0; h < sizeof(r.sb) / 4; ++h) r.sb[h] = h < blocks ? __ldg(sbp + h * g.b_lds + kb) : 0.0f;
             const float* p = g.as + (uint64_t)kb * g.a_lds + tc.row0;
 #pragma unroll
             for (uint32_t i = 0; i < sizeof(r.v) / 4; ++i) {
                 const uint32_t j = lane + 32 * i;
-                r.v[i] = j < TN && tc.row0 + j < tc.row1 ? __ldg(p + j) : 0.0f;
+                r.v[i] = (TOK || j < TN) && tc.row0 + j < tc.row1 ? __ldg(p + j) : 0.0f;
             }
         };
         uint32_t item = warp - 2;
@@ -416,7 +497,9 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG>::THREADS, 1)
 #pragma unroll
                         for (uint32_t i = 0; i < sizeof(regs[p].v) / 4; ++i) {
                             const uint32_t j = lane + 32 * i;
-                            if (j < TN) ring[slot * TN + j] = regs[p].v[i] * regs[p].sb;
+#pragma unroll
+                            for (uint32_t h = 0; h < sizeof(regs[p].sb) / 4; ++h)
+                                if (TOK || j < TN) ring[slot * TN + h * 128 + j] = regs[p].v[i] * regs[p].sb[h];
                         }
                         __syncwarp();
                         if (lane == 0) mbar_arrive(smem_u32(&sfull_b[slot]));
@@ -428,12 +511,13 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG>::THREADS, 1)
             }
         }
     } else {
+        if constexpr (C::SPLIT_REGS) more_regs();
         const uint32_t quarter = warp & 3u, col0 = (warp - 4) / 4 * C::COLS;
         uint32_t buf = 0, bphase = 0, slot = 0, sphase = 0;
         bool ok = true;
         const uint32_t acce0 = CG == 2 ? map_to_rank(smem_u32(&acce_b[0]), 0) : smem_u32(&acce_b[0]);
         for (uint32_t t = cid; ok && t < total; t += ncl) {
-            const TileF8 tc = decode_tile<TN, CG>(g, first, ends, t, rank);
+            const TileF8 tc = decode_tile<C>(g, first, ends, t);
             uint64_t acc[C::COLS / 2];
 #pragma unroll
             for (int j = 0; j < C::COLS / 2; ++j) acc[j] = 0;      // two positive zeros
@@ -443,26 +527,39 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG>::THREADS, 1)
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem + buf * TN + col0 + (quarter << 21);
-                const float* sc = ring + slot * TN + col0;
+                // TOK: a lane is a token and the warp's columns one weight block, so a scale a thread;
+                // else a scale a column, read four at a time
+                const float* sc = ring + slot * TN + (TOK ? col0 / 128 * 128 + quarter * 32 + lane : col0);
+                uint64_t one = 0;
+                if (TOK) one = pack2(*sc, *sc);
+                constexpr int CW = C::COLS < 32 ? 16 : 32, NC = C::COLS / CW;
+                uint32_t r[2][CW];
+                tmem_ld(d, r[0]);
 #pragma unroll
-                for (int c0 = 0; c0 < C::COLS; c0 += 16) {
-                    uint32_t r[16];
-                    tmem_ld16(d + c0, r);
-                    tmem_ld_done(r);
+                for (int c = 0; c < NC; ++c) {
+                    // the next columns are on their way while these are added
+                    tmem_ld_done(r[c & 1]);
+                    if (c + 1 < NC) tmem_ld(d + (c + 1) * CW, r[(c + 1) & 1]);
+                    else {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (CG == 2) mbar_arrive_cluster(acce0 + 8 * buf);
+                            else mbar_arrive(smem_u32(&acce_b[buf]));
+                        }
+                    }
+                    uint64_t* a = acc + c * CW / 2;
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        const ulonglong2 s2 = *reinterpret_cast<const ulonglong2*>(sc + c0 + j);
-                        acc[(c0 + j) / 2] = fma2(pack2(r[j], r[j + 1]), s2.x, acc[(c0 + j) / 2]);
-                        acc[(c0 + j) / 2 + 1] = fma2(pack2(r[j + 2], r[j + 3]), s2.y, acc[(c0 + j) / 2 + 1]);
+                    for (int j = 0; j < CW; j += 4) {
+                        ulonglong2 s2;
+                        if (TOK) s2 = make_ulonglong2(one, one);
+                        else s2 = *reinterpret_cast<const ulonglong2*>(sc + c * CW + j);
+                        a[j / 2] = fma2(pack2(r[c & 1][j], r[c & 1][j + 1]), s2.x, a[j / 2]);
+                        a[j / 2 + 1] = fma2(pack2(r[c & 1][j + 2], r[c & 1][j + 3]), s2.y, a[j / 2 + 1]);
                     }
                 }
-                tc_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    if (CG == 2) mbar_arrive_cluster(acce0 + 8 * buf);
-                    else mbar_arrive(smem_u32(&acce_b[buf]));
-                    mbar_arrive(smem_u32(&sempty_b[slot]));
-                }
+                if (lane == 0) mbar_arrive(smem_u32(&sempty_b[slot]));
                 if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
                 if (++slot == C::SLOTS) { slot = 0; sphase ^= 1; }
             }
@@ -478,7 +575,18 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG>::THREADS, 1)
                     part[(col0 + 2 * j + 1) * 128] = hi;
                 }
             } else if (ok) {
-                const uint32_t mrow = tc.m0 + quarter * 32 + lane;
+                if constexpr (TOK) {
+                    uint8_t* stage = (uint8_t*)bars + 512 + C::TABLES + (warp - 4) * 2048;
+                    const uint32_t row0 = tc.row0 + rank * 128 + quarter * 32, mcol = tc.m0 + col0;
+                    switch (g.c_type) {
+                        case CM_T_Q88: store_rows<int16_t>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                        case CM_T_F32: store_rows<float>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                        case CM_T_F16: store_rows<__half>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                        default: store_rows<__nv_bfloat16>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                    }
+                    continue;
+                }
+                const uint32_t mrow = tc.m0 + rank * 128 + quarter * 32 + lane;
                 switch (g.c_type) {
                     case CM_T_Q88: store_cols<int16_t, C::COLS>(g, tc, col0, mrow, acc); break;
                     case CM_T_F32: store_cols<float, C::COLS>(g, tc, col0, mrow, acc); break;
@@ -493,7 +601,7 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG>::THREADS, 1)
         __syncwarp();
         cluster_sync_all();                 // every CTA's part is written
         if (cid < total) {
-            const TileF8 tc = decode_tile<TN, CG>(g, first, ends, cid, rank);
+            const TileF8 tc = decode_tile<C>(g, first, ends, cid);
             const uint32_t lo = TN * crank / csize, hi = TN * (crank + 1) / csize;
             const uint32_t base = smem_u32(smem);
             for (uint32_t e = threadIdx.x; e < (hi - lo) * 128; e += C::THREADS) {
@@ -598,20 +706,20 @@ int make_map(CUtensorMap* map, const uint8_t* base, uint32_t k, uint64_t ld, uin
 }
 
 // Clusters of `size` CTAs of this kernel that the GPU holds at once.
-template <int TN, int CG, bool KS>
+template <int TN, int CG, bool TOK, bool KS>
 int resident_clusters(const Context* cx, uint32_t size, int* out) {
     static int known[16][9] = {};        // by device and size (function attributes are a device's own)
     const int dev = cx->device < 16 ? cx->device : 15;
     if (!known[dev][size] || dev == 15) {
-        const auto kern = gemm_f8_kernel<TN, CG, KS>;
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F8Cfg<TN, CG>::SMEM);
+        const auto kern = gemm_f8_kernel<TN, CG, TOK, KS>;
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F8Cfg<TN, CG, TOK>::SMEM);
         if (e != cudaSuccess) return cuda_error(e, "cudaFuncSetAttribute(gemm_f8)");
         int n = cx->sm_count / (int)size;
         if (size > 1) {
             cudaLaunchConfig_t q{};
             q.gridDim = dim3(size * n);
-            q.blockDim = dim3(F8Cfg<TN, CG>::THREADS);
-            q.dynamicSmemBytes = F8Cfg<TN, CG>::SMEM;
+            q.blockDim = dim3(F8Cfg<TN, CG, TOK>::THREADS);
+            q.dynamicSmemBytes = F8Cfg<TN, CG, TOK>::SMEM;
             cudaLaunchAttribute at{};
             at.id = cudaLaunchAttributeClusterDimension;
             at.val.clusterDim.x = size; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
@@ -626,16 +734,16 @@ int resident_clusters(const Context* cx, uint32_t size, int* out) {
     return CM_OK;
 }
 
-template <int TN, int CG, bool KS>
+template <int TN, int CG, bool TOK, bool KS>
 int launch_tiles(const Context* cx, const CUtensorMap& tw, const CUtensorMap& tt, const KArgs& g, uint32_t size, uint64_t most, cudaStream_t s) {
     int resident = 0;
-    int rc = resident_clusters<TN, CG, KS>(cx, size, &resident);
+    int rc = resident_clusters<TN, CG, TOK, KS>(cx, size, &resident);
     if (rc) return rc;
     const unsigned clusters = (unsigned)std::min<uint64_t>(most, KS ? most : (uint64_t)resident);
     cudaLaunchConfig_t q{};
     q.gridDim = dim3(size * clusters);
-    q.blockDim = dim3(F8Cfg<TN, CG>::THREADS);
-    q.dynamicSmemBytes = F8Cfg<TN, CG>::SMEM;
+    q.blockDim = dim3(F8Cfg<TN, CG, TOK>::THREADS);
+    q.dynamicSmemBytes = F8Cfg<TN, CG, TOK>::SMEM;
     q.stream = s;
     cudaLaunchAttribute at[2]{};
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -646,30 +754,33 @@ int launch_tiles(const Context* cx, const CUtensorMap& tw, const CUtensorMap& tt
     cudaError_t e;
     {
         ProfScope ps_(PK_FP8_GEMM, s);
-        e = cudaLaunchKernelEx(&q, gemm_f8_kernel<TN, CG, KS>, tw, tt, g);
+        e = cudaLaunchKernelEx(&q, gemm_f8_kernel<TN, CG, TOK, KS>, tw, tt, g);
     }
     count_launch();
     return e == cudaSuccess ? CM_OK : cuda_error(e, "gemm_f8 launch");
 }
 
-template <int TN, int CG>
+template <int TN, int CG, bool TOK>
 int run_tiles(const Context* cx, const uint8_t* a, uint64_t lda, const uint8_t* b, uint64_t ldb, uint64_t b_gs, const Fp8Args& f, KArgs g,
               cudaStream_t s) {
-    g.tiles_m = (f.m + 128 * CG - 1) / (128 * CG);
-    g.tiles_t = (f.n + TN - 1) / TN;
-    // a group's last tile may be partial, so grouped rows make at most n / TN + groups tiles
-    const uint64_t token_tiles = f.offsets ? std::min<uint64_t>((uint64_t)f.n / TN + f.groups, f.n) : g.tiles_t;
+    using C = F8Cfg<TN, CG, TOK>;
+    g.tiles_m = (f.m + C::WEIGHTS - 1) / C::WEIGHTS;
+    g.tiles_t = (f.n + C::TOKENS - 1) / C::TOKENS;
+    // a group's last tile may be partial, so grouped rows make at most n / TOKENS + groups tiles
+    const uint64_t token_tiles = f.offsets ? std::min<uint64_t>((uint64_t)f.n / C::TOKENS + f.groups, f.n) : g.tiles_t;
     const uint64_t most = token_tiles * g.tiles_m;
     if (most >= (1ull << 31)) return set_error(CM_EUNSUPPORTED, "cm_matmul_fp8: more than 2^31 tiles");
     g.total = (uint32_t)most;
     g.fd_m = FastDiv(g.tiles_m);
-    // D fp32; A = weights, B = tokens, both K-major; M = 128 a CTA, N = TN
-    g.idesc = (1u << 4) | (f.b_format << 7) | (f.a_format << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(CG * 128 >> 4) << 24);
+    // D fp32; M operand and N operand (weights and tokens, TOK: tokens and weights), both K-major;
+    // M = 128 a CTA, N = TN
+    const uint32_t mf = TOK ? f.a_format : f.b_format, nf = TOK ? f.b_format : f.a_format;
+    g.idesc = (1u << 4) | (mf << 7) | (nf << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(CG * 128 >> 4) << 24);
     const uint32_t stored_groups = f.offsets && b_gs ? f.groups : 1u;
     g.group_step = stored_groups > 1 ? 1u : 0u;
     CUtensorMap tw, tt;
-    int rc = make_map(&tw, b, f.k, ldb, f.m, stored_groups, stored_groups > 1 ? b_gs : (uint64_t)f.m * ldb, 128, 3);
-    if (!rc) rc = make_map(&tt, a, f.k, lda, f.n, 1, 0, TN / CG, 2);
+    int rc = make_map(&tw, b, f.k, ldb, f.m, stored_groups, stored_groups > 1 ? b_gs : (uint64_t)f.m * ldb, C::WEIGHTS / CG, 3);
+    if (!rc) rc = make_map(&tt, a, f.k, lda, f.n, 1, 0, C::TOKENS / CG, 2);
     if (rc) return rc;
     if constexpr (CG == 1) {
         // few tiles: the largest cluster whose CTAs each take at least one K block of one tile and
@@ -677,12 +788,12 @@ int run_tiles(const Context* cx, const uint8_t* a, uint64_t lda, const uint8_t* 
         for (uint32_t size = 8; size >= 2; size /= 2) {
             int resident = 0;
             if (size > g.kb || most * size > (uint64_t)cx->sm_count) continue;
-            rc = resident_clusters<TN, CG, true>(cx, size, &resident);
+            rc = resident_clusters<TN, CG, TOK, true>(cx, size, &resident);
             if (rc) return rc;
-            if (most <= (uint64_t)resident) return launch_tiles<TN, CG, true>(cx, tw, tt, g, size, most, s);
+            if (most <= (uint64_t)resident) return launch_tiles<TN, CG, TOK, true>(cx, tw, tt, g, size, most, s);
         }
     }
-    return launch_tiles<TN, CG, false>(cx, tw, tt, g, CG, most, s);
+    return launch_tiles<TN, CG, TOK, false>(cx, tw, tt, g, CG, most, s);
 }
 
 int fp8_launch(const char* who, const Context* cx, const Fp8Args& f, cudaStream_t s) {
@@ -723,11 +834,11 @@ int fp8_launch(const char* who, const Context* cx, const Fp8Args& f, cudaStream_
     const uint64_t pa = a_bytes ? k16 : lda, pb = b_bytes ? k16 : ldb, gsb = one ? 0 : b_bytes ? f.m * k16 : f.b_gs;
     // rows a weight tile meets at once: the smallest tile that holds a group's (mean) rows
     const uint64_t rows = f.offsets ? (f.n + (uint64_t)f.groups - 1) / f.groups : f.n;
-    if (rows <= 16) rc = run_tiles<16, 1>(cx, a, pa, b, pb, gsb, f, g, s);
-    else if (rows <= 32) rc = run_tiles<32, 1>(cx, a, pa, b, pb, gsb, f, g, s);
-    else if (rows <= 64) rc = run_tiles<64, 1>(cx, a, pa, b, pb, gsb, f, g, s);
-    else if (rows <= 128) rc = run_tiles<128, 1>(cx, a, pa, b, pb, gsb, f, g, s);
-    else rc = run_tiles<256, 2>(cx, a, pa, b, pb, gsb, f, g, s);
+    if (rows <= 16) rc = run_tiles<16, 1, false>(cx, a, pa, b, pb, gsb, f, g, s);
+    else if (rows <= 32) rc = run_tiles<32, 1, false>(cx, a, pa, b, pb, gsb, f, g, s);
+    else if (rows <= 64) rc = run_tiles<64, 1, false>(cx, a, pa, b, pb, gsb, f, g, s);
+    else if (rows <= 128) rc = run_tiles<128, 1, false>(cx, a, pa, b, pb, gsb, f, g, s);
+    else rc = run_tiles<256, 2, true>(cx, a, pa, b, pb, gsb, f, g, s);
     scratch_free(scratch, s);
     if (rc) return rc;
     cudaError_t e = cudaGetLastError();
