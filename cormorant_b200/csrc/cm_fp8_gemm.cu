@@ -9,7 +9,7 @@
 // token costs a 16-column tile instead of a 128-row one, and an output column is 32 neighbouring
 // lanes: its stores are whole sectors.  A block's product is a fresh accumulator (4 MMAs, 32 deep);
 // epilogue warps take it out of TMEM and add it, times token scale * weight scale, to fp32 sums in
-// registers, two columns an instruction, while the next blocks' MMAs run into other TMEM buffers.
+// registers while the next blocks' MMAs run into other TMEM buffers.
 //
 // Warps: 0 TMA producer, 1 MMA issuer (of the pair's leader), 2-3 token scales (global memory ->
 // times the weight scale -> a ring in shared memory), 4.. epilogue.  Every mbarrier wait is bounded
@@ -60,9 +60,15 @@ struct F8Cfg {
     static constexpr int A_TILE = 128 * 128, B_TILE = TN / CG * 128;
     static constexpr int STAGE = A_TILE + B_TILE;
     static constexpr int STAGES = TN >= 128 ? 6 : TN == 64 ? 8 : TN == 32 ? 9 : 10;
-    static constexpr int NBUF = TN == 256 ? 2 : 4;           // accumulators in TMEM
+    // TOK: a block's product is made in two halves of 128 columns, one for each four epilogue warps,
+    // each with two accumulators: four MMA halves pass between a half's end and the next that needs
+    // its accumulator, which covers the way to the epilogue and back (256-column accumulators, of
+    // which only two fit TMEM, left the tensor cores waiting)
+    static constexpr int HALVES = TOK ? 2 : 1;
+    static constexpr int MMA_N = TN / HALVES;
+    static constexpr int NBUF = 4;                           // accumulators in TMEM
     static constexpr int SLOTS = 8;                          // scale ring
-    static constexpr uint32_t TMEM_COLS = NBUF * TN;
+    static constexpr uint32_t TMEM_COLS = NBUF * MMA_N;
     static constexpr int TABLES = (2 * (kMaxGroups + 1) * 4 + 15) / 16 * 16;
     static_assert((STAGES * STAGE + SLOTS * TN * 4) % 16 == 0, "what follows the ring is 16-byte aligned");
     static constexpr int OUT = TOK ? EPI_WARPS * 2048 : 0;   // output staging: 32 rows x 64 bytes a warp
@@ -145,6 +151,20 @@ __device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[32]) {
 #undef CM_IO
 #undef CM_8
 
+// One thread of a converged warp.  The compiler knows that a branch on it holds one thread and keeps
+// the operands of the MMA and copy instructions in uniform registers; behind `lane == 0` it moves
+// them there for every instruction (measured: 4 MMAs and their commit take 157 cycles to issue
+// behind an elected branch, 817 behind a comparison, whatever the tile's width).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
+}
+
 struct TileF8 {
     uint32_t m0;             // first weight row
     uint32_t row0, row1;     // token rows row0 .. row1 - 1, at most a tile's used
@@ -183,18 +203,14 @@ __device__ __forceinline__ TileF8 decode_tile(const KArgs& g, const uint32_t* fi
 }
 
 template <typename T, int COLS>
-__device__ __forceinline__ void store_cols(const KArgs& g, const TileF8& tc, uint32_t col0, uint32_t mrow, const uint64_t (&acc)[COLS / 2]) {
+__device__ __forceinline__ void store_cols(const KArgs& g, const TileF8& tc, uint32_t col0, uint32_t mrow, const float (&acc)[COLS]) {
     if (mrow >= g.m) return;
     const uint32_t tok = tc.row0 + col0;
     T* p = (T*)g.c + (uint64_t)tok * g.ldc + mrow;
     const uint32_t live = tc.row1 > tok ? tc.row1 - tok : 0u;
 #pragma unroll
-    for (uint32_t j = 0; j < COLS / 2; ++j) {
-        float lo, hi;
-        unpack2(acc[j], lo, hi);
-        if (2 * j < live) from_f32(lo, *p);
-        p += g.ldc;
-        if (2 * j + 1 < live) from_f32(hi, *p);
+    for (uint32_t j = 0; j < COLS; ++j) {
+        if (j < live) from_f32(acc[j], *p);
         p += g.ldc;
     }
 }
@@ -204,7 +220,7 @@ __device__ __forceinline__ void store_cols(const KArgs& g, const TileF8& tc, uin
 // 64-byte runs of eight rows instead of 16 bytes of 32.
 template <typename T>
 __device__ __forceinline__ void store_rows(const KArgs& g, uint32_t row0, uint32_t row1, uint32_t mcol, uint8_t* stage, uint32_t lane,
-                                           const uint64_t (&acc)[64]) {
+                                           const float (&acc)[128]) {
     constexpr uint32_t W = 64 / sizeof(T);           // columns of a pass
     const bool vec = (uintptr_t)g.c % 16 == 0 && g.ldc * sizeof(T) % 16 == 0;
 #pragma unroll
@@ -218,12 +234,7 @@ __device__ __forceinline__ void store_rows(const KArgs& g, uint32_t row0, uint32
                 uint4 u;
             } o;
 #pragma unroll
-            for (uint32_t j = 0; j < W / 4; j += 2) {
-                float lo, hi;
-                unpack2(acc[(c0 + p * (W / 4) + j) / 2], lo, hi);
-                from_f32(lo, o.t[j]);
-                from_f32(hi, o.t[j + 1]);
-            }
+            for (uint32_t j = 0; j < W / 4; ++j) from_f32(acc[c0 + p * (W / 4) + j], o.t[j]);
             *reinterpret_cast<uint4*>(stage + lane * 64 + ((p ^ (lane >> 1)) & 3) * 16) = o.u;
         }
         __syncwarp();
@@ -312,7 +323,7 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
         }
         for (int b = 0; b < C::NBUF; ++b) {
             mbar_init(smem_u32(&accf_b[b]), 1);
-            mbar_init(smem_u32(&acce_b[b]), C::EPI_WARPS * CG);
+            mbar_init(smem_u32(&acce_b[b]), C::EPI_WARPS / C::HALVES * CG);
         }
         for (int s = 0; s < C::SLOTS; ++s) {
             mbar_init(smem_u32(&sfull_b[s]), 1);
@@ -377,7 +388,7 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
     // each role moves its registers: 168 a thread at launch, 128 x 56 + 256 x 224 = 384 x 168
     if (warp == 0) {
         if constexpr (C::SPLIT_REGS) fewer_regs();
-        if (lane == 0) {
+        if (elect_one()) {
             uint32_t s = 0, phase = 1, it = 0;
             bool ok = true;
             for (uint32_t t = cid; ok && t < total; t += ncl) {
@@ -388,11 +399,12 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                     if (CG == 2) {
                         const uint32_t full = map_to_rank(smem_u32(&full_b[s]), 0);
                         if (leader) mbar_expect_tx(smem_u32(&full_b[s]), 2 * C::STAGE);
-                        // each CTA its 128 rows of the M operand and its half of the N operand
-                        const uint32_t w = TOK ? C::A_TILE : 0, x = TOK ? 0 : C::A_TILE;
-                        tma_load_3d_pair(st + w, &tmW, full, (int)(kb * 128), (int)(tc.m0 + rank * (C::WEIGHTS / 2)),
-                                         (int)(tc.group * g.group_step));
-                        tma_load_2d_pair(st + x, &tmT, full, (int)(kb * 128), (int)(tc.row0 + rank * (C::TOKENS / 2)));
+                        // each CTA its 128 rows of the M operand and, of each half of the N operand, its 64
+                        tma_load_2d_pair(st, &tmT, full, (int)(kb * 128), (int)(tc.row0 + rank * 128));
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h)
+                            tma_load_3d_pair(st + C::A_TILE + h * 8192, &tmW, full, (int)(kb * 128), (int)(tc.m0 + h * 128 + rank * 64),
+                                             (int)(tc.group * g.group_step));
                     } else {
                         const uint32_t full = smem_u32(&full_b[s]);
                         mbar_expect_tx(full, C::STAGE);
@@ -412,31 +424,29 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
         }
     } else if (warp == 1) {
         if constexpr (C::SPLIT_REGS) fewer_regs();
-        if (lane == 0 && leader) {
+        if (leader && elect_one()) {
             uint32_t s = 0, phase = 0, buf = 0, bphase = 1;
             bool ok = true;
             for (uint32_t t = cid; ok && t < total; t += ncl) {
-                for (uint32_t kb = kb0; kb < kb1; ++kb) {
-                    if (!mbar_wait(smem_u32(&acce_b[buf]), bphase, wc) || !mbar_wait(smem_u32(&full_b[s]), phase, wc)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
+                for (uint32_t kb = kb0; ok && kb < kb1; ++kb) {
+                    if (!(ok = mbar_wait(smem_u32(&full_b[s]), phase, wc))) break;
                     const uint64_t da = sdesc(smem_u32(smem + s * C::STAGE)), db = sdesc(smem_u32(smem + s * C::STAGE + C::A_TILE));
-                    const uint32_t d = tmem + buf * TN;
                     const uint32_t steps = g.ksteps - kb * 4;        // 32-deep steps with any column below k
 #pragma unroll
-                    for (uint32_t kk = 0; kk < 4; ++kk)
-                        if (kk < steps) umma_f8<CG>(d, da + 2 * kk, db + 2 * kk, g.idesc, kk != 0);
-                    if (CG == 2) {
-                        umma_commit_pair(smem_u32(&empty_b[s]), kPairMask);
-                        umma_commit_pair(smem_u32(&accf_b[buf]), kPairMask);
-                    } else {
-                        umma_commit(smem_u32(&empty_b[s]));
-                        umma_commit(smem_u32(&accf_b[buf]));
+                    for (uint32_t h = 0; h < C::HALVES; ++h) {
+                        if (!(ok = mbar_wait(smem_u32(&acce_b[buf]), bphase, wc))) break;
+                        tc_fence_after();
+                        const uint32_t d = tmem + buf * C::MMA_N;
+#pragma unroll
+                        for (uint32_t kk = 0; kk < 4; ++kk)
+                            if (kk < steps) umma_f8<CG>(d, da + 2 * kk, db + h * (8192 >> 4) + 2 * kk, g.idesc, kk != 0);
+                        if (CG == 2) umma_commit_pair(smem_u32(&accf_b[buf]), kPairMask);
+                        else umma_commit(smem_u32(&accf_b[buf]));
+                        if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
                     }
+                    if (CG == 2) umma_commit_pair(smem_u32(&empty_b[s]), kPairMask);
+                    else umma_commit(smem_u32(&empty_b[s]));
                     if (++s == C::STAGES) { s = 0; phase ^= 1; }
-                    if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
                 }
             }
             // every MMA issued by this thread has completed once `done` fires
@@ -513,25 +523,24 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
     } else {
         if constexpr (C::SPLIT_REGS) more_regs();
         const uint32_t quarter = warp & 3u, col0 = (warp - 4) / 4 * C::COLS;
-        uint32_t buf = 0, bphase = 0, slot = 0, sphase = 0;
+        uint32_t buf = TOK ? (warp - 4) / 4 : 0, bphase = 0, slot = 0, sphase = 0;
         bool ok = true;
         const uint32_t acce0 = CG == 2 ? map_to_rank(smem_u32(&acce_b[0]), 0) : smem_u32(&acce_b[0]);
         for (uint32_t t = cid; ok && t < total; t += ncl) {
             const TileF8 tc = decode_tile<C>(g, first, ends, t);
-            uint64_t acc[C::COLS / 2];
+            float acc[C::COLS];
 #pragma unroll
-            for (int j = 0; j < C::COLS / 2; ++j) acc[j] = 0;      // two positive zeros
+            for (int j = 0; j < C::COLS; ++j) acc[j] = 0.0f;
             for (uint32_t kb = kb0; kb < kb1; ++kb) {
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sfull_b[slot]), sphase, wc) &&
                                                  mbar_wait(smem_u32(&accf_b[buf]), bphase, wc));
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t d = tmem + buf * TN + col0 + (quarter << 21);
+                const uint32_t d = tmem + buf * C::MMA_N + (TOK ? 0 : col0) + (quarter << 21);
                 // TOK: a lane is a token and the warp's columns one weight block, so a scale a thread;
                 // else a scale a column, read four at a time
                 const float* sc = ring + slot * TN + (TOK ? col0 / 128 * 128 + quarter * 32 + lane : col0);
-                uint64_t one = 0;
-                if (TOK) one = pack2(*sc, *sc);
+                const float one = TOK ? *sc : 0.0f;
                 constexpr int CW = C::COLS < 32 ? 16 : 32, NC = C::COLS / CW;
                 uint32_t r[2][CW];
                 tmem_ld(d, r[0]);
@@ -548,19 +557,19 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                             else mbar_arrive(smem_u32(&acce_b[buf]));
                         }
                     }
-                    uint64_t* a = acc + c * CW / 2;
 #pragma unroll
                     for (int j = 0; j < CW; j += 4) {
-                        ulonglong2 s2;
-                        if (TOK) s2 = make_ulonglong2(one, one);
-                        else s2 = *reinterpret_cast<const ulonglong2*>(sc + c * CW + j);
-                        a[j / 2] = fma2(pack2(r[c & 1][j], r[c & 1][j + 1]), s2.x, a[j / 2]);
-                        a[j / 2 + 1] = fma2(pack2(r[c & 1][j + 2], r[c & 1][j + 3]), s2.y, a[j / 2 + 1]);
+                        const float4 s4 = TOK ? make_float4(one, one, one, one) : *reinterpret_cast<const float4*>(sc + c * CW + j);
+                        float* a = acc + c * CW + j;
+                        a[0] = fmaf(__uint_as_float(r[c & 1][j]), s4.x, a[0]);
+                        a[1] = fmaf(__uint_as_float(r[c & 1][j + 1]), s4.y, a[1]);
+                        a[2] = fmaf(__uint_as_float(r[c & 1][j + 2]), s4.z, a[2]);
+                        a[3] = fmaf(__uint_as_float(r[c & 1][j + 3]), s4.w, a[3]);
                     }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sempty_b[slot]));
-                if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
+                if ((buf += C::HALVES) >= C::NBUF) { buf -= C::NBUF; bphase ^= 1; }
                 if (++slot == C::SLOTS) { slot = 0; sphase ^= 1; }
             }
             if (KS) {
@@ -568,12 +577,7 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                 // the MMAs that read them are complete (this tile is the CTA's only one)
                 float* part = (float*)smem + quarter * 32 + lane;
 #pragma unroll
-                for (int j = 0; j < C::COLS / 2; ++j) {
-                    float lo, hi;
-                    unpack2(acc[j], lo, hi);
-                    part[(col0 + 2 * j) * 128] = lo;
-                    part[(col0 + 2 * j + 1) * 128] = hi;
-                }
+                for (int j = 0; j < C::COLS; ++j) part[(col0 + j) * 128] = acc[j];
             } else if (ok) {
                 if constexpr (TOK) {
                     uint8_t* stage = (uint8_t*)bars + 512 + C::TABLES + (warp - 4) * 2048;
@@ -773,13 +777,13 @@ int run_tiles(const Context* cx, const uint8_t* a, uint64_t lda, const uint8_t* 
     g.total = (uint32_t)most;
     g.fd_m = FastDiv(g.tiles_m);
     // D fp32; M operand and N operand (weights and tokens, TOK: tokens and weights), both K-major;
-    // M = 128 a CTA, N = TN
+    // M = 128 a CTA
     const uint32_t mf = TOK ? f.a_format : f.b_format, nf = TOK ? f.b_format : f.a_format;
-    g.idesc = (1u << 4) | (mf << 7) | (nf << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(CG * 128 >> 4) << 24);
+    g.idesc = (1u << 4) | (mf << 7) | (nf << 10) | ((uint32_t)(C::MMA_N >> 3) << 17) | ((uint32_t)(CG * 128 >> 4) << 24);
     const uint32_t stored_groups = f.offsets && b_gs ? f.groups : 1u;
     g.group_step = stored_groups > 1 ? 1u : 0u;
     CUtensorMap tw, tt;
-    int rc = make_map(&tw, b, f.k, ldb, f.m, stored_groups, stored_groups > 1 ? b_gs : (uint64_t)f.m * ldb, C::WEIGHTS / CG, 3);
+    int rc = make_map(&tw, b, f.k, ldb, f.m, stored_groups, stored_groups > 1 ? b_gs : (uint64_t)f.m * ldb, TOK ? 64 : 128, 3);
     if (!rc) rc = make_map(&tt, a, f.k, lda, f.n, 1, 0, C::TOKENS / CG, 2);
     if (rc) return rc;
     if constexpr (CG == 1) {
