@@ -60,15 +60,10 @@ struct F8Cfg {
     static constexpr int A_TILE = 128 * 128, B_TILE = TN / CG * 128;
     static constexpr int STAGE = A_TILE + B_TILE;
     static constexpr int STAGES = TN >= 128 ? 6 : TN == 64 ? 8 : TN == 32 ? 9 : 10;
-    // TOK: a block's product is made in two halves of 128 columns, one for each four epilogue warps,
-    // each with two accumulators: four MMA halves pass between a half's end and the next that needs
-    // its accumulator, which covers the way to the epilogue and back (256-column accumulators, of
-    // which only two fit TMEM, left the tensor cores waiting)
-    static constexpr int HALVES = TOK ? 2 : 1;
-    static constexpr int MMA_N = TN / HALVES;
-    static constexpr int NBUF = 4;                           // accumulators in TMEM
-    static constexpr int SLOTS = 8;                          // scale ring
-    static constexpr uint32_t TMEM_COLS = NBUF * MMA_N;
+    static constexpr int NBUF = TN == 256 ? 2 : 4;           // accumulators in TMEM
+    static constexpr int SLOTS = 8;                          // scale ring: K blocks, in groups of 4 with a barrier each way
+    static constexpr int GROUPS = SLOTS / 4;
+    static constexpr uint32_t TMEM_COLS = NBUF * TN;
     static constexpr int TABLES = (2 * (kMaxGroups + 1) * 4 + 15) / 16 * 16;
     static_assert((STAGES * STAGE + SLOTS * TN * 4) % 16 == 0, "what follows the ring is 16-byte aligned");
     static constexpr int OUT = TOK ? EPI_WARPS * 2048 : 0;   // output staging: 32 rows x 64 bytes a warp
@@ -163,6 +158,30 @@ __device__ __forceinline__ bool elect_one() {
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(r));
     return r != 0;
+}
+
+// An arrival by the lanes with `on`, without a branch; on a barrier of this CTA, or of the cluster
+// (a shared::cluster address).
+__device__ __forceinline__ void arrive_if(bool on, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar), "r"((uint32_t)on)
+                 : "memory");
+}
+__device__ __forceinline__ void arrive_cluster_if(bool on, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar), "r"((uint32_t)on)
+                 : "memory");
+}
+
+// Whether the phase is complete, without waiting (try_wait may hold the thread for a while).
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 
 struct TileF8 {
@@ -297,8 +316,8 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
     uint64_t* accf_b = empty_b + C::STAGES;
     uint64_t* acce_b = accf_b + C::NBUF;
     uint64_t* sfull_b = acce_b + C::NBUF;
-    uint64_t* sempty_b = sfull_b + C::SLOTS;
-    uint64_t* done_b = sempty_b + C::SLOTS;
+    uint64_t* sempty_b = sfull_b + C::GROUPS;
+    uint64_t* done_b = sempty_b + C::GROUPS;
     volatile uint32_t* tmem_slot = (volatile uint32_t*)(done_b + 1);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     uint32_t* first = (uint32_t*)((uint8_t*)bars + 512);      // grouped: first token tile of each group
@@ -323,10 +342,10 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
         }
         for (int b = 0; b < C::NBUF; ++b) {
             mbar_init(smem_u32(&accf_b[b]), 1);
-            mbar_init(smem_u32(&acce_b[b]), C::EPI_WARPS / C::HALVES * CG);
+            mbar_init(smem_u32(&acce_b[b]), C::EPI_WARPS * CG);
         }
-        for (int s = 0; s < C::SLOTS; ++s) {
-            mbar_init(smem_u32(&sfull_b[s]), 1);
+        for (int s = 0; s < C::GROUPS; ++s) {
+            mbar_init(smem_u32(&sfull_b[s]), 2);
             mbar_init(smem_u32(&sempty_b[s]), C::EPI_WARPS);
         }
         mbar_init(smem_u32(done_b), 1);
@@ -399,12 +418,9 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                     if (CG == 2) {
                         const uint32_t full = map_to_rank(smem_u32(&full_b[s]), 0);
                         if (leader) mbar_expect_tx(smem_u32(&full_b[s]), 2 * C::STAGE);
-                        // each CTA its 128 rows of the M operand and, of each half of the N operand, its 64
+                        // each CTA its 128 rows of the M operand and its half of the N operand
                         tma_load_2d_pair(st, &tmT, full, (int)(kb * 128), (int)(tc.row0 + rank * 128));
-#pragma unroll
-                        for (uint32_t h = 0; h < 2; ++h)
-                            tma_load_3d_pair(st + C::A_TILE + h * 8192, &tmW, full, (int)(kb * 128), (int)(tc.m0 + h * 128 + rank * 64),
-                                             (int)(tc.group * g.group_step));
+                        tma_load_3d_pair(st + C::A_TILE, &tmW, full, (int)(kb * 128), (int)(tc.m0 + rank * 128), (int)(tc.group * g.group_step));
                     } else {
                         const uint32_t full = smem_u32(&full_b[s]);
                         mbar_expect_tx(full, C::STAGE);
@@ -425,28 +441,35 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
     } else if (warp == 1) {
         if constexpr (C::SPLIT_REGS) fewer_regs();
         if (leader && elect_one()) {
+            // What a block's MMAs need is worked out before the wait for its accumulator, which is the
+            // short side of the loop: descriptors advance by a stage, barriers by their address.
+            constexpr uint32_t DSTEP = C::STAGE >> 4;
+            const uint64_t da0 = sdesc(smem_u32(smem)), db0 = sdesc(smem_u32(smem + C::A_TILE));
             uint32_t s = 0, phase = 0, buf = 0, bphase = 1;
             bool ok = true;
             for (uint32_t t = cid; ok && t < total; t += ncl) {
-                for (uint32_t kb = kb0; ok && kb < kb1; ++kb) {
-                    if (!(ok = mbar_wait(smem_u32(&full_b[s]), phase, wc))) break;
-                    const uint64_t da = sdesc(smem_u32(smem + s * C::STAGE)), db = sdesc(smem_u32(smem + s * C::STAGE + C::A_TILE));
-                    const uint32_t steps = g.ksteps - kb * 4;        // 32-deep steps with any column below k
+                for (uint32_t steps = g.ksteps - kb0 * 4, left = kb1 - kb0; left; --left, steps -= 4) {
+                    const uint64_t da = da0 + s * DSTEP, db = db0 + s * DSTEP;
+                    const uint32_t d = tmem + buf * TN, full = smem_u32(&full_b[s]), empty = smem_u32(&empty_b[s]);
+                    const uint32_t accf = smem_u32(&accf_b[buf]), acce = smem_u32(&acce_b[buf]);
+                    if (!mbar_test(full, phase) && !mbar_wait(full, phase, wc)) { ok = false; break; }
+                    if (!mbar_test(acce, bphase) && !mbar_wait(acce, bphase, wc)) { ok = false; break; }
+                    tc_fence_after();
+                    if (steps >= 4) {
 #pragma unroll
-                    for (uint32_t h = 0; h < C::HALVES; ++h) {
-                        if (!(ok = mbar_wait(smem_u32(&acce_b[buf]), bphase, wc))) break;
-                        tc_fence_after();
-                        const uint32_t d = tmem + buf * C::MMA_N;
-#pragma unroll
-                        for (uint32_t kk = 0; kk < 4; ++kk)
-                            if (kk < steps) umma_f8<CG>(d, da + 2 * kk, db + h * (8192 >> 4) + 2 * kk, g.idesc, kk != 0);
-                        if (CG == 2) umma_commit_pair(smem_u32(&accf_b[buf]), kPairMask);
-                        else umma_commit(smem_u32(&accf_b[buf]));
-                        if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
+                        for (uint32_t kk = 0; kk < 4; ++kk) umma_f8<CG>(d, da + 2 * kk, db + 2 * kk, g.idesc, kk != 0);
+                    } else {                        // the last block's 32-deep steps with any column below k
+                        for (uint32_t kk = 0; kk < steps; ++kk) umma_f8<CG>(d, da + 2 * kk, db + 2 * kk, g.idesc, kk != 0);
                     }
-                    if (CG == 2) umma_commit_pair(smem_u32(&empty_b[s]), kPairMask);
-                    else umma_commit(smem_u32(&empty_b[s]));
+                    if (CG == 2) {
+                        umma_commit_pair(accf, kPairMask);
+                        umma_commit_pair(empty, kPairMask);
+                    } else {
+                        umma_commit(accf);
+                        umma_commit(empty);
+                    }
                     if (++s == C::STAGES) { s = 0; phase ^= 1; }
+                    if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
                 }
             }
             // every MMA issued by this thread has completed once `done` fires
@@ -457,8 +480,9 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
             mbar_wait(smem_u32(done_b), 0, drain);
         }
     } else if (warp < 4) {
-        // Scale warps: 2 takes the even (tile, K block) items of this CTA, 3 the odd ones.
         if constexpr (C::SPLIT_REGS) fewer_regs();
+        // Scale warps: of the (tile, K block) items of this CTA, in groups of four, 2 takes the even
+        // ones and 3 the odd ones; the next group's loads are in flight while this one waits for room.
         constexpr uint32_t AHEAD = 2;
         ScaleRegs<TN, TOK> regs[AHEAD];
         uint32_t t = cid, kb = kb0;
@@ -488,89 +512,166 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                 r.v[i] = (TOK || j < TN) && tc.row0 + j < tc.row1 ? __ldg(p + j) : 0.0f;
             }
         };
-        uint32_t item = warp - 2;
-        advance(item);
+        advance(warp - 2);
         bool have[AHEAD];
-#pragma unroll
-        for (uint32_t p = 0; p < AHEAD; ++p) {
-            have[p] = t < total;
-            if (have[p]) { load(regs[p]); advance(2); }
-        }
-        bool ok = true;
-        while (ok && have[0]) {
+        auto fetch = [&]() {
 #pragma unroll
             for (uint32_t p = 0; p < AHEAD; ++p) {
-                if (ok && have[p]) {
-                    const uint32_t slot = item % C::SLOTS, use = item / C::SLOTS;
-                    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sempty_b[slot]), (use & 1u) ^ 1u, wc));
-                    if (ok) {
+                have[p] = t < total;
+                if (have[p]) { load(regs[p]); advance(2); }
+            }
+        };
+        // groups: this CTA's tiles times its K blocks, in fours (the last one may be partial)
+        const uint64_t items = (uint64_t)(cid < total ? (total - cid + ncl - 1) / ncl : 0u) * (kb1 - kb0);
+        fetch();
+        for (uint64_t grp = 0; grp * 4 < items; ++grp) {
+            const uint32_t gs = (uint32_t)grp % C::GROUPS, use = (uint32_t)(grp / C::GROUPS);
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sempty_b[gs]), (use & 1u) ^ 1u, wc))) break;
 #pragma unroll
-                        for (uint32_t i = 0; i < sizeof(regs[p].v) / 4; ++i) {
-                            const uint32_t j = lane + 32 * i;
+            for (uint32_t p = 0; p < AHEAD; ++p) {
+                float* dst = ring + (gs * 4 + 2 * p + warp - 2) * TN;
+                if (have[p]) {
 #pragma unroll
-                            for (uint32_t h = 0; h < sizeof(regs[p].sb) / 4; ++h)
-                                if (TOK || j < TN) ring[slot * TN + h * 128 + j] = regs[p].v[i] * regs[p].sb[h];
-                        }
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&sfull_b[slot]));
-                        item += 2;
-                        have[p] = t < total;
-                        if (have[p]) { load(regs[p]); advance(2); }
+                    for (uint32_t i = 0; i < sizeof(regs[p].v) / 4; ++i) {
+                        const uint32_t j = lane + 32 * i;
+#pragma unroll
+                        for (uint32_t h = 0; h < sizeof(regs[p].sb) / 4; ++h)
+                            if (TOK || j < TN) dst[h * 128 + j] = regs[p].v[i] * regs[p].sb[h];
                     }
                 }
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sfull_b[gs]));
+            fetch();
+        }
+    } else if constexpr (TOK) {
+        // A lane is a token row and the warp's 128 columns are one weight block, so a block's scale is
+        // one number a thread.
+        //
+        // 128 sums leave registers for half of a block's columns.  The second half is fetched as the
+        // first is added, the accumulator is given back when it is here, and the next block's first
+        // half is fetched while it is added.  Everything in shared memory answers
+        // slowly while the tensor cores read their operands there (a barrier test takes some 200
+        // cycles), so the next block's accumulator and scale are asked for at the top of this one.
+        more_regs();
+        constexpr int CW = 32;
+        const uint32_t quarter = warp & 3u, half = (warp - 4) / 4;
+        const uint32_t acce0 = map_to_rank(smem_u32(&acce_b[0]), 0), accf0 = smem_u32(&accf_b[0]);
+        const uint32_t d0 = tmem + half * 128 + (quarter << 21);
+        const float* sc = ring + half * 128 + quarter * 32 + lane;
+        uint32_t buf = 0, bphase = 0, slot = 0, sphase = 0;
+        bool ok = true;
+        for (uint32_t t = cid; t < total; t += ncl) {
+            float acc[128];
+#pragma unroll
+            for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+            uint32_t r0[CW], r1[CW];
+            // Between a load and its wait there are only additions and barrier tests: nothing that makes
+            // the compiler move a register that the load still writes.
+            auto scale_there = [&]() {            // scales come in groups of four
+                if (slot % 4 == 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sfull_b[slot / 4]), sphase, wc));
+            };
+            auto columns_there = [&]() {
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(accf0 + 8 * buf, bphase, wc));
+                tc_fence_after();
+            };
+            scale_there();
+            columns_there();
+            if (!ok) break;
+            float one = sc[slot * TN];
+            tmem_ld(d0 + buf * TN, r0);
+            tmem_ld(d0 + buf * TN + CW, r1);
+            auto add = [&](int c, const uint32_t (&r)[CW]) {
+#pragma unroll
+                for (int j = 0; j < CW; ++j) acc[c * CW + j] = fmaf(__uint_as_float(r[j]), one, acc[c * CW + j]);
+            };
+            for (uint32_t left = g.kb; left; --left) {
+                const uint32_t d = d0 + buf * TN, acce = acce0 + 8 * buf, sempty = smem_u32(&sempty_b[slot / 4]);
+                const bool last_of_group = slot % 4 == 3;
+                buf ^= 1u;
+                bphase ^= buf ^ 1u;
+                if (++slot == C::SLOTS) { slot = 0; sphase ^= 1u; }
+                const bool early = mbar_test(accf0 + 8 * buf, bphase);
+                float next = 0.0f;
+                if (left > 1) {
+                    scale_there();
+                    next = sc[slot * TN];
+                }
+                tmem_ld_done(r0);
+                tmem_ld_done(r1);
+                add(0, r0);
+                tmem_ld(d + 2 * CW, r0);
+                add(1, r1);
+                tmem_ld(d + 3 * CW, r1);
+                tmem_ld_done(r0);
+                tmem_ld_done(r1);
+                tc_fence_before();
+                __syncwarp();
+                arrive_cluster_if(lane == 0, acce);                  // the accumulator's columns are in registers
+                arrive_if(lane == 0 && last_of_group, sempty);       // and so is the group's last scale
+                add(2, r0);
+                if (left > 1) {
+                    if (__all_sync(0xffffffffu, early)) tc_fence_after();
+                    else columns_there();
+                    if (!ok) break;
+                    tmem_ld(d0 + buf * TN, r0);
+                }
+                add(3, r1);
+                if (left > 1) tmem_ld(d0 + buf * TN + CW, r1);
+                one = next;
+            }
+            if (!ok) break;
+            const TileF8 tc = decode_tile<C>(g, first, ends, t);
+            uint8_t* stage = (uint8_t*)bars + 512 + C::TABLES + (warp - 4) * 2048;
+            const uint32_t row0 = tc.row0 + rank * 128 + quarter * 32, mcol = tc.m0 + half * C::COLS;
+            switch (g.c_type) {
+                case CM_T_Q88: store_rows<int16_t>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                case CM_T_F32: store_rows<float>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                case CM_T_F16: store_rows<__half>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                default: store_rows<__nv_bfloat16>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+            }
         }
     } else {
-        if constexpr (C::SPLIT_REGS) more_regs();
         const uint32_t quarter = warp & 3u, col0 = (warp - 4) / 4 * C::COLS;
-        uint32_t buf = TOK ? (warp - 4) / 4 : 0, bphase = 0, slot = 0, sphase = 0;
+        uint32_t buf = 0, bphase = 0, item = 0;
         bool ok = true;
-        const uint32_t acce0 = CG == 2 ? map_to_rank(smem_u32(&acce_b[0]), 0) : smem_u32(&acce_b[0]);
+        constexpr int CW = C::COLS < 32 ? 16 : 32, NC = C::COLS / CW;
+        static_assert(NC == 1 || NC == 2, "chunks of a warp's columns");
         for (uint32_t t = cid; ok && t < total; t += ncl) {
             const TileF8 tc = decode_tile<C>(g, first, ends, t);
             float acc[C::COLS];
 #pragma unroll
             for (int j = 0; j < C::COLS; ++j) acc[j] = 0.0f;
+            uint32_t r0[CW], r1[CW];
             for (uint32_t kb = kb0; kb < kb1; ++kb) {
-                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sfull_b[slot]), sphase, wc) &&
-                                                 mbar_wait(smem_u32(&accf_b[buf]), bphase, wc));
+                const uint32_t slot = item % C::SLOTS, gs = slot / 4;
+                const bool early = mbar_test(smem_u32(&accf_b[buf]), bphase);
+                if (item % 4 == 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sfull_b[gs]), (item / C::SLOTS) & 1u, wc));
+                if (!__all_sync(0xffffffffu, early)) ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&accf_b[buf]), bphase, wc));
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t d = tmem + buf * C::MMA_N + (TOK ? 0 : col0) + (quarter << 21);
-                // TOK: a lane is a token and the warp's columns one weight block, so a scale a thread;
-                // else a scale a column, read four at a time
-                const float* sc = ring + slot * TN + (TOK ? col0 / 128 * 128 + quarter * 32 + lane : col0);
-                const float one = TOK ? *sc : 0.0f;
-                constexpr int CW = C::COLS < 32 ? 16 : 32, NC = C::COLS / CW;
-                uint32_t r[2][CW];
-                tmem_ld(d, r[0]);
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    // the next columns are on their way while these are added
-                    tmem_ld_done(r[c & 1]);
-                    if (c + 1 < NC) tmem_ld(d + (c + 1) * CW, r[(c + 1) & 1]);
-                    else {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (CG == 2) mbar_arrive_cluster(acce0 + 8 * buf);
-                            else mbar_arrive(smem_u32(&acce_b[buf]));
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < CW; j += 4) {
-                        const float4 s4 = TOK ? make_float4(one, one, one, one) : *reinterpret_cast<const float4*>(sc + c * CW + j);
-                        float* a = acc + c * CW + j;
-                        a[0] = fmaf(__uint_as_float(r[c & 1][j]), s4.x, a[0]);
-                        a[1] = fmaf(__uint_as_float(r[c & 1][j + 1]), s4.y, a[1]);
-                        a[2] = fmaf(__uint_as_float(r[c & 1][j + 2]), s4.z, a[2]);
-                        a[3] = fmaf(__uint_as_float(r[c & 1][j + 3]), s4.w, a[3]);
-                    }
-                }
+                const uint32_t d = tmem + buf * TN + col0 + (quarter << 21);
+                tmem_ld(d, r0);
+                if (NC > 1) tmem_ld(d + CW, r1);
+                tmem_ld_done(r0);
+                if (NC > 1) tmem_ld_done(r1);
+                tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sempty_b[slot]));
-                if ((buf += C::HALVES) >= C::NBUF) { buf -= C::NBUF; bphase ^= 1; }
-                if (++slot == C::SLOTS) { slot = 0; sphase ^= 1; }
+                arrive_if(lane == 0, smem_u32(&acce_b[buf]));
+                if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
+                const float* sc = ring + slot * TN + col0;       // a scale a column
+#pragma unroll
+                for (int j = 0; j < C::COLS; j += 4) {
+                    const float4 s4 = *reinterpret_cast<const float4*>(sc + j);
+                    const uint32_t* r = j < CW ? r0 + j : r1 + (j - CW);
+                    acc[j] = fmaf(__uint_as_float(r[0]), s4.x, acc[j]);
+                    acc[j + 1] = fmaf(__uint_as_float(r[1]), s4.y, acc[j + 1]);
+                    acc[j + 2] = fmaf(__uint_as_float(r[2]), s4.z, acc[j + 2]);
+                    acc[j + 3] = fmaf(__uint_as_float(r[3]), s4.w, acc[j + 3]);
+                }
+                ++item;
+                __syncwarp();
+                arrive_if(lane == 0 && item % 4 == 0, smem_u32(&sempty_b[gs]));
             }
             if (KS) {
                 // this CTA's part, [column][weight row], over the stages: their copies have landed and
@@ -579,18 +680,7 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
 #pragma unroll
                 for (int j = 0; j < C::COLS; ++j) part[(col0 + j) * 128] = acc[j];
             } else if (ok) {
-                if constexpr (TOK) {
-                    uint8_t* stage = (uint8_t*)bars + 512 + C::TABLES + (warp - 4) * 2048;
-                    const uint32_t row0 = tc.row0 + rank * 128 + quarter * 32, mcol = tc.m0 + col0;
-                    switch (g.c_type) {
-                        case CM_T_Q88: store_rows<int16_t>(g, row0, tc.row1, mcol, stage, lane, acc); break;
-                        case CM_T_F32: store_rows<float>(g, row0, tc.row1, mcol, stage, lane, acc); break;
-                        case CM_T_F16: store_rows<__half>(g, row0, tc.row1, mcol, stage, lane, acc); break;
-                        default: store_rows<__nv_bfloat16>(g, row0, tc.row1, mcol, stage, lane, acc); break;
-                    }
-                    continue;
-                }
-                const uint32_t mrow = tc.m0 + rank * 128 + quarter * 32 + lane;
+                const uint32_t mrow = tc.m0 + quarter * 32 + lane;
                 switch (g.c_type) {
                     case CM_T_Q88: store_cols<int16_t, C::COLS>(g, tc, col0, mrow, acc); break;
                     case CM_T_F32: store_cols<float, C::COLS>(g, tc, col0, mrow, acc); break;
@@ -777,13 +867,13 @@ int run_tiles(const Context* cx, const uint8_t* a, uint64_t lda, const uint8_t* 
     g.total = (uint32_t)most;
     g.fd_m = FastDiv(g.tiles_m);
     // D fp32; M operand and N operand (weights and tokens, TOK: tokens and weights), both K-major;
-    // M = 128 a CTA
+    // M = 128 a CTA, N = TN
     const uint32_t mf = TOK ? f.a_format : f.b_format, nf = TOK ? f.b_format : f.a_format;
-    g.idesc = (1u << 4) | (mf << 7) | (nf << 10) | ((uint32_t)(C::MMA_N >> 3) << 17) | ((uint32_t)(CG * 128 >> 4) << 24);
+    g.idesc = (1u << 4) | (mf << 7) | (nf << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(CG * 128 >> 4) << 24);
     const uint32_t stored_groups = f.offsets && b_gs ? f.groups : 1u;
     g.group_step = stored_groups > 1 ? 1u : 0u;
     CUtensorMap tw, tt;
-    int rc = make_map(&tw, b, f.k, ldb, f.m, stored_groups, stored_groups > 1 ? b_gs : (uint64_t)f.m * ldb, TOK ? 64 : 128, 3);
+    int rc = make_map(&tw, b, f.k, ldb, f.m, stored_groups, stored_groups > 1 ? b_gs : (uint64_t)f.m * ldb, 128, 3);
     if (!rc) rc = make_map(&tt, a, f.k, lda, f.n, 1, 0, C::TOKENS / CG, 2);
     if (rc) return rc;
     if constexpr (CG == 1) {
