@@ -50,7 +50,6 @@ struct KArgs {
 
 template <int TN, int CG, bool TOK>
 struct F8Cfg {
-    static_assert(!TOK || (TN == 256 && CG == 2), "tokens are the M operand of 256 x 256 pair tiles");
     static constexpr int EPI_WARPS = TN >= 128 ? 8 : 4;
     static constexpr int COLS = TN / (EPI_WARPS / 4);        // accumulator columns of an epilogue warp
     static constexpr int THREADS = 128 + 32 * EPI_WARPS;
@@ -287,9 +286,6 @@ __device__ __forceinline__ void store_one(const KArgs& g, uint64_t i, float v) {
     }
 }
 
-__device__ __forceinline__ void fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
-__device__ __forceinline__ void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
-
 // The token scales of one (tile, K block), as a scale warp holds them on their way from global
 // memory: the loads are issued two blocks of this warp (four of the CTA) ahead of their use.
 template <int TN, bool TOK>
@@ -404,288 +400,287 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
     const uint32_t total = g.offsets ? first[g.groups] * g.tiles_m : g.total;
     const WaitCtl wc{abort_flag, g.status, g.timeout_ns};
 
-    // each role moves its registers: 168 a thread at launch, 128 x 56 + 256 x 224 = 384 x 168
-    if (warp == 0) {
-        if constexpr (C::SPLIT_REGS) fewer_regs();
-        if (elect_one()) {
-            uint32_t s = 0, phase = 1, it = 0;
-            bool ok = true;
-            for (uint32_t t = cid; ok && t < total; t += ncl) {
-                const TileF8 tc = decode_tile<C>(g, first, ends, t);
-                for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-                    if (!mbar_wait(smem_u32(&empty_b[s]), phase, wc)) { ok = false; break; }
-                    const uint32_t st = smem_u32(smem + s * C::STAGE);
-                    if (CG == 2) {
-                        const uint32_t full = map_to_rank(smem_u32(&full_b[s]), 0);
-                        if (leader) mbar_expect_tx(smem_u32(&full_b[s]), 2 * C::STAGE);
-                        // each CTA its 128 rows of the M operand and its half of the N operand
-                        tma_load_2d_pair(st, &tmT, full, (int)(kb * 128), (int)(tc.row0 + rank * 128));
-                        tma_load_3d_pair(st + C::A_TILE, &tmW, full, (int)(kb * 128), (int)(tc.m0 + rank * 128), (int)(tc.group * g.group_step));
-                    } else {
-                        const uint32_t full = smem_u32(&full_b[s]);
-                        mbar_expect_tx(full, C::STAGE);
-                        tma_load_3d(st, &tmW, full, (int)(kb * 128), (int)tc.m0, (int)(tc.group * g.group_step));
-                        tma_load_2d(st + C::A_TILE, &tmT, full, (int)(kb * 128), (int)tc.row0);
+    // The first four warps hand registers to the epilogue warps: 168 a thread at launch,
+    // 128 x 56 + 256 x 224 = 384 x 168.  A warpgroup's warps execute one and the same instruction for
+    // it, so the roles branch after it.
+    if (warp < 4) {
+        if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0) {
+            if (elect_one()) {
+                uint32_t s = 0, phase = 1, it = 0;
+                bool ok = true;
+                for (uint32_t t = cid; ok && t < total; t += ncl) {
+                    const TileF8 tc = decode_tile<C>(g, first, ends, t);
+                    for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
+                        if (!mbar_wait(smem_u32(&empty_b[s]), phase, wc)) { ok = false; break; }
+                        const uint32_t st = smem_u32(smem + s * C::STAGE);
+                        if (CG == 2) {
+                            const uint32_t full = map_to_rank(smem_u32(&full_b[s]), 0);
+                            if (leader) mbar_expect_tx(smem_u32(&full_b[s]), 2 * C::STAGE);
+                            // each CTA its 128 rows of the M operand and its half of the N operand
+                            tma_load_2d_pair(st, &tmT, full, (int)(kb * 128), (int)(tc.row0 + rank * 128));
+                            tma_load_3d_pair(st + C::A_TILE, &tmW, full, (int)(kb * 128), (int)(tc.m0 + rank * 128), (int)(tc.group * g.group_step));
+                        } else {
+                            const uint32_t full = smem_u32(&full_b[s]);
+                            mbar_expect_tx(full, C::STAGE);
+                            tma_load_3d(st + (TOK ? C::A_TILE : 0), &tmW, full, (int)(kb * 128), (int)tc.m0, (int)(tc.group * g.group_step));
+                            tma_load_2d(st + (TOK ? 0 : C::A_TILE), &tmT, full, (int)(kb * 128), (int)tc.row0);
+                        }
+                        if (++s == C::STAGES) { s = 0; phase ^= 1; }
                     }
-                    if (++s == C::STAGES) { s = 0; phase ^= 1; }
+                }
+                if (*abort_flag && leader) {
+                    // let copies already in flight land before the CTA exits
+                    const uint32_t from = it > C::STAGES ? it - C::STAGES : 0u;
+                    volatile int never = 0;
+                    WaitCtl drain{&never, g.status, g.timeout_ns};
+                    for (uint32_t k = from; k < it; ++k) mbar_wait(smem_u32(&full_b[k % C::STAGES]), (k / C::STAGES) & 1u, drain);
                 }
             }
-            if (*abort_flag && leader) {
-                // let copies already in flight land before the CTA exits
-                const uint32_t from = it > C::STAGES ? it - C::STAGES : 0u;
+        } else if (warp == 1) {
+            if (leader && elect_one()) {
+                // What a block's MMAs need is worked out before the wait for its accumulator, which is the
+                // short side of the loop: descriptors advance by a stage, barriers by their address.
+                constexpr uint32_t DSTEP = C::STAGE >> 4;
+                const uint64_t da0 = sdesc(smem_u32(smem)), db0 = sdesc(smem_u32(smem + C::A_TILE));
+                uint32_t s = 0, phase = 0, buf = 0, bphase = 1;
+                bool ok = true;
+                for (uint32_t t = cid; ok && t < total; t += ncl) {
+                    for (uint32_t steps = g.ksteps - kb0 * 4, left = kb1 - kb0; left; --left, steps -= 4) {
+                        const uint64_t da = da0 + s * DSTEP, db = db0 + s * DSTEP;
+                        const uint32_t d = tmem + buf * TN, full = smem_u32(&full_b[s]), empty = smem_u32(&empty_b[s]);
+                        const uint32_t accf = smem_u32(&accf_b[buf]), acce = smem_u32(&acce_b[buf]);
+                        if (!mbar_test(full, phase) && !mbar_wait(full, phase, wc)) { ok = false; break; }
+                        if (!mbar_test(acce, bphase) && !mbar_wait(acce, bphase, wc)) { ok = false; break; }
+                        tc_fence_after();
+                        if (steps >= 4) {
+#pragma unroll
+                            for (uint32_t kk = 0; kk < 4; ++kk) umma_f8<CG>(d, da + 2 * kk, db + 2 * kk, g.idesc, kk != 0);
+                        } else {                        // the last block's 32-deep steps with any column below k
+                            for (uint32_t kk = 0; kk < steps; ++kk) umma_f8<CG>(d, da + 2 * kk, db + 2 * kk, g.idesc, kk != 0);
+                        }
+                        if (CG == 2) {
+                            umma_commit_pair(accf, kPairMask);
+                            umma_commit_pair(empty, kPairMask);
+                        } else {
+                            umma_commit(accf);
+                            umma_commit(empty);
+                        }
+                        if (++s == C::STAGES) { s = 0; phase ^= 1; }
+                        if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
+                    }
+                }
+                // every MMA issued by this thread has completed once `done` fires
+                if (CG == 2) umma_commit_pair(smem_u32(done_b), 0x1);
+                else umma_commit(smem_u32(done_b));
                 volatile int never = 0;
                 WaitCtl drain{&never, g.status, g.timeout_ns};
-                for (uint32_t k = from; k < it; ++k) mbar_wait(smem_u32(&full_b[k % C::STAGES]), (k / C::STAGES) & 1u, drain);
+                mbar_wait(smem_u32(done_b), 0, drain);
             }
-        }
-    } else if (warp == 1) {
-        if constexpr (C::SPLIT_REGS) fewer_regs();
-        if (leader && elect_one()) {
-            // What a block's MMAs need is worked out before the wait for its accumulator, which is the
-            // short side of the loop: descriptors advance by a stage, barriers by their address.
-            constexpr uint32_t DSTEP = C::STAGE >> 4;
-            const uint64_t da0 = sdesc(smem_u32(smem)), db0 = sdesc(smem_u32(smem + C::A_TILE));
-            uint32_t s = 0, phase = 0, buf = 0, bphase = 1;
-            bool ok = true;
-            for (uint32_t t = cid; ok && t < total; t += ncl) {
-                for (uint32_t steps = g.ksteps - kb0 * 4, left = kb1 - kb0; left; --left, steps -= 4) {
-                    const uint64_t da = da0 + s * DSTEP, db = db0 + s * DSTEP;
-                    const uint32_t d = tmem + buf * TN, full = smem_u32(&full_b[s]), empty = smem_u32(&empty_b[s]);
-                    const uint32_t accf = smem_u32(&accf_b[buf]), acce = smem_u32(&acce_b[buf]);
-                    if (!mbar_test(full, phase) && !mbar_wait(full, phase, wc)) { ok = false; break; }
-                    if (!mbar_test(acce, bphase) && !mbar_wait(acce, bphase, wc)) { ok = false; break; }
-                    tc_fence_after();
-                    if (steps >= 4) {
-#pragma unroll
-                        for (uint32_t kk = 0; kk < 4; ++kk) umma_f8<CG>(d, da + 2 * kk, db + 2 * kk, g.idesc, kk != 0);
-                    } else {                        // the last block's 32-deep steps with any column below k
-                        for (uint32_t kk = 0; kk < steps; ++kk) umma_f8<CG>(d, da + 2 * kk, db + 2 * kk, g.idesc, kk != 0);
-                    }
-                    if (CG == 2) {
-                        umma_commit_pair(accf, kPairMask);
-                        umma_commit_pair(empty, kPairMask);
-                    } else {
-                        umma_commit(accf);
-                        umma_commit(empty);
-                    }
-                    if (++s == C::STAGES) { s = 0; phase ^= 1; }
-                    if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
+        } else {
+            // Scale warps: of the (tile, K block) items of this CTA, in groups of four, 2 takes the even
+            // ones and 3 the odd ones; the next group's loads are in flight while this one waits for room.
+            constexpr uint32_t AHEAD = 2;
+            ScaleRegs<TN, TOK> regs[AHEAD];
+            uint32_t t = cid, kb = kb0;
+            TileF8 tc{};
+            const float* sbp = nullptr;
+            uint32_t blocks = 0;                 // weight blocks of this CTA's part of the tile that exist
+            bool fresh = true;
+            auto advance = [&](uint32_t by) {
+                for (uint32_t i = 0; i < by; ++i)
+                    if (++kb == kb1) { kb = kb0; t += ncl; fresh = true; }
+            };
+            auto load = [&](ScaleRegs<TN, TOK>& r) {
+                if (fresh) {
+                    tc = decode_tile<C>(g, first, ends, t);
+                    if (TOK) tc.row0 += rank * 128;
+                    else tc.m0 += rank * 128;
+                    blocks = tc.m0 < g.m ? (g.m - tc.m0 + 127) / 128 : 0u;
+                    sbp = g.bs + tc.group * g.bs_gs + (uint64_t)(tc.m0 / 128) * g.b_lds;
+                    fresh = false;
                 }
-            }
-            // every MMA issued by this thread has completed once `done` fires
-            if (CG == 2) umma_commit_pair(smem_u32(done_b), 0x1);
-            else umma_commit(smem_u32(done_b));
-            volatile int never = 0;
-            WaitCtl drain{&never, g.status, g.timeout_ns};
-            mbar_wait(smem_u32(done_b), 0, drain);
-        }
-    } else if (warp < 4) {
-        if constexpr (C::SPLIT_REGS) fewer_regs();
-        // Scale warps: of the (tile, K block) items of this CTA, in groups of four, 2 takes the even
-        // ones and 3 the odd ones; the next group's loads are in flight while this one waits for room.
-        constexpr uint32_t AHEAD = 2;
-        ScaleRegs<TN, TOK> regs[AHEAD];
-        uint32_t t = cid, kb = kb0;
-        TileF8 tc{};
-        const float* sbp = nullptr;
-        uint32_t blocks = 0;                 // weight blocks of this CTA's part of the tile that exist
-        bool fresh = true;
-        auto advance = [&](uint32_t by) {
-            for (uint32_t i = 0; i < by; ++i)
-                if (++kb == kb1) { kb = kb0; t += ncl; fresh = true; }
-        };
-        auto load = [&](ScaleRegs<TN, TOK>& r) {
-            if (fresh) {
-                tc = decode_tile<C>(g, first, ends, t);
-                if (TOK) tc.row0 += rank * 128;
-                else tc.m0 += rank * 128;
-                blocks = tc.m0 < g.m ? (g.m - tc.m0 + 127) / 128 : 0u;
-                sbp = g.bs + tc.group * g.bs_gs + (uint64_t)(tc.m0 / 128) * g.b_lds;
-                fresh = false;
-            }
 #pragma unroll
-            for (uint32_t h = 0; h < sizeof(r.sb) / 4; ++h) r.sb[h] = h < blocks ? __ldg(sbp + h * g.b_lds + kb) : 0.0f;
-            const float* p = g.as + (uint64_t)kb * g.a_lds + tc.row0;
+                for (uint32_t h = 0; h < sizeof(r.sb) / 4; ++h) r.sb[h] = h < blocks ? __ldg(sbp + h * g.b_lds + kb) : 0.0f;
+                const float* p = g.as + (uint64_t)kb * g.a_lds + tc.row0;
 #pragma unroll
-            for (uint32_t i = 0; i < sizeof(r.v) / 4; ++i) {
-                const uint32_t j = lane + 32 * i;
-                r.v[i] = (TOK || j < TN) && tc.row0 + j < tc.row1 ? __ldg(p + j) : 0.0f;
-            }
-        };
-        advance(warp - 2);
-        bool have[AHEAD];
-        auto fetch = [&]() {
-#pragma unroll
-            for (uint32_t p = 0; p < AHEAD; ++p) {
-                have[p] = t < total;
-                if (have[p]) { load(regs[p]); advance(2); }
-            }
-        };
-        // groups: this CTA's tiles times its K blocks, in fours (the last one may be partial)
-        const uint64_t items = (uint64_t)(cid < total ? (total - cid + ncl - 1) / ncl : 0u) * (kb1 - kb0);
-        fetch();
-        for (uint64_t grp = 0; grp * 4 < items; ++grp) {
-            const uint32_t gs = (uint32_t)grp % C::GROUPS, use = (uint32_t)(grp / C::GROUPS);
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sempty_b[gs]), (use & 1u) ^ 1u, wc))) break;
-#pragma unroll
-            for (uint32_t p = 0; p < AHEAD; ++p) {
-                float* dst = ring + (gs * 4 + 2 * p + warp - 2) * TN;
-                if (have[p]) {
-#pragma unroll
-                    for (uint32_t i = 0; i < sizeof(regs[p].v) / 4; ++i) {
-                        const uint32_t j = lane + 32 * i;
-#pragma unroll
-                        for (uint32_t h = 0; h < sizeof(regs[p].sb) / 4; ++h)
-                            if (TOK || j < TN) dst[h * 128 + j] = regs[p].v[i] * regs[p].sb[h];
-                    }
+                for (uint32_t i = 0; i < sizeof(r.v) / 4; ++i) {
+                    const uint32_t j = lane + 32 * i;
+                    r.v[i] = (TOK || j < TN) && tc.row0 + j < tc.row1 ? __ldg(p + j) : 0.0f;
                 }
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sfull_b[gs]));
+            };
+            advance(warp - 2);
+            bool have[AHEAD];
+            auto fetch = [&]() {
+#pragma unroll
+                for (uint32_t p = 0; p < AHEAD; ++p) {
+                    have[p] = t < total;
+                    if (have[p]) { load(regs[p]); advance(2); }
+                }
+            };
+            // groups: this CTA's tiles times its K blocks, in fours (the last one may be partial)
+            const uint64_t items = (uint64_t)(cid < total ? (total - cid + ncl - 1) / ncl : 0u) * (kb1 - kb0);
             fetch();
-        }
-    } else if constexpr (TOK) {
-        // A lane is a token row and the warp's 128 columns are one weight block, so a block's scale is
-        // one number a thread.
-        //
-        // 128 sums leave registers for half of a block's columns.  The second half is fetched as the
-        // first is added, the accumulator is given back when it is here, and the next block's first
-        // half is fetched while it is added.  Everything in shared memory answers
-        // slowly while the tensor cores read their operands there (a barrier test takes some 200
-        // cycles), so the next block's accumulator and scale are asked for at the top of this one.
-        more_regs();
-        constexpr int CW = 32;
-        const uint32_t quarter = warp & 3u, half = (warp - 4) / 4;
-        const uint32_t acce0 = map_to_rank(smem_u32(&acce_b[0]), 0), accf0 = smem_u32(&accf_b[0]);
-        const uint32_t d0 = tmem + half * 128 + (quarter << 21);
-        const float* sc = ring + half * 128 + quarter * 32 + lane;
-        uint32_t buf = 0, bphase = 0, slot = 0, sphase = 0;
-        bool ok = true;
-        for (uint32_t t = cid; t < total; t += ncl) {
-            float acc[128];
+            for (uint64_t grp = 0; grp * 4 < items; ++grp) {
+                const uint32_t gs = (uint32_t)grp % C::GROUPS, use = (uint32_t)(grp / C::GROUPS);
+                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sempty_b[gs]), (use & 1u) ^ 1u, wc))) break;
 #pragma unroll
-            for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
-            uint32_t r0[CW], r1[CW];
-            // Between a load and its wait there are only additions and barrier tests: nothing that makes
-            // the compiler move a register that the load still writes.
-            auto scale_there = [&]() {            // scales come in groups of four
-                if (slot % 4 == 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sfull_b[slot / 4]), sphase, wc));
-            };
-            auto columns_there = [&]() {
-                ok = ok && __all_sync(0xffffffffu, mbar_wait(accf0 + 8 * buf, bphase, wc));
-                tc_fence_after();
-            };
-            scale_there();
-            columns_there();
-            if (!ok) break;
-            float one = sc[slot * TN];
-            tmem_ld(d0 + buf * TN, r0);
-            tmem_ld(d0 + buf * TN + CW, r1);
-            auto add = [&](int c, const uint32_t (&r)[CW]) {
+                for (uint32_t p = 0; p < AHEAD; ++p) {
+                    float* dst = ring + (gs * 4 + 2 * p + warp - 2) * TN;
+                    if (have[p]) {
 #pragma unroll
-                for (int j = 0; j < CW; ++j) acc[c * CW + j] = fmaf(__uint_as_float(r[j]), one, acc[c * CW + j]);
-            };
-            for (uint32_t left = g.kb; left; --left) {
-                const uint32_t d = d0 + buf * TN, acce = acce0 + 8 * buf, sempty = smem_u32(&sempty_b[slot / 4]);
-                const bool last_of_group = slot % 4 == 3;
-                buf ^= 1u;
-                bphase ^= buf ^ 1u;
-                if (++slot == C::SLOTS) { slot = 0; sphase ^= 1u; }
-                const bool early = mbar_test(accf0 + 8 * buf, bphase);
-                float next = 0.0f;
-                if (left > 1) {
-                    scale_there();
-                    next = sc[slot * TN];
+                        for (uint32_t i = 0; i < sizeof(regs[p].v) / 4; ++i) {
+                            const uint32_t j = lane + 32 * i;
+#pragma unroll
+                            for (uint32_t h = 0; h < sizeof(regs[p].sb) / 4; ++h)
+                                if (TOK || j < TN) dst[h * 128 + j] = regs[p].v[i] * regs[p].sb[h];
+                        }
+                    }
                 }
-                tmem_ld_done(r0);
-                tmem_ld_done(r1);
-                add(0, r0);
-                tmem_ld(d + 2 * CW, r0);
-                add(1, r1);
-                tmem_ld(d + 3 * CW, r1);
-                tmem_ld_done(r0);
-                tmem_ld_done(r1);
-                tc_fence_before();
                 __syncwarp();
-                arrive_cluster_if(lane == 0, acce);                  // the accumulator's columns are in registers
-                arrive_if(lane == 0 && last_of_group, sempty);       // and so is the group's last scale
-                add(2, r0);
-                if (left > 1) {
-                    if (__all_sync(0xffffffffu, early)) tc_fence_after();
-                    else columns_there();
-                    if (!ok) break;
-                    tmem_ld(d0 + buf * TN, r0);
-                }
-                add(3, r1);
-                if (left > 1) tmem_ld(d0 + buf * TN + CW, r1);
-                one = next;
-            }
-            if (!ok) break;
-            const TileF8 tc = decode_tile<C>(g, first, ends, t);
-            uint8_t* stage = (uint8_t*)bars + 512 + C::TABLES + (warp - 4) * 2048;
-            const uint32_t row0 = tc.row0 + rank * 128 + quarter * 32, mcol = tc.m0 + half * C::COLS;
-            switch (g.c_type) {
-                case CM_T_Q88: store_rows<int16_t>(g, row0, tc.row1, mcol, stage, lane, acc); break;
-                case CM_T_F32: store_rows<float>(g, row0, tc.row1, mcol, stage, lane, acc); break;
-                case CM_T_F16: store_rows<__half>(g, row0, tc.row1, mcol, stage, lane, acc); break;
-                default: store_rows<__nv_bfloat16>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                if (lane == 0) mbar_arrive(smem_u32(&sfull_b[gs]));
+                fetch();
             }
         }
     } else {
-        const uint32_t quarter = warp & 3u, col0 = (warp - 4) / 4 * C::COLS;
-        uint32_t buf = 0, bphase = 0, item = 0;
-        bool ok = true;
-        constexpr int CW = C::COLS < 32 ? 16 : 32, NC = C::COLS / CW;
-        static_assert(NC == 1 || NC == 2, "chunks of a warp's columns");
-        for (uint32_t t = cid; ok && t < total; t += ncl) {
-            const TileF8 tc = decode_tile<C>(g, first, ends, t);
-            float acc[C::COLS];
+        if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        if constexpr (TOK) {
+            // A lane is a token row and the warp's 128 columns are one weight block, so a block's scale is
+            // one number a thread.
+            //
+            // 128 sums leave registers for half of a block's columns.  The second half is fetched as the
+            // first is added, the accumulator is given back when it is here, and the next block's first
+            // half is fetched while it is added.  Everything in shared memory answers
+            // slowly while the tensor cores read their operands there (a barrier test takes some 200
+            // cycles), so the next block's accumulator and scale are asked for at the top of this one.
+            constexpr int CW = 32;
+            const uint32_t quarter = warp & 3u, half = (warp - 4) / 4;
+            const uint32_t acce0 = CG == 2 ? map_to_rank(smem_u32(&acce_b[0]), 0) : smem_u32(&acce_b[0]), accf0 = smem_u32(&accf_b[0]);
+            const uint32_t d0 = tmem + half * 128 + (quarter << 21);
+            const float* sc = ring + half * 128 + quarter * 32 + lane;
+            uint32_t buf = 0, bphase = 0, slot = 0, sphase = 0;
+            bool ok = true;
+            for (uint32_t t = cid; t < total; t += ncl) {
+                float acc[128];
 #pragma unroll
-            for (int j = 0; j < C::COLS; ++j) acc[j] = 0.0f;
-            uint32_t r0[CW], r1[CW];
-            for (uint32_t kb = kb0; kb < kb1; ++kb) {
-                const uint32_t slot = item % C::SLOTS, gs = slot / 4;
-                const bool early = mbar_test(smem_u32(&accf_b[buf]), bphase);
-                if (item % 4 == 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sfull_b[gs]), (item / C::SLOTS) & 1u, wc));
-                if (!__all_sync(0xffffffffu, early)) ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&accf_b[buf]), bphase, wc));
+                for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+                uint32_t r0[CW], r1[CW];
+                // Between a load and its wait there are only additions and barrier tests: nothing that makes
+                // the compiler move a register that the load still writes.
+                auto scale_there = [&]() {            // scales come in groups of four
+                    if (slot % 4 == 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sfull_b[slot / 4]), sphase, wc));
+                };
+                auto columns_there = [&]() {
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait(accf0 + 8 * buf, bphase, wc));
+                    tc_fence_after();
+                };
+                scale_there();
+                columns_there();
                 if (!ok) break;
-                tc_fence_after();
-                const uint32_t d = tmem + buf * TN + col0 + (quarter << 21);
-                tmem_ld(d, r0);
-                if (NC > 1) tmem_ld(d + CW, r1);
-                tmem_ld_done(r0);
-                if (NC > 1) tmem_ld_done(r1);
-                tc_fence_before();
-                __syncwarp();
-                arrive_if(lane == 0, smem_u32(&acce_b[buf]));
-                if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
-                const float* sc = ring + slot * TN + col0;       // a scale a column
+                float one = sc[slot * TN];
+                tmem_ld(d0 + buf * TN, r0);
+                tmem_ld(d0 + buf * TN + CW, r1);
+                auto add = [&](int c, const uint32_t (&r)[CW]) {
 #pragma unroll
-                for (int j = 0; j < C::COLS; j += 4) {
-                    const float4 s4 = *reinterpret_cast<const float4*>(sc + j);
-                    const uint32_t* r = j < CW ? r0 + j : r1 + (j - CW);
-                    acc[j] = fmaf(__uint_as_float(r[0]), s4.x, acc[j]);
-                    acc[j + 1] = fmaf(__uint_as_float(r[1]), s4.y, acc[j + 1]);
-                    acc[j + 2] = fmaf(__uint_as_float(r[2]), s4.z, acc[j + 2]);
-                    acc[j + 3] = fmaf(__uint_as_float(r[3]), s4.w, acc[j + 3]);
+                    for (int j = 0; j < CW; ++j) acc[c * CW + j] = fmaf(__uint_as_float(r[j]), one, acc[c * CW + j]);
+                };
+                for (uint32_t left = g.kb; left; --left) {
+                    const uint32_t d = d0 + buf * TN, acce = acce0 + 8 * buf, sempty = smem_u32(&sempty_b[slot / 4]);
+                    const bool last_of_group = slot % 4 == 3;
+                    buf ^= 1u;
+                    bphase ^= buf ^ 1u;
+                    if (++slot == C::SLOTS) { slot = 0; sphase ^= 1u; }
+                    tmem_ld_done(r0);
+                    tmem_ld_done(r1);
+                    add(0, r0);
+                    tmem_ld(d + 2 * CW, r0);
+                    add(1, r1);
+                    tmem_ld(d + 3 * CW, r1);
+                    tmem_ld_done(r0);
+                    tmem_ld_done(r1);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (CG == 2) arrive_cluster_if(lane == 0, acce);
+                    else arrive_if(lane == 0, acce);                     // the accumulator's columns are in registers
+                    arrive_if(lane == 0 && last_of_group, sempty);       // and so is the group's last scale
+                    add(2, r0);
+                    add(3, r1);
+                    if (left > 1) {
+                        scale_there();
+                        one = sc[slot * TN];
+                        columns_there();
+                        if (!ok) break;
+                        tmem_ld(d0 + buf * TN, r0);
+                        tmem_ld(d0 + buf * TN + CW, r1);
+                    }
                 }
-                ++item;
-                __syncwarp();
-                arrive_if(lane == 0 && item % 4 == 0, smem_u32(&sempty_b[gs]));
-            }
-            if (KS) {
-                // this CTA's part, [column][weight row], over the stages: their copies have landed and
-                // the MMAs that read them are complete (this tile is the CTA's only one)
-                float* part = (float*)smem + quarter * 32 + lane;
-#pragma unroll
-                for (int j = 0; j < C::COLS; ++j) part[(col0 + j) * 128] = acc[j];
-            } else if (ok) {
-                const uint32_t mrow = tc.m0 + quarter * 32 + lane;
+                if (!ok) break;
+                const TileF8 tc = decode_tile<C>(g, first, ends, t);
+                uint8_t* stage = (uint8_t*)bars + 512 + C::TABLES + (warp - 4) * 2048;
+                const uint32_t row0 = tc.row0 + rank * 128 + quarter * 32, mcol = tc.m0 + half * C::COLS;
                 switch (g.c_type) {
-                    case CM_T_Q88: store_cols<int16_t, C::COLS>(g, tc, col0, mrow, acc); break;
-                    case CM_T_F32: store_cols<float, C::COLS>(g, tc, col0, mrow, acc); break;
-                    case CM_T_F16: store_cols<__half, C::COLS>(g, tc, col0, mrow, acc); break;
-                    default: store_cols<__nv_bfloat16, C::COLS>(g, tc, col0, mrow, acc); break;
+                    case CM_T_Q88: store_rows<int16_t>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                    case CM_T_F32: store_rows<float>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                    case CM_T_F16: store_rows<__half>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                    default: store_rows<__nv_bfloat16>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                }
+            }
+        } else {
+            const uint32_t quarter = warp & 3u, col0 = (warp - 4) / 4 * C::COLS;
+            uint32_t buf = 0, bphase = 0, item = 0;
+            bool ok = true;
+            constexpr int CW = C::COLS < 32 ? 16 : 32, NC = C::COLS / CW;
+            static_assert(NC == 1 || NC == 2, "chunks of a warp's columns");
+            for (uint32_t t = cid; ok && t < total; t += ncl) {
+                const TileF8 tc = decode_tile<C>(g, first, ends, t);
+                float acc[C::COLS];
+#pragma unroll
+                for (int j = 0; j < C::COLS; ++j) acc[j] = 0.0f;
+                uint32_t r0[CW], r1[CW];
+                for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                    const uint32_t slot = item % C::SLOTS, gs = slot / 4;
+                    const bool early = mbar_test(smem_u32(&accf_b[buf]), bphase);
+                    if (item % 4 == 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sfull_b[gs]), (item / C::SLOTS) & 1u, wc));
+                    if (!__all_sync(0xffffffffu, early)) ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&accf_b[buf]), bphase, wc));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t d = tmem + buf * TN + col0 + (quarter << 21);
+                    tmem_ld(d, r0);
+                    if (NC > 1) tmem_ld(d + CW, r1);
+                    tmem_ld_done(r0);
+                    if (NC > 1) tmem_ld_done(r1);
+                    tc_fence_before();
+                    __syncwarp();
+                    arrive_if(lane == 0, smem_u32(&acce_b[buf]));
+                    if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
+                    const float* sc = ring + slot * TN + col0;       // a scale a column
+#pragma unroll
+                    for (int j = 0; j < C::COLS; j += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4*>(sc + j);
+                        const uint32_t* r = j < CW ? r0 + j : r1 + (j - CW);
+                        acc[j] = fmaf(__uint_as_float(r[0]), s4.x, acc[j]);
+                        acc[j + 1] = fmaf(__uint_as_float(r[1]), s4.y, acc[j + 1]);
+                        acc[j + 2] = fmaf(__uint_as_float(r[2]), s4.z, acc[j + 2]);
+                        acc[j + 3] = fmaf(__uint_as_float(r[3]), s4.w, acc[j + 3]);
+                    }
+                    ++item;
+                    __syncwarp();
+                    arrive_if(lane == 0 && item % 4 == 0, smem_u32(&sempty_b[gs]));
+                }
+                if (KS) {
+                    // this CTA's part, [column][weight row], over the stages: their copies have landed and
+                    // the MMAs that read them are complete (this tile is the CTA's only one)
+                    float* part = (float*)smem + quarter * 32 + lane;
+#pragma unroll
+                    for (int j = 0; j < C::COLS; ++j) part[(col0 + j) * 128] = acc[j];
+                } else if (ok) {
+                    const uint32_t mrow = tc.m0 + quarter * 32 + lane;
+                    switch (g.c_type) {
+                        case CM_T_Q88: store_cols<int16_t, C::COLS>(g, tc, col0, mrow, acc); break;
+                        case CM_T_F32: store_cols<float, C::COLS>(g, tc, col0, mrow, acc); break;
+                        case CM_T_F16: store_cols<__half, C::COLS>(g, tc, col0, mrow, acc); break;
+                        default: store_cols<__nv_bfloat16, C::COLS>(g, tc, col0, mrow, acc); break;
+                    }
                 }
             }
         }
@@ -873,10 +868,10 @@ int run_tiles(const Context* cx, const uint8_t* a, uint64_t lda, const uint8_t* 
     const uint32_t stored_groups = f.offsets && b_gs ? f.groups : 1u;
     g.group_step = stored_groups > 1 ? 1u : 0u;
     CUtensorMap tw, tt;
-    int rc = make_map(&tw, b, f.k, ldb, f.m, stored_groups, stored_groups > 1 ? b_gs : (uint64_t)f.m * ldb, 128, 3);
+    int rc = make_map(&tw, b, f.k, ldb, f.m, stored_groups, stored_groups > 1 ? b_gs : (uint64_t)f.m * ldb, C::WEIGHTS / CG, 3);
     if (!rc) rc = make_map(&tt, a, f.k, lda, f.n, 1, 0, C::TOKENS / CG, 2);
     if (rc) return rc;
-    if constexpr (CG == 1) {
+    if constexpr (CG == 1 && !TOK) {
         // few tiles: the largest cluster whose CTAs each take at least one K block of one tile and
         // are all resident
         for (uint32_t size = 8; size >= 2; size /= 2) {
