@@ -1,4 +1,4 @@
-"""Build libcormorant_cuda.so in-tree for sm_100a (nvcc cross-compiles; no GPU needed).
+"""Build libcormorant_cuda.so (and its CPython binding _bind.so) in-tree for sm_100a (nvcc cross-compiles; no GPU needed).
 
     python -m cormorant_b200.build [--force] [--ptxas-info]
 """
@@ -8,6 +8,7 @@ import argparse
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -15,6 +16,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libcormorant_cuda.so"
+BIND = PKG / "_bind.so"              # the CPython side of the 8-bit floating-point entries (csrc/bind.c)
 INCLUDE = ROOT / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -50,6 +52,13 @@ def build(force: bool = False, ptxas_info: bool = False, quiet: bool = True) -> 
             subprocess.run(cmd, check=True)
     if force or _stale(LIB, objs):
         cmd = [_nvcc(), *ARCH, "-shared", "--cudart", "static", "-o", str(LIB), *map(str, objs), "-lrt", "-ldl", "-lpthread"]
+        subprocess.run(cmd, check=True)
+    src = CSRC / "bind.c"
+    if force or _stale(BIND, [src, INCLUDE / "cormorant_cuda.h", Path(__file__)]):
+        cmd = ["gcc", "-O2", "-Wall", "-Wextra", "-Werror", "-std=gnu11", "-shared", "-fPIC", "-fvisibility=hidden",
+               "-I", sysconfig.get_paths()["include"], "-I", str(INCLUDE), "-o", str(BIND), str(src)]
+        if not quiet:
+            print(" ".join(cmd), file=sys.stderr)
         subprocess.run(cmd, check=True)
     return LIB
 

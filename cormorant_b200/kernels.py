@@ -367,71 +367,26 @@ def PoolingKernel(x, y, batch, channels, in_h, in_w, out_h, out_w, pool_h, pool_
 
 T_Q88, T_F32, T_F16, T_BF16 = range(4)         # CM_T_*: element types
 F8_E4M3, F8_E5M2 = 0, 1                        # CM_F8_*: 8-bit formats
-_TYPE_OF = {"torch.int16": T_Q88, "torch.float32": T_F32, "torch.float16": T_F16, "torch.bfloat16": T_BF16}
-_FORMAT_OF = {"torch.float8_e4m3fn": F8_E4M3, "torch.float8_e5m2": F8_E5M2, "torch.uint8": None}
-_SCALE_OF = {"torch.float32": T_F32}
-_OFFSETS_OF = {"torch.int32": 0}
-_CODES: dict = {}
+_native_module = None
 
 
-def _code(t, table, what):
-    """The code of tensor t's dtype in `table`; TypeError if it is not there."""
-    key = (t.dtype, id(table))
-    if key not in _CODES:
-        name = str(t.dtype)
-        if name not in table:
-            raise TypeError(f"{what}: expected one of {', '.join(table)}, got {name}")
-        _CODES[key] = table[name]
-    return _CODES[key]
+def _native():
+    """The native side of the entries below (csrc/bind.c), given the C ABI's addresses.  An operand is
+    None, a raw device address or a CUDA tensor: a tensor of two or more dimensions has its own row
+    pitch (and batch stride) unless they are given, a flat one and a raw address are dense unless they
+    are given; raw addresses need their type.  TypeError / ValueError for tensors of the wrong type or
+    device, too small, or with rows that are not contiguous."""
+    global _native_module
+    if _native_module is None:
+        import ctypes as C
 
-
-def _matrix(t, rows, cols, ld, table, what, device, batch=1, bs=None):
-    """(address, row pitch, batch stride, code) of the [batch][rows][cols] operand t.  A tensor of two
-    or more dimensions has its own pitch (and batch stride) unless they are given; a flat one and
-    a raw address are dense unless they are given.  A tensor has to be large enough."""
-    if t is None:
-        return None, 0, 0, None
-    if isinstance(t, int):
-        ld = cols if ld is None else ld
-        return t, ld, rows * ld if bs is None else bs, None
-    if not getattr(t, "is_cuda", False):
-        raise TypeError(f"{what}: buffers must be CUDA tensors or device addresses")
-    code = _code(t, table, what)
-    if t.get_device() != device and device >= 0:
-        raise ValueError(f"{what}: a tensor of cuda:{t.get_device()}, but the library runs on cuda:{device}")
-    shape, strides = t.shape, t.stride()
-    if shape and shape[-1] > 1 and strides[-1] != 1:
-        raise ValueError(f"{what}: the elements of a row must be contiguous")
-    if len(shape) >= 2 and ld is None:
-        if shape[-2] < rows or shape[-1] < cols:
-            raise ValueError(f"{what}: {tuple(shape)} holds no {rows} x {cols} matrix")
-        ld = strides[-2] if rows > 1 else max(strides[-2], cols)
-        if len(shape) == 3 and bs is None:
-            if shape[0] < batch:
-                raise ValueError(f"{what}: {tuple(shape)} holds fewer than {batch} matrices")
-            return t.data_ptr(), ld, strides[0], code
-    ld = cols if ld is None else ld
-    bs = rows * ld if bs is None else bs
-    if rows and cols and batch:
-        room = shape[0] if len(shape) == 1 else t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
-        if (batch - 1) * bs + (rows - 1) * ld + cols > room:
-            raise ValueError(f"{what}: the buffer is too short for {batch} x {rows} x {cols} at pitch {ld}")
-    return t.data_ptr(), ld, bs, code
-
-
-def _pick(code, given, default, what):
-    """An element type or format: the tensor's own, or the one given for a raw address or bytes."""
-    if code is None:
-        code = default if given is None else given
-        if code is None:
-            raise TypeError(f"{what}: a raw address needs its type")
-    elif given is not None and given != code:
-        raise TypeError(f"{what}: the tensor's type is not the one given")
-    return code
-
-
-def _blocks(v: int) -> int:
-    return -(-v // 128)
+        from . import _bind                    # ImportError if it is not built: there is no other path
+        L = lib()
+        names = ["cm_device"] + [n + t for n in ("cm_quant_fp8", "cm_rmsnorm_fp8", "cm_matmul_fp8", "cm_matmul_fp8_grouped")
+                                 for t in ("", "_async")]
+        _bind.setup(*(C.cast(getattr(L, n), C.c_void_p).value for n in names))
+        _native_module = _bind
+    return _native_module
 
 
 def QuantKernelFp8(x, q, scale, rows, cols, batch=1, ldx=None, ldq=None, lds=None, x_batch_stride=None,
@@ -441,15 +396,10 @@ def QuantKernelFp8(x, q, scale, rows, cols, batch=1, ldx=None, ldq=None, lds=Non
     columns (block_rows 1: scale [ceil(cols/128)][rows]) or for each 128 x 128 block (block_rows
     128: scale [ceil(rows/128)][ceil(cols/128)]) (cm_quant_fp8).  q: torch.float8_e4m3fn,
     float8_e5m2 or uint8 (then `fmt`, default F8_E4M3).  Not a reference kernel."""
-    L = lib()
-    dev = L.cm_device()
-    srows, scols = (_blocks(cols), rows) if block_rows == 1 else (_blocks(rows), _blocks(cols))
-    xp, ldx, xbs, xt = _matrix(x, rows, cols, ldx, _TYPE_OF, "x", dev, batch, x_batch_stride)
-    qp, ldq, qbs, qf = _matrix(q, rows, cols, ldq, _FORMAT_OF, "q", dev, batch, q_batch_stride)
-    sp, lds, sbs, _ = _matrix(scale, srows, scols, lds, _SCALE_OF, "scale", dev, batch, scale_batch_stride)
-    args = (xp, _pick(xt, x_type, None, "x"), qp, sp, rows, cols, batch, ldx, ldq, lds, xbs, qbs, sbs,
-            _pick(qf, fmt, F8_E4M3, "q"), block_rows)
-    check(L.cm_quant_fp8(*args) if stream is None else L.cm_quant_fp8_async(*args, _stream(stream)))
+    rc = (_native_module or _native()).quant_fp8(x, q, scale, rows, cols, batch, ldx, ldq, lds, x_batch_stride, q_batch_stride,
+                                                 scale_batch_stride, fmt, block_rows, x_type, stream)
+    if rc:
+        check(rc)
 
 
 def RmsNormKernelFp8(x, weight, q, scale, rows, cols, eps=1e-6, resid=None, resid_out=None, y=None, ldx=None,
@@ -458,21 +408,10 @@ def RmsNormKernelFp8(x, weight, q, scale, rows, cols, eps=1e-6, resid=None, resi
     """h = x + resid; resid_out = h; y = h / sqrt(mean(h^2) + eps) * weight; q, scale = the 1 x 128
     blocks of y in 8-bit floating point (cm_rmsnorm_fp8).  resid, resid_out, weight, y, and q with
     scale may be None.  Not a reference kernel."""
-    L = lib()
-    dev = L.cm_device()
-    xp, ldx, _, xt = _matrix(x, rows, cols, ldx, _TYPE_OF, "x", dev)
-    xt = _pick(xt, x_type, None, "x")
-    rp, ldr, _, rt = _matrix(resid, rows, cols, ldr, _TYPE_OF, "resid", dev)
-    op, ldo, _, ot = _matrix(resid_out, rows, cols, ldo, _TYPE_OF, "resid_out", dev)
-    yp, ldy, _, yt = _matrix(y, rows, cols, ldy, _TYPE_OF, "y", dev)
-    if any(t is not None and t != xt for t in (rt, ot, yt)):
-        raise TypeError("resid, resid_out and y are of x's type")
-    wp, _, _, wt = _matrix(weight, 1, cols, None, _TYPE_OF, "weight", dev)
-    qp, ldq, _, qf = _matrix(q, rows, cols, ldq, _FORMAT_OF, "q", dev)
-    sp, lds, _, _ = _matrix(scale, _blocks(cols), rows, lds, _SCALE_OF, "scale", dev)
-    args = (xp, rp, wp, op, yp, qp, sp, rows, cols, ldx, ldr, ldo, ldy, ldq, lds, xt,
-            _pick(wt, weight_type, xt, "weight"), eps, _pick(qf, fmt, F8_E4M3, "q"))
-    check(L.cm_rmsnorm_fp8(*args) if stream is None else L.cm_rmsnorm_fp8_async(*args, _stream(stream)))
+    rc = (_native_module or _native()).rmsnorm_fp8(x, weight, q, scale, rows, cols, eps, resid, resid_out, y, ldx, ldr, ldo, ldy,
+                                                   ldq, lds, fmt, x_type, weight_type, stream)
+    if rc:
+        check(rc)
 
 
 def MatmulKernelFp8(a, a_scale, b, b_scale, c, n, k, m, lda=None, a_scale_ld=None, ldb=None, b_scale_ld=None,
@@ -480,17 +419,10 @@ def MatmulKernelFp8(a, a_scale, b, b_scale, c, n, k, m, lda=None, a_scale_ld=Non
     """c [n][m] = a [n][k] . b [m][k] transposed, of 8-bit floating point operands with block
     scales: a_scale [ceil(k/128)][n], b_scale [ceil(m/128)][ceil(k/128)] (cm_matmul_fp8), as
     QuantKernelFp8 and RmsNormKernelFp8 write them.  Not a reference kernel."""
-    L = lib()
-    dev = L.cm_device()
-    kb = _blocks(k)
-    ap, lda, _, af = _matrix(a, n, k, lda, _FORMAT_OF, "a", dev)
-    bp, ldb, _, bf = _matrix(b, m, k, ldb, _FORMAT_OF, "b", dev)
-    asp, a_scale_ld, _, _ = _matrix(a_scale, kb, n, a_scale_ld, _SCALE_OF, "a_scale", dev)
-    bsp, b_scale_ld, _, _ = _matrix(b_scale, _blocks(m), kb, b_scale_ld, _SCALE_OF, "b_scale", dev)
-    cp, ldc, _, ct = _matrix(c, n, m, ldc, _TYPE_OF, "c", dev)
-    args = (ap, asp, bp, bsp, cp, n, k, m, lda, a_scale_ld, ldb, b_scale_ld, ldc, _pick(af, a_fmt, F8_E4M3, "a"),
-            _pick(bf, b_fmt, F8_E4M3, "b"), _pick(ct, c_type, None, "c"))
-    check(L.cm_matmul_fp8(*args) if stream is None else L.cm_matmul_fp8_async(*args, _stream(stream)))
+    rc = (_native_module or _native()).matmul_fp8(a, a_scale, b, b_scale, c, n, k, m, lda, a_scale_ld, ldb, b_scale_ld, ldc, a_fmt,
+                                                  b_fmt, c_type, stream)
+    if rc:
+        check(rc)
 
 
 def MatmulKernelFp8Grouped(a, a_scale, b, b_scale, c, offsets, groups, n, k, m, lda=None, a_scale_ld=None, ldb=None,
@@ -500,16 +432,8 @@ def MatmulKernelFp8Grouped(a, a_scale, b, b_scale, c, offsets, groups, n, k, m, 
     use b[g] [m][k] and b_scale[g] (cm_matmul_fp8_grouped).  offsets: groups + 1 int32 on the
     device, read by the kernel; rows outside the groups are left as they were.  Not a reference
     kernel."""
-    L = lib()
-    dev = L.cm_device()
-    kb = _blocks(k)
-    ap, lda, _, af = _matrix(a, n, k, lda, _FORMAT_OF, "a", dev)
-    bp, ldb, bgs, bf = _matrix(b, m, k, ldb, _FORMAT_OF, "b", dev, groups, b_group_stride)
-    asp, a_scale_ld, _, _ = _matrix(a_scale, kb, n, a_scale_ld, _SCALE_OF, "a_scale", dev)
-    bsp, b_scale_ld, bsgs, _ = _matrix(b_scale, _blocks(m), kb, b_scale_ld, _SCALE_OF, "b_scale", dev, groups,
-                                       b_scale_group_stride)
-    cp, ldc, _, ct = _matrix(c, n, m, ldc, _TYPE_OF, "c", dev)
-    op, _, _, _ = _matrix(offsets, 1, groups + 1, None, _OFFSETS_OF, "offsets", dev)
-    args = (ap, asp, bp, bsp, cp, op, groups, n, k, m, lda, a_scale_ld, ldb, b_scale_ld, bgs, bsgs, ldc,
-            _pick(af, a_fmt, F8_E4M3, "a"), _pick(bf, b_fmt, F8_E4M3, "b"), _pick(ct, c_type, None, "c"))
-    check(L.cm_matmul_fp8_grouped(*args) if stream is None else L.cm_matmul_fp8_grouped_async(*args, _stream(stream)))
+    rc = (_native_module or _native()).matmul_fp8_grouped(a, a_scale, b, b_scale, c, offsets, groups, n, k, m, lda, a_scale_ld, ldb,
+                                                          b_scale_ld, b_group_stride, b_scale_group_stride, ldc, a_fmt, b_fmt,
+                                                          c_type, stream)
+    if rc:
+        check(rc)
