@@ -50,22 +50,27 @@ struct KArgs {
 
 template <int TN, int CG, bool TOK>
 struct F8Cfg {
-    static constexpr int EPI_WARPS = TN >= 128 ? 8 : 4;
-    static constexpr int COLS = TN / (EPI_WARPS / 4);        // accumulator columns of an epilogue warp
+    // eight epilogue warps: from 128 columns on, four for each half of the columns; narrower tiles'
+    // K blocks go to the two fours in turn, which add their sums at the end of a tile (a block costs a
+    // warp some 500 cycles of waiting whatever its width)
+    static constexpr int EPI_WARPS = 8;
+    static constexpr int TURNS = TN >= 128 ? 1 : 2;
+    static constexpr int COLS = TURNS == 1 ? TN / 2 : TN;    // accumulator columns of an epilogue warp
     static constexpr int THREADS = 128 + 32 * EPI_WARPS;
     static constexpr uint32_t TOKENS = TOK ? 128 * CG : TN;  // token rows of a tile
     static constexpr uint32_t WEIGHTS = TOK ? TN : 128 * CG; // weight rows of a tile
     static constexpr bool SPLIT_REGS = TN == 256;            // 128 sums a thread: registers move to the epilogue warps
     static constexpr int A_TILE = 128 * 128, B_TILE = TN / CG * 128;
     static constexpr int STAGE = A_TILE + B_TILE;
-    static constexpr int STAGES = TN >= 128 ? 6 : TN == 64 ? 8 : TN == 32 ? 9 : 10;
+    static constexpr int STAGES = TN >= 128 ? 6 : TN == 64 ? 7 : TN == 32 ? 9 : 10;
     static constexpr int NBUF = TN == 256 ? 2 : 4;           // accumulators in TMEM
     static constexpr int SLOTS = 8;                          // scale ring: K blocks, in groups of 4 with a barrier each way
     static constexpr int GROUPS = SLOTS / 4;
     static constexpr uint32_t TMEM_COLS = NBUF * TN;
     static constexpr int TABLES = (2 * (kMaxGroups + 1) * 4 + 15) / 16 * 16;
     static_assert((STAGES * STAGE + SLOTS * TN * 4) % 16 == 0, "what follows the ring is 16-byte aligned");
-    static constexpr int OUT = TOK ? EPI_WARPS * 2048 : 0;   // output staging: 32 rows x 64 bytes a warp
+    // output staging, 32 rows x 64 bytes a warp; or the sums that the two fours exchange
+    static constexpr int OUT = TOK ? EPI_WARPS * 2048 : TURNS == 2 ? TN * 128 * 4 : 0;
     static constexpr int SMEM = 1024 + STAGES * STAGE + SLOTS * TN * 4 + 512 + TABLES + OUT;
     static_assert(SMEM <= 232448 && 2 * SMEM > 232448, "one CTA an SM");
     static_assert(TN * 512 <= STAGES * STAGE, "partial sums of a split tile fit the stages");
@@ -183,6 +188,17 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
+// 16 bytes of another CTA's shared memory (of this cluster; between two cluster barriers)
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+    return v;
+}
+
+// a barrier of the epilogue warps alone
+template <int THREADS>
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
+
 struct TileF8 {
     uint32_t m0;             // first weight row
     uint32_t row0, row1;     // token rows row0 .. row1 - 1, at most a tile's used
@@ -221,7 +237,7 @@ __device__ __forceinline__ TileF8 decode_tile(const KArgs& g, const uint32_t* fi
 }
 
 template <typename T, int COLS>
-__device__ __forceinline__ void store_cols(const KArgs& g, const TileF8& tc, uint32_t col0, uint32_t mrow, const float (&acc)[COLS]) {
+__device__ __forceinline__ void store_cols(const KArgs& g, const TileF8& tc, uint32_t col0, uint32_t mrow, const float* acc) {
     if (mrow >= g.m) return;
     const uint32_t tok = tc.row0 + col0;
     T* p = (T*)g.c + (uint64_t)tok * g.ldc + mrow;
@@ -287,7 +303,7 @@ __device__ __forceinline__ void store_one(const KArgs& g, uint64_t i, float v) {
 }
 
 // The token scales of one (tile, K block), as a scale warp holds them on their way from global
-// memory: the loads are issued two blocks of this warp (four of the CTA) ahead of their use.
+// memory: the loads of a group of four are issued while the group before it waits for room.
 template <int TN, bool TOK>
 struct ScaleRegs {
     float v[TOK ? 4 : TN < 32 ? 1 : TN / 32];
@@ -300,9 +316,7 @@ template <int TN, int CG, bool TOK, bool KS>
 __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
     gemm_f8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT, const KArgs g) {
     using C = F8Cfg<TN, CG, TOK>;
-    static_assert(CG == 1 || !KS, "a pair does not split K");
-    griddep_wait();
-    griddep_launch_dependents();   // all CTAs are resident
+    static_assert(TN == 16 || !KS, "only the narrowest tiles split K");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     float* ring = (float*)(smem + C::STAGES * C::STAGE);
@@ -332,13 +346,15 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
     constexpr uint16_t kPairMask = 0x3;
 
     if (threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmW) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmT) : "memory");
         for (int s = 0; s < C::STAGES; ++s) {
             mbar_init(smem_u32(&full_b[s]), 1);
             mbar_init(smem_u32(&empty_b[s]), 1);
         }
         for (int b = 0; b < C::NBUF; ++b) {
             mbar_init(smem_u32(&accf_b[b]), 1);
-            mbar_init(smem_u32(&acce_b[b]), C::EPI_WARPS * CG);
+            mbar_init(smem_u32(&acce_b[b]), C::EPI_WARPS / C::TURNS * CG);
         }
         for (int s = 0; s < C::GROUPS; ++s) {
             mbar_init(smem_u32(&sfull_b[s]), 2);
@@ -363,34 +379,41 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
         }
         tc_fence_before();
     }
-    if (g.offsets && warp == 2) {
-        // running maximum of the offsets held to 0..n, then running sum of the groups' token tiles:
-        // whatever the offsets hold, no row outside 0..n-1 is reached
-        uint32_t high = 0, tiles = 0;
-        for (uint32_t base = 0; base <= g.groups; base += 32) {
-            const uint32_t i = base + lane;
-            uint32_t e = i <= g.groups ? (uint32_t)min(max(g.offsets[i], 0), (int)g.n) : 0u;
+    // up to here nothing of the kernel before this one is touched
+    griddep_wait();
+    griddep_launch_dependents();   // all CTAs are resident
+    if (g.offsets) {
+        // the offsets in one round of loads; then one warp's running maximum of them, held to 0..n, and
+        // running sum of the groups' token tiles: whatever the offsets hold, no row outside 0..n-1 is reached
+        for (uint32_t i = threadIdx.x; i <= g.groups; i += C::THREADS) ends[i] = (uint32_t)min(max(g.offsets[i], 0), (int)g.n);
+        __syncthreads();
+        if (warp == 2) {
+            uint32_t high = 0, tiles = 0;
+            for (uint32_t base = 0; base <= g.groups; base += 32) {
+                const uint32_t i = base + lane;
+                uint32_t e = i <= g.groups ? ends[i] : 0u;
 #pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const uint32_t p = __shfl_up_sync(0xffffffffu, e, o);
-                if (lane >= (uint32_t)o) e = max(e, p);
-            }
-            e = max(e, high);
-            uint32_t before = __shfl_up_sync(0xffffffffu, e, 1);
-            if (lane == 0) before = high;
-            // tiles of the group that ends at offset i (none ends at offset 0)
-            uint32_t cnt = i > 0 ? (e - before + C::TOKENS - 1) / C::TOKENS : 0u;
+                for (int o = 1; o < 32; o *= 2) {
+                    const uint32_t p = __shfl_up_sync(0xffffffffu, e, o);
+                    if (lane >= (uint32_t)o) e = max(e, p);
+                }
+                e = max(e, high);
+                uint32_t before = __shfl_up_sync(0xffffffffu, e, 1);
+                if (lane == 0) before = high;
+                // tiles of the group that ends at offset i (none ends at offset 0)
+                uint32_t cnt = i > 0 ? (e - before + C::TOKENS - 1) / C::TOKENS : 0u;
 #pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const uint32_t p = __shfl_up_sync(0xffffffffu, cnt, o);
-                if (lane >= (uint32_t)o) cnt += p;
+                for (int o = 1; o < 32; o *= 2) {
+                    const uint32_t p = __shfl_up_sync(0xffffffffu, cnt, o);
+                    if (lane >= (uint32_t)o) cnt += p;
+                }
+                if (i <= g.groups) {
+                    ends[i] = e;
+                    first[i] = tiles + cnt;
+                }
+                high = __shfl_sync(0xffffffffu, e, 31);
+                tiles += __shfl_sync(0xffffffffu, cnt, 31);
             }
-            if (i <= g.groups) {
-                ends[i] = e;
-                first[i] = tiles + cnt;
-            }
-            high = __shfl_sync(0xffffffffu, e, 31);
-            tiles += __shfl_sync(0xffffffffu, cnt, 31);
         }
     }
     __syncthreads();
@@ -478,63 +501,56 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                 mbar_wait(smem_u32(done_b), 0, drain);
             }
         } else {
-            // Scale warps: of the (tile, K block) items of this CTA, in groups of four, 2 takes the even
-            // ones and 3 the odd ones; the next group's loads are in flight while this one waits for room.
-            constexpr uint32_t AHEAD = 2;
-            ScaleRegs<TN, TOK> regs[AHEAD];
-            uint32_t t = cid, kb = kb0;
+            // Scale warps: of a tile's K blocks, in groups of four, 2 takes the even ones and 3 the odd
+            // ones; the next group's loads are in flight while this one waits for room.
+            const uint32_t nkb = kb1 - kb0, per = (nkb + 3) / 4;
+            ScaleRegs<TN, TOK> regs[2];
+            bool have[2] = {false, false};
+            uint32_t t = cid, at = 0;            // the next group: tile and place in it
             TileF8 tc{};
             const float* sbp = nullptr;
             uint32_t blocks = 0;                 // weight blocks of this CTA's part of the tile that exist
-            bool fresh = true;
-            auto advance = [&](uint32_t by) {
-                for (uint32_t i = 0; i < by; ++i)
-                    if (++kb == kb1) { kb = kb0; t += ncl; fresh = true; }
-            };
-            auto load = [&](ScaleRegs<TN, TOK>& r) {
-                if (fresh) {
+            auto fetch = [&]() {
+                if (t >= total) return;
+                if (at == 0) {
                     tc = decode_tile<C>(g, first, ends, t);
                     if (TOK) tc.row0 += rank * 128;
                     else tc.m0 += rank * 128;
                     blocks = tc.m0 < g.m ? (g.m - tc.m0 + 127) / 128 : 0u;
                     sbp = g.bs + tc.group * g.bs_gs + (uint64_t)(tc.m0 / 128) * g.b_lds;
-                    fresh = false;
                 }
 #pragma unroll
-                for (uint32_t h = 0; h < sizeof(r.sb) / 4; ++h) r.sb[h] = h < blocks ? __ldg(sbp + h * g.b_lds + kb) : 0.0f;
-                const float* p = g.as + (uint64_t)kb * g.a_lds + tc.row0;
+                for (uint32_t p = 0; p < 2; ++p) {
+                    const uint32_t i = at * 4 + 2 * p + warp - 2, kb = kb0 + i;
+                    have[p] = i < nkb;
+                    if (!have[p]) continue;
+                    ScaleRegs<TN, TOK>& r = regs[p];
 #pragma unroll
-                for (uint32_t i = 0; i < sizeof(r.v) / 4; ++i) {
-                    const uint32_t j = lane + 32 * i;
-                    r.v[i] = (TOK || j < TN) && tc.row0 + j < tc.row1 ? __ldg(p + j) : 0.0f;
+                    for (uint32_t h = 0; h < sizeof(r.sb) / 4; ++h) r.sb[h] = h < blocks ? __ldg(sbp + h * g.b_lds + kb) : 0.0f;
+                    const float* a = g.as + (uint64_t)kb * g.a_lds + tc.row0;
+#pragma unroll
+                    for (uint32_t q = 0; q < sizeof(r.v) / 4; ++q) {
+                        const uint32_t j = lane + 32 * q;
+                        r.v[q] = (TOK || j < TN) && tc.row0 + j < tc.row1 ? __ldg(a + j) : 0.0f;
+                    }
                 }
+                if (++at == per) { at = 0; t += ncl; }
             };
-            advance(warp - 2);
-            bool have[AHEAD];
-            auto fetch = [&]() {
-#pragma unroll
-                for (uint32_t p = 0; p < AHEAD; ++p) {
-                    have[p] = t < total;
-                    if (have[p]) { load(regs[p]); advance(2); }
-                }
-            };
-            // groups: this CTA's tiles times its K blocks, in fours (the last one may be partial)
-            const uint64_t items = (uint64_t)(cid < total ? (total - cid + ncl - 1) / ncl : 0u) * (kb1 - kb0);
+            const uint64_t groups = (uint64_t)(cid < total ? (total - cid + ncl - 1) / ncl : 0u) * per;
             fetch();
-            for (uint64_t grp = 0; grp * 4 < items; ++grp) {
+            for (uint64_t grp = 0; grp < groups; ++grp) {
                 const uint32_t gs = (uint32_t)grp % C::GROUPS, use = (uint32_t)(grp / C::GROUPS);
                 if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sempty_b[gs]), (use & 1u) ^ 1u, wc))) break;
 #pragma unroll
-                for (uint32_t p = 0; p < AHEAD; ++p) {
+                for (uint32_t p = 0; p < 2; ++p) {
                     float* dst = ring + (gs * 4 + 2 * p + warp - 2) * TN;
-                    if (have[p]) {
+                    if (!have[p]) continue;
 #pragma unroll
-                        for (uint32_t i = 0; i < sizeof(regs[p].v) / 4; ++i) {
-                            const uint32_t j = lane + 32 * i;
+                    for (uint32_t q = 0; q < sizeof(regs[p].v) / 4; ++q) {
+                        const uint32_t j = lane + 32 * q;
 #pragma unroll
-                            for (uint32_t h = 0; h < sizeof(regs[p].sb) / 4; ++h)
-                                if (TOK || j < TN) dst[h * 128 + j] = regs[p].v[i] * regs[p].sb[h];
-                        }
+                        for (uint32_t h = 0; h < sizeof(regs[p].sb) / 4; ++h)
+                            if (TOK || j < TN) dst[h * 128 + j] = regs[p].v[q] * regs[p].sb[h];
                     }
                 }
                 __syncwarp();
@@ -586,10 +602,11 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                 };
                 for (uint32_t left = g.kb; left; --left) {
                     const uint32_t d = d0 + buf * TN, acce = acce0 + 8 * buf, sempty = smem_u32(&sempty_b[slot / 4]);
-                    const bool last_of_group = slot % 4 == 3;
+                    const bool last_of_group = slot % 4 == 3 || left == 1;
                     buf ^= 1u;
                     bphase ^= buf ^ 1u;
-                    if (++slot == C::SLOTS) { slot = 0; sphase ^= 1u; }
+                    slot = left == 1 ? (slot | 3u) + 1u : slot + 1u;    // a tile's groups are its own
+                    if (slot == C::SLOTS) { slot = 0; sphase ^= 1u; }
                     tmem_ld_done(r0);
                     tmem_ld_done(r1);
                     add(0, r0);
@@ -626,60 +643,75 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                 }
             }
         } else {
-            const uint32_t quarter = warp & 3u, col0 = (warp - 4) / 4 * C::COLS;
-            uint32_t buf = 0, bphase = 0, item = 0;
+            const uint32_t quarter = warp & 3u, four = (warp - 4) / 4;
+            const uint32_t col0 = C::TURNS == 1 ? four * C::COLS : 0u, turn = C::TURNS == 1 ? 0u : four;
+            const uint32_t nkb = kb1 - kb0;
+            uint32_t item = 0, grp = 0;          // K blocks and groups of scales before this tile
             bool ok = true;
             constexpr int CW = C::COLS < 32 ? 16 : 32, NC = C::COLS / CW;
             static_assert(NC == 1 || NC == 2, "chunks of a warp's columns");
-            for (uint32_t t = cid; ok && t < total; t += ncl) {
+            for (uint32_t t = cid; t < total; t += ncl, item += nkb) {
                 const TileF8 tc = decode_tile<C>(g, first, ends, t);
                 float acc[C::COLS];
 #pragma unroll
                 for (int j = 0; j < C::COLS; ++j) acc[j] = 0.0f;
                 uint32_t r0[CW], r1[CW];
-                for (uint32_t kb = kb0; kb < kb1; ++kb) {
-                    const uint32_t slot = item % C::SLOTS, gs = slot / 4;
-                    const bool early = mbar_test(smem_u32(&accf_b[buf]), bphase);
-                    if (item % 4 == 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sfull_b[gs]), (item / C::SLOTS) & 1u, wc));
-                    if (!__all_sync(0xffffffffu, early)) ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&accf_b[buf]), bphase, wc));
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t d = tmem + buf * TN + col0 + (quarter << 21);
-                    tmem_ld(d, r0);
-                    if (NC > 1) tmem_ld(d + CW, r1);
-                    tmem_ld_done(r0);
-                    if (NC > 1) tmem_ld_done(r1);
-                    tc_fence_before();
-                    __syncwarp();
-                    arrive_if(lane == 0, smem_u32(&acce_b[buf]));
-                    if (++buf == C::NBUF) { buf = 0; bphase ^= 1; }
-                    const float* sc = ring + slot * TN + col0;       // a scale a column
+                for (uint32_t g4 = 0; ok && g4 < nkb; g4 += 4, ++grp) {
+                    const uint32_t gs = grp % C::GROUPS;
+                    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sfull_b[gs]), (grp / C::GROUPS) & 1u, wc));
+                    for (uint32_t q = turn; ok && q < 4 && g4 + q < nkb; q += C::TURNS) {
+                        const uint32_t it = item + g4 + q, buf = it % C::NBUF;
+                        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&accf_b[buf]), (it / C::NBUF) & 1u, wc));
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t d = tmem + buf * TN + col0 + (quarter << 21);
+                        tmem_ld(d, r0);
+                        if (NC > 1) tmem_ld(d + CW, r1);
+                        tmem_ld_done(r0);
+                        if (NC > 1) tmem_ld_done(r1);
+                        tc_fence_before();
+                        __syncwarp();
+                        arrive_if(lane == 0, smem_u32(&acce_b[buf]));
+                        const float* sc = ring + (gs * 4 + q) * TN + col0;      // a scale a column
 #pragma unroll
-                    for (int j = 0; j < C::COLS; j += 4) {
-                        const float4 s4 = *reinterpret_cast<const float4*>(sc + j);
-                        const uint32_t* r = j < CW ? r0 + j : r1 + (j - CW);
-                        acc[j] = fmaf(__uint_as_float(r[0]), s4.x, acc[j]);
-                        acc[j + 1] = fmaf(__uint_as_float(r[1]), s4.y, acc[j + 1]);
-                        acc[j + 2] = fmaf(__uint_as_float(r[2]), s4.z, acc[j + 2]);
-                        acc[j + 3] = fmaf(__uint_as_float(r[3]), s4.w, acc[j + 3]);
+                        for (int j = 0; j < C::COLS; j += 4) {
+                            const float4 s4 = *reinterpret_cast<const float4*>(sc + j);
+                            const uint32_t* r = j < CW ? r0 + j : r1 + (j - CW);
+                            acc[j] = fmaf(__uint_as_float(r[0]), s4.x, acc[j]);
+                            acc[j + 1] = fmaf(__uint_as_float(r[1]), s4.y, acc[j + 1]);
+                            acc[j + 2] = fmaf(__uint_as_float(r[2]), s4.z, acc[j + 2]);
+                            acc[j + 3] = fmaf(__uint_as_float(r[3]), s4.w, acc[j + 3]);
+                        }
                     }
-                    ++item;
                     __syncwarp();
-                    arrive_if(lane == 0 && item % 4 == 0, smem_u32(&sempty_b[gs]));
+                    arrive_if(lane == 0, smem_u32(&sempty_b[gs]));
                 }
+                if (C::TURNS == 2) {
+                    // each four finishes half of the columns, adding what the other one summed of them
+                    constexpr int H = C::COLS / 2;
+                    float* mine = (float*)((uint8_t*)bars + 512 + C::TABLES) + quarter * 32 + lane;
+#pragma unroll
+                    for (int j = 0; j < H; ++j) mine[(turn * H + j) * 128] = turn ? acc[j] : acc[H + j];
+                    epilogue_sync<C::EPI_WARPS * 32>();
+#pragma unroll
+                    for (int j = 0; j < H; ++j) acc[j] = (turn ? acc[H + j] : acc[j]) + mine[((turn ^ 1u) * H + j) * 128];
+                    if (t + ncl < total) epilogue_sync<C::EPI_WARPS * 32>();      // read before the next tile writes
+                }
+                constexpr int OWN = C::COLS / C::TURNS;
+                const uint32_t own0 = C::TURNS == 1 ? col0 : turn * OWN;
                 if (KS) {
                     // this CTA's part, [column][weight row], over the stages: their copies have landed and
                     // the MMAs that read them are complete (this tile is the CTA's only one)
                     float* part = (float*)smem + quarter * 32 + lane;
 #pragma unroll
-                    for (int j = 0; j < C::COLS; ++j) part[(col0 + j) * 128] = acc[j];
+                    for (int j = 0; j < OWN; ++j) part[(own0 + j) * 128] = acc[j];
                 } else if (ok) {
                     const uint32_t mrow = tc.m0 + quarter * 32 + lane;
                     switch (g.c_type) {
-                        case CM_T_Q88: store_cols<int16_t, C::COLS>(g, tc, col0, mrow, acc); break;
-                        case CM_T_F32: store_cols<float, C::COLS>(g, tc, col0, mrow, acc); break;
-                        case CM_T_F16: store_cols<__half, C::COLS>(g, tc, col0, mrow, acc); break;
-                        default: store_cols<__nv_bfloat16, C::COLS>(g, tc, col0, mrow, acc); break;
+                        case CM_T_Q88: store_cols<int16_t, OWN>(g, tc, own0, mrow, acc); break;
+                        case CM_T_F32: store_cols<float, OWN>(g, tc, own0, mrow, acc); break;
+                        case CM_T_F16: store_cols<__half, OWN>(g, tc, own0, mrow, acc); break;
+                        default: store_cols<__nv_bfloat16, OWN>(g, tc, own0, mrow, acc); break;
                     }
                 }
             }
@@ -693,16 +725,24 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
             const TileF8 tc = decode_tile<C>(g, first, ends, cid);
             const uint32_t lo = TN * crank / csize, hi = TN * (crank + 1) / csize;
             const uint32_t base = smem_u32(smem);
-            for (uint32_t e = threadIdx.x; e < (hi - lo) * 128; e += C::THREADS) {
-                const uint32_t col = lo + e / 128, r = e % 128;
+            for (uint32_t e = threadIdx.x; e < (hi - lo) * 32; e += C::THREADS) {
+                const uint32_t col = lo + e / 32, r = e % 32 * 4;
                 if (tc.row0 + col >= tc.row1 || tc.m0 + r >= g.m) continue;
-                float v = 0.0f;
-                for (uint32_t p = 0; p < csize; ++p) {
-                    float x;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(map_to_rank(base + (col * 128 + r) * 4, p)) : "memory");
-                    v += x;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (uint32_t p = 0; p < csize; p += 2) {          // 2, 4 or 8 parts, in order
+                    const float4 x = ld_cluster4(map_to_rank(base + (col * 128 + r) * 4, p));
+                    const float4 y = ld_cluster4(map_to_rank(base + (col * 128 + r) * 4, p + 1));
+                    v.x = v.x + x.x + y.x;
+                    v.y = v.y + x.y + y.y;
+                    v.z = v.z + x.z + y.z;
+                    v.w = v.w + x.w + y.w;
                 }
-                store_one(g, (uint64_t)(tc.row0 + col) * g.ldc + tc.m0 + r, v);
+                const uint64_t i = (uint64_t)(tc.row0 + col) * g.ldc + tc.m0 + r;
+                const uint32_t live = g.m - tc.m0 - r;
+                store_one(g, i, v.x);
+                if (live > 1) store_one(g, i + 1, v.y);
+                if (live > 2) store_one(g, i + 2, v.z);
+                if (live > 3) store_one(g, i + 3, v.w);
             }
         }
     }
@@ -871,18 +911,48 @@ int run_tiles(const Context* cx, const uint8_t* a, uint64_t lda, const uint8_t* 
     int rc = make_map(&tw, b, f.k, ldb, f.m, stored_groups, stored_groups > 1 ? b_gs : (uint64_t)f.m * ldb, C::WEIGHTS / CG, 3);
     if (!rc) rc = make_map(&tt, a, f.k, lda, f.n, 1, 0, C::TOKENS / CG, 2);
     if (rc) return rc;
-    if constexpr (CG == 1 && !TOK) {
-        // few tiles: the largest cluster whose CTAs each take at least one K block of one tile and
-        // are all resident
-        for (uint32_t size = 8; size >= 2; size /= 2) {
+    if constexpr (TN == 16) {
+        // Few tiles (wider ones are taken only where narrow ones fill the SMs): a cluster of CTAs to a tile, as many as are resident at once, where the blocks that
+        // a CTA is spared cost more than the cluster's launch, barriers and additions.  (Hundredths of a
+        // microsecond: one token, m = k = 4096, 32 blocks of 0.18 us: 9.7 us on one CTA a tile, 8.3 on
+        // two, 7.6 on four; m = k = 1024, 8 blocks: 4.3, 5.0 and 4.8.)
+        constexpr uint32_t block = 18, extra = 180;
+        uint32_t best = 1, least = g.kb * block;
+        for (uint32_t size = 2; size <= 8 && size <= g.kb && most * size <= (uint64_t)cx->sm_count; size *= 2) {
+            const uint32_t cost = (g.kb + size - 1) / size * block + extra;
             int resident = 0;
-            if (size > g.kb || most * size > (uint64_t)cx->sm_count) continue;
+            if (cost >= least) continue;
             rc = resident_clusters<TN, CG, TOK, true>(cx, size, &resident);
             if (rc) return rc;
-            if (most <= (uint64_t)resident) return launch_tiles<TN, CG, TOK, true>(cx, tw, tt, g, size, most, s);
+            if (most <= (uint64_t)resident) { best = size; least = cost; }
         }
+        if (best > 1) return launch_tiles<TN, CG, TOK, true>(cx, tw, tt, g, best, most, s);
     }
     return launch_tiles<TN, CG, TOK, false>(cx, tw, tt, g, CG, most, s);
+}
+
+// The tile, by its token rows: 16 to 128 tokens x 128 weight rows on one SM, or 256 x 256 on two.  A
+// wider tile reads the weights less often and does more a block, but a block takes it longer and
+// there are fewer tiles to spread over the SMs.  The one is taken whose whole waves cost least:
+// waves x (K blocks x time of a block + time of a tile's output), in hundredths of a microsecond as
+// measured at k = 4096 and 1024 (16 to 256 tokens: 0.18, 0.20, 0.24, 0.42, 0.48 a block).  With m = k
+// = 4096, for instance, 128 tokens take 10.6 us in tiles of 32 and 17.6 in one of 128; 512 tokens
+// 18.5 in tiles of 128, 21.4 of 64 and 20.5 of 256; 1024 tokens 21.1 of 256 and 33.0 of 128.
+uint32_t pick_tokens(const Context* cx, const Fp8Args& f, uint32_t kb) {
+    static const struct { uint32_t tokens, weights, sms, block, out; } kinds[] = {
+        {16, 128, 1, 18, 30}, {32, 128, 1, 20, 30}, {64, 128, 1, 24, 60}, {128, 128, 1, 42, 80}, {256, 256, 2, 48, 200}};
+    uint32_t best = 16;
+    uint64_t least = ~0ull;
+    for (const auto& t : kinds) {
+        // groups: their sizes are on the device; on average half a tile of each is not filled
+        uint64_t token_tiles = (f.n + (uint64_t)t.tokens - 1) / t.tokens;
+        if (f.offsets) token_tiles = std::min<uint64_t>(f.n, f.n / t.tokens + (f.groups + 1) / 2 + 1);
+        const uint64_t tiles = token_tiles * ((f.m + (uint64_t)t.weights - 1) / t.weights);
+        const uint64_t at_once = (uint64_t)cx->sm_count / t.sms;
+        const uint64_t cost = (tiles + at_once - 1) / at_once * ((uint64_t)kb * t.block + t.out);
+        if (cost < least) { least = cost; best = t.tokens; }
+    }
+    return best;
 }
 
 int fp8_launch(const char* who, const Context* cx, const Fp8Args& f, cudaStream_t s) {
@@ -921,13 +991,13 @@ int fp8_launch(const char* who, const Context* cx, const Fp8Args& f, cudaStream_
     const uint8_t* a = a_bytes ? scratch : f.a;
     const uint8_t* b = b_bytes ? scratch + a_bytes : f.b;
     const uint64_t pa = a_bytes ? k16 : lda, pb = b_bytes ? k16 : ldb, gsb = one ? 0 : b_bytes ? f.m * k16 : f.b_gs;
-    // rows a weight tile meets at once: the smallest tile that holds a group's (mean) rows
-    const uint64_t rows = f.offsets ? (f.n + (uint64_t)f.groups - 1) / f.groups : f.n;
-    if (rows <= 16) rc = run_tiles<16, 1, false>(cx, a, pa, b, pb, gsb, f, g, s);
-    else if (rows <= 32) rc = run_tiles<32, 1, false>(cx, a, pa, b, pb, gsb, f, g, s);
-    else if (rows <= 64) rc = run_tiles<64, 1, false>(cx, a, pa, b, pb, gsb, f, g, s);
-    else if (rows <= 128) rc = run_tiles<128, 1, false>(cx, a, pa, b, pb, gsb, f, g, s);
-    else rc = run_tiles<256, 2, true>(cx, a, pa, b, pb, gsb, f, g, s);
+    switch (pick_tokens(cx, f, g.kb)) {
+        case 16: rc = run_tiles<16, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
+        case 32: rc = run_tiles<32, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
+        case 64: rc = run_tiles<64, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
+        case 128: rc = run_tiles<128, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
+        default: rc = run_tiles<256, 2, true>(cx, a, pa, b, pb, gsb, f, g, s); break;
+    }
     scratch_free(scratch, s);
     if (rc) return rc;
     cudaError_t e = cudaGetLastError();

@@ -279,6 +279,10 @@ MATMUL = [  # n, k, m, c type, a format, b format
     (255, 256, 512, F32, E4, E4), (257, 129, 300, F32, E4, E4), (300, 1000, 1001, F32, E5, E4), (513, 2048, 640, F16, E4, E4),
     (1000, 512, 384, Q88, E4, E4), (1100, 1152, 1300, BF16, E4, E4), (4, 16384, 136, F32, E4, E4), (2048, 640, 16, F32, E4, E4),
     (777, 96, 2048, BF16, E4, E4),
+    # K split over two, four and eight CTAs; tiles of 64, 128 and 256 tokens, several of a CTA
+    (308, 2716, 129, F32, E4, E4), (163, 1794, 141, BF16, E4, E5), (1, 1545, 16, F32, E5, E4), (2413, 300, 135, F32, E4, E4),
+    (1000, 700, 2049, F16, E4, E4), (3454, 100, 265, BF16, E4, E5), (520, 300, 1500, F32, E4, E4), (2720, 300, 797, F32, E5, E4),
+    (1300, 1500, 2500, BF16, E4, E4), (1300, 1500, 2501, F32, E4, E4), (4000, 129, 1100, Q88, E4, E4), (1025, 515, 2100, F16, E4, E4),
 ]
 
 
@@ -362,6 +366,10 @@ GROUPED = [  # row counts, rows before the first, rows behind the last, k, m, c 
     ([0, 0, 0], 2, 3, 256, 64, F32, E4, E4), ([17, 0, 1, 40], 3, 5, 515, 200, F16, E5, E4), ([129, 128, 127], 0, 1, 640, 260, F32, E4, E5),
     ([300, 0, 5, 211], 1, 0, 1000, 520, F32, E4, E4), ([2] * 40, 0, 0, 512, 128, BF16, E4, E4), ([600, 700], 0, 9, 256, 384, BF16, E4, E4),
     ([0, 513], 0, 0, 129, 130, Q88, E4, E4), ([1] * 100 + [0] * 900 + [30], 0, 0, 128, 32, F32, E4, E4), ([900, 20, 0, 400, 256, 100], 7, 13, 1152, 640, BF16, E4, E4),
+    # as above: split K, wider tiles, several tiles of a CTA
+    ([100, 0, 180], 0, 0, 1795, 17, F32, E4, E4), ([3, 550, 8], 1, 1, 2751, 20, F32, E4, E4), ([2] * 40, 0, 0, 512, 1024, BF16, E4, E4),
+    ([1000, 0, 1395], 0, 5, 130, 140, F32, E4, E4), ([600, 1, 0, 1500, 700, 370], 2, 0, 200, 267, F16, E4, E5),
+    ([900, 0, 1300, 213], 3, 4, 300, 914, F32, E4, E4), ([257, 0, 255, 900, 1], 0, 87, 600, 1300, BF16, E4, E4),
 ]
 
 
