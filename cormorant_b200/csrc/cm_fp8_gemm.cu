@@ -272,6 +272,16 @@ __device__ __forceinline__ void store_rows(const KArgs& g, uint32_t row0, uint32
             *reinterpret_cast<uint4*>(stage + lane * 64 + ((p ^ (lane >> 1)) & 3) * 16) = o.u;
         }
         __syncwarp();
+        if (!vec) {
+            // rows at any pitch: an element a lane, so that a store covers whole runs all the same
+#pragma unroll 4
+            for (uint32_t r0 = 0; r0 < W; ++r0) {          // 32 / W rows at a time
+                const uint32_t r = r0 * (32 / W) + lane / W, e = lane % W, p = e / (W / 4);
+                const T v = *reinterpret_cast<const T*>(stage + r * 64 + ((p ^ (r >> 1)) & 3) * 16 + e % (W / 4) * sizeof(T));
+                if (row0 + r < row1 && mcol + c0 + e < g.m) ((T*)g.c)[(uint64_t)(row0 + r) * g.ldc + mcol + c0 + e] = v;
+            }
+            continue;
+        }
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
             const uint32_t r = 8 * i + lane / 4, p = lane % 4, col = mcol + c0 + p * (W / 4);
@@ -282,7 +292,7 @@ __device__ __forceinline__ void store_rows(const KArgs& g, uint32_t row0, uint32
             o.u = *reinterpret_cast<const uint4*>(stage + r * 64 + ((p ^ (r >> 1)) & 3) * 16);
             if (row0 + r >= row1) continue;
             T* d = (T*)g.c + (uint64_t)(row0 + r) * g.ldc + col;
-            if (vec && col + W / 4 <= g.m) {
+            if (col + W / 4 <= g.m) {
                 *reinterpret_cast<uint4*>(d) = o.u;
             } else {
 #pragma unroll
@@ -304,10 +314,10 @@ __device__ __forceinline__ void store_one(const KArgs& g, uint64_t i, float v) {
 
 // The token scales of one (tile, K block), as a scale warp holds them on their way from global
 // memory: the loads of a group of four are issued while the group before it waits for room.
-template <int TN, bool TOK>
+template <int TN>
 struct ScaleRegs {
-    float v[TOK ? 4 : TN < 32 ? 1 : TN / 32];
-    float sb[TOK ? 2 : 1];
+    float v[TN < 32 ? 1 : TN / 32];
+    float sb;
 };
 
 // KS: the CTAs of a cluster share one tile, each a contiguous part of its K blocks, and add their
@@ -353,10 +363,10 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
             mbar_init(smem_u32(&empty_b[s]), 1);
         }
         for (int b = 0; b < C::NBUF; ++b) {
-            mbar_init(smem_u32(&accf_b[b]), 1);
+            mbar_init(smem_u32(&accf_b[b]), TOK ? 2 : 1);     // TOK: its MMAs and its scales
             mbar_init(smem_u32(&acce_b[b]), C::EPI_WARPS / C::TURNS * CG);
         }
-        for (int s = 0; s < C::GROUPS; ++s) {
+        for (int s = 0; s < C::GROUPS; ++s) {        // not used by TOK
             mbar_init(smem_u32(&sfull_b[s]), 2);
             mbar_init(smem_u32(&sempty_b[s]), C::EPI_WARPS);
         }
@@ -501,61 +511,112 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                 mbar_wait(smem_u32(done_b), 0, drain);
             }
         } else {
-            // Scale warps: of a tile's K blocks, in groups of four, 2 takes the even ones and 3 the odd
-            // ones; the next group's loads are in flight while this one waits for room.
-            const uint32_t nkb = kb1 - kb0, per = (nkb + 3) / 4;
-            ScaleRegs<TN, TOK> regs[2];
-            bool have[2] = {false, false};
-            uint32_t t = cid, at = 0;            // the next group: tile and place in it
-            TileF8 tc{};
-            const float* sbp = nullptr;
-            uint32_t blocks = 0;                 // weight blocks of this CTA's part of the tile that exist
-            auto fetch = [&]() {
-                if (t >= total) return;
-                if (at == 0) {
-                    tc = decode_tile<C>(g, first, ends, t);
-                    if (TOK) tc.row0 += rank * 128;
-                    else tc.m0 += rank * 128;
-                    blocks = tc.m0 < g.m ? (g.m - tc.m0 + 127) / 128 : 0u;
-                    sbp = g.bs + tc.group * g.bs_gs + (uint64_t)(tc.m0 / 128) * g.b_lds;
-                }
-#pragma unroll
-                for (uint32_t p = 0; p < 2; ++p) {
-                    const uint32_t i = at * 4 + 2 * p + warp - 2, kb = kb0 + i;
-                    have[p] = i < nkb;
-                    if (!have[p]) continue;
-                    ScaleRegs<TN, TOK>& r = regs[p];
-#pragma unroll
-                    for (uint32_t h = 0; h < sizeof(r.sb) / 4; ++h) r.sb[h] = h < blocks ? __ldg(sbp + h * g.b_lds + kb) : 0.0f;
+            if constexpr (TOK) {
+                // Scale warps: K blocks are counted over all tiles of this CTA; warp 2 has the even ones and
+                // with them accumulator 0, warp 3 the odd ones and accumulator 1.  A block's barrier
+                // completes with its MMAs and with its scales' arrival here, so the epilogue waits once.
+                // When block i - 2 is complete, its MMAs were issued, so every epilogue warp has given back
+                // the accumulator of block i - 4 and has read that block's scales: block i + 4 may take
+                // their place in the ring of eight.
+                const uint32_t par = warp - 2;
+                uint32_t t = cid, kb = 0, wblocks = 0;       // the next block to load
+                TileF8 tc{};
+                const float* sbp = nullptr;
+                bool fresh = true;
+                float sa[2][4], sb[2][2];                    // two blocks on their way
+                auto step = [&](uint32_t by) {
+                    for (uint32_t i = 0; i < by; ++i)
+                        if (++kb == g.kb) { kb = 0; t += ncl; fresh = true; }
+                };
+                auto load = [&](float (&a4)[4], float (&b2)[2]) {
+                    if (t >= total) return;
+                    if (fresh) {
+                        tc = decode_tile<C>(g, first, ends, t);
+                        tc.row0 += rank * 128;
+                        wblocks = (g.m - tc.m0 + 127) / 128;       // of which a tile has two at most
+                        sbp = g.bs + tc.group * g.bs_gs + (uint64_t)(tc.m0 / 128) * g.b_lds;
+                        fresh = false;
+                    }
+                    b2[0] = __ldg(sbp + kb);
+                    b2[1] = wblocks > 1 ? __ldg(sbp + g.b_lds + kb) : 0.0f;
                     const float* a = g.as + (uint64_t)kb * g.a_lds + tc.row0;
 #pragma unroll
-                    for (uint32_t q = 0; q < sizeof(r.v) / 4; ++q) {
-                        const uint32_t j = lane + 32 * q;
-                        r.v[q] = (TOK || j < TN) && tc.row0 + j < tc.row1 ? __ldg(a + j) : 0.0f;
+                    for (uint32_t q = 0; q < 4; ++q) a4[q] = tc.row0 + lane + 32 * q < tc.row1 ? __ldg(a + lane + 32 * q) : 0.0f;
+                    step(2);
+                };
+                auto store = [&](uint64_t i, const float (&a4)[4], const float (&b2)[2]) {
+                    float* dst = ring + (uint32_t)(i % C::SLOTS) * TN;
+#pragma unroll
+                    for (uint32_t q = 0; q < 4; ++q) {
+                        dst[lane + 32 * q] = a4[q] * b2[0];
+                        dst[128 + lane + 32 * q] = a4[q] * b2[1];
                     }
+                };
+                const uint64_t items = (uint64_t)(cid < total ? (total - cid + ncl - 1) / ncl : 0u) * g.kb;
+                const uint32_t accf = smem_u32(&accf_b[par]);
+                step(par);
+                load(sa[0], sb[0]);
+                load(sa[1], sb[1]);
+                if (par < items) store(par, sa[0], sb[0]);
+                load(sa[0], sb[0]);
+                if (par + 2 < items) store(par + 2, sa[1], sb[1]);
+                for (uint64_t i = par; i < items; i += 2) {
+                    if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(accf, (uint32_t)(i / 2 - 1) & 1u, wc))) break;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(accf);
+                    if (i + 4 < items) store(i + 4, sa[0], sb[0]);
+                    load(sa[0], sb[0]);
                 }
-                if (++at == per) { at = 0; t += ncl; }
-            };
-            const uint64_t groups = (uint64_t)(cid < total ? (total - cid + ncl - 1) / ncl : 0u) * per;
-            fetch();
-            for (uint64_t grp = 0; grp < groups; ++grp) {
-                const uint32_t gs = (uint32_t)grp % C::GROUPS, use = (uint32_t)(grp / C::GROUPS);
-                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sempty_b[gs]), (use & 1u) ^ 1u, wc))) break;
-#pragma unroll
-                for (uint32_t p = 0; p < 2; ++p) {
-                    float* dst = ring + (gs * 4 + 2 * p + warp - 2) * TN;
-                    if (!have[p]) continue;
-#pragma unroll
-                    for (uint32_t q = 0; q < sizeof(regs[p].v) / 4; ++q) {
-                        const uint32_t j = lane + 32 * q;
-#pragma unroll
-                        for (uint32_t h = 0; h < sizeof(regs[p].sb) / 4; ++h)
-                            if (TOK || j < TN) dst[h * 128 + j] = regs[p].v[q] * regs[p].sb[h];
+            } else {
+                // Scale warps: of a tile's K blocks, in groups of four, 2 takes the even ones and 3 the odd
+                // ones; the next group's loads are in flight while this one waits for room.
+                const uint32_t nkb = kb1 - kb0, per = (nkb + 3) / 4;
+                ScaleRegs<TN> regs[2];
+                bool have[2] = {false, false};
+                uint32_t t = cid, at = 0;            // the next group: tile and place in it
+                TileF8 tc{};
+                const float* sbp = nullptr;
+                auto fetch = [&]() {
+                    if (t >= total) return;
+                    if (at == 0) {
+                        tc = decode_tile<C>(g, first, ends, t);
+                        sbp = g.bs + tc.group * g.bs_gs + (uint64_t)(tc.m0 / 128) * g.b_lds;
                     }
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sfull_b[gs]));
+#pragma unroll
+                    for (uint32_t p = 0; p < 2; ++p) {
+                        const uint32_t i = at * 4 + 2 * p + warp - 2, kb = kb0 + i;
+                        have[p] = i < nkb;
+                        if (!have[p]) continue;
+                        ScaleRegs<TN>& r = regs[p];
+                        r.sb = __ldg(sbp + kb);
+                        const float* a = g.as + (uint64_t)kb * g.a_lds + tc.row0;
+#pragma unroll
+                        for (uint32_t q = 0; q < sizeof(r.v) / 4; ++q) {
+                            const uint32_t j = lane + 32 * q;
+                            r.v[q] = j < TN && tc.row0 + j < tc.row1 ? __ldg(a + j) : 0.0f;
+                        }
+                    }
+                    if (++at == per) { at = 0; t += ncl; }
+                };
+                const uint64_t groups = (uint64_t)(cid < total ? (total - cid + ncl - 1) / ncl : 0u) * per;
                 fetch();
+                for (uint64_t grp = 0; grp < groups; ++grp) {
+                    const uint32_t gs = (uint32_t)grp % C::GROUPS, use = (uint32_t)(grp / C::GROUPS);
+                    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sempty_b[gs]), (use & 1u) ^ 1u, wc))) break;
+#pragma unroll
+                    for (uint32_t p = 0; p < 2; ++p) {
+                        float* dst = ring + (gs * 4 + 2 * p + warp - 2) * TN;
+                        if (!have[p]) continue;
+#pragma unroll
+                        for (uint32_t q = 0; q < sizeof(regs[p].v) / 4; ++q) {
+                            const uint32_t j = lane + 32 * q;
+                            if (j < TN) dst[j] = regs[p].v[q] * regs[p].sb;
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sfull_b[gs]));
+                    fetch();
+                }
             }
         }
     } else {
@@ -574,7 +635,7 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
             const uint32_t acce0 = CG == 2 ? map_to_rank(smem_u32(&acce_b[0]), 0) : smem_u32(&acce_b[0]), accf0 = smem_u32(&accf_b[0]);
             const uint32_t d0 = tmem + half * 128 + (quarter << 21);
             const float* sc = ring + half * 128 + quarter * 32 + lane;
-            uint32_t buf = 0, bphase = 0, slot = 0, sphase = 0;
+            uint32_t buf = 0, bphase = 0, slot = 0;
             bool ok = true;
             for (uint32_t t = cid; t < total; t += ncl) {
                 float acc[128];
@@ -583,30 +644,23 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                 uint32_t r0[CW], r1[CW];
                 // Between a load and its wait there are only additions and barrier tests: nothing that makes
                 // the compiler move a register that the load still writes.
-                auto scale_there = [&]() {            // scales come in groups of four
-                    if (slot % 4 == 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sfull_b[slot / 4]), sphase, wc));
-                };
-                auto columns_there = [&]() {
-                    ok = ok && __all_sync(0xffffffffu, mbar_wait(accf0 + 8 * buf, bphase, wc));
+                float one = 0.0f;
+                auto begin = [&]() {                 // the block's accumulator and scales are there: fetch its first half
+                    ok = __all_sync(0xffffffffu, mbar_wait(accf0 + 8 * buf, bphase, wc));
+                    if (!ok) return;
                     tc_fence_after();
+                    one = sc[slot * TN];
+                    tmem_ld(d0 + buf * TN, r0);
+                    tmem_ld(d0 + buf * TN + CW, r1);
                 };
-                scale_there();
-                columns_there();
+                begin();
                 if (!ok) break;
-                float one = sc[slot * TN];
-                tmem_ld(d0 + buf * TN, r0);
-                tmem_ld(d0 + buf * TN + CW, r1);
                 auto add = [&](int c, const uint32_t (&r)[CW]) {
 #pragma unroll
                     for (int j = 0; j < CW; ++j) acc[c * CW + j] = fmaf(__uint_as_float(r[j]), one, acc[c * CW + j]);
                 };
                 for (uint32_t left = g.kb; left; --left) {
-                    const uint32_t d = d0 + buf * TN, acce = acce0 + 8 * buf, sempty = smem_u32(&sempty_b[slot / 4]);
-                    const bool last_of_group = slot % 4 == 3 || left == 1;
-                    buf ^= 1u;
-                    bphase ^= buf ^ 1u;
-                    slot = left == 1 ? (slot | 3u) + 1u : slot + 1u;    // a tile's groups are its own
-                    if (slot == C::SLOTS) { slot = 0; sphase ^= 1u; }
+                    const uint32_t d = d0 + buf * TN, acce = acce0 + 8 * buf;
                     tmem_ld_done(r0);
                     tmem_ld_done(r1);
                     add(0, r0);
@@ -617,19 +671,14 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                     tmem_ld_done(r1);
                     tc_fence_before();
                     __syncwarp();
-                    if (CG == 2) arrive_cluster_if(lane == 0, acce);
-                    else arrive_if(lane == 0, acce);                     // the accumulator's columns are in registers
-                    arrive_if(lane == 0 && last_of_group, sempty);       // and so is the group's last scale
+                    arrive_cluster_if(lane == 0, acce);      // the accumulator's columns are in registers
                     add(2, r0);
                     add(3, r1);
-                    if (left > 1) {
-                        scale_there();
-                        one = sc[slot * TN];
-                        columns_there();
-                        if (!ok) break;
-                        tmem_ld(d0 + buf * TN, r0);
-                        tmem_ld(d0 + buf * TN + CW, r1);
-                    }
+                    buf ^= 1u;
+                    bphase ^= buf ^ 1u;
+                    slot = (slot + 1u) % C::SLOTS;
+                    if (left > 1) begin();
+                    if (!ok) break;
                 }
                 if (!ok) break;
                 const TileF8 tc = decode_tile<C>(g, first, ends, t);
