@@ -313,7 +313,7 @@ struct NormArgs {
 // threads have no registers to spare for either: they are loaded, and so is the weight, row by row.
 template <typename T, typename WT>
 constexpr uint32_t norm_ctas(uint32_t g) {     // resident an SM
-    return g > 256 ? 1 : g == 256 ? 2 : sizeof(T) + sizeof(WT) == 4 ? 5 : 4 - sizeof(T) / 4;
+    return g > 256 ? 1 : g == 256 ? 2 : sizeof(T) + sizeof(WT) == 4 ? 4 : 4 - sizeof(T) / 4;
 }
 
 template <typename T, typename WT, uint32_t G, bool VEC>

@@ -249,55 +249,81 @@ __device__ __forceinline__ void store_cols(const KArgs& g, const TileF8& tc, uin
     }
 }
 
+// 16 / sizeof(T) values in 16 bytes
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float* v);
+template <>
+__device__ __forceinline__ uint4 pack16<float>(const float* v) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+template <>
+__device__ __forceinline__ uint4 pack16<__nv_bfloat16>(const float* v) {
+    union {
+        __nv_bfloat162 h[4];
+        uint4 u;
+    } o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o.h[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+    return o.u;
+}
+template <>
+__device__ __forceinline__ uint4 pack16<__half>(const float* v) {
+    union {
+        __half2 h[4];
+        uint4 u;
+    } o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o.h[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+    return o.u;
+}
+template <>
+__device__ __forceinline__ uint4 pack16<int16_t>(const float* v) {
+    union {
+        int16_t h[8];
+        uint4 u;
+    } o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) from_f32(v[j], o.h[j]);
+    return o.u;
+}
+
 // TOK: 32 token rows of 128 columns, a row a lane.  64 bytes of each row go through shared memory
 // at a time (16-byte pieces XOR-swizzled over the bank groups), so that a store covers whole
-// 64-byte runs of eight rows instead of 16 bytes of 32.
+// 64-byte runs of eight rows instead of 16 bytes of 32.  The code is passed through once a tile, at
+// the pace of instruction fetches, so what counts is its length.
 template <typename T>
 __device__ __forceinline__ void store_rows(const KArgs& g, uint32_t row0, uint32_t row1, uint32_t mcol, uint8_t* stage, uint32_t lane,
                                            const float (&acc)[128]) {
-    constexpr uint32_t W = 64 / sizeof(T);           // columns of a pass
+    constexpr uint32_t W = 64 / sizeof(T), P = W / 4;          // columns of a pass and of a piece
     const bool vec = (uintptr_t)g.c % 16 == 0 && g.ldc * sizeof(T) % 16 == 0;
+    const uint32_t rows = row1 > row0 ? row1 - row0 : 0u, sw = (lane >> 1) & 3u, rsw = (lane >> 3) & 3u;
+    uint8_t* in = stage + lane * 64;                           // this lane's row
+    const uint8_t* out = stage + lane / 4 * 64 + ((lane ^ rsw) & 3u) * 16;   // piece lane % 4 of rows lane / 4, + 8, ..
+    T* d = (T*)g.c + (uint64_t)(row0 + lane / 4) * g.ldc + mcol + lane % 4 * P;
+    const uint64_t down = 8 * g.ldc;
 #pragma unroll
     for (uint32_t c0 = 0; c0 < 128; c0 += W) {
-        if (mcol + c0 >= g.m) break;                  // the whole warp
+        if (mcol + c0 >= g.m) break;                            // the whole warp
         __syncwarp();
 #pragma unroll
-        for (uint32_t p = 0; p < 4; ++p) {
-            union {
-                T t[W / 4];
-                uint4 u;
-            } o;
-#pragma unroll
-            for (uint32_t j = 0; j < W / 4; ++j) from_f32(acc[c0 + p * (W / 4) + j], o.t[j]);
-            *reinterpret_cast<uint4*>(stage + lane * 64 + ((p ^ (lane >> 1)) & 3) * 16) = o.u;
-        }
+        for (uint32_t p = 0; p < 4; ++p) *reinterpret_cast<uint4*>(in + ((p ^ sw) & 3u) * 16) = pack16<T>(acc + c0 + p * P);
         __syncwarp();
-        if (!vec) {
-            // rows at any pitch: an element a lane, so that a store covers whole runs all the same
-#pragma unroll 4
-            for (uint32_t r0 = 0; r0 < W; ++r0) {          // 32 / W rows at a time
-                const uint32_t r = r0 * (32 / W) + lane / W, e = lane % W, p = e / (W / 4);
-                const T v = *reinterpret_cast<const T*>(stage + r * 64 + ((p ^ (r >> 1)) & 3) * 16 + e % (W / 4) * sizeof(T));
-                if (row0 + r < row1 && mcol + c0 + e < g.m) ((T*)g.c)[(uint64_t)(row0 + r) * g.ldc + mcol + c0 + e] = v;
+        if (vec && mcol + c0 + W <= g.m) {
+            T* e = d + c0;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint4 v = *reinterpret_cast<const uint4*>(out + i * 512);
+                if (8 * i + lane / 4 < rows) *reinterpret_cast<uint4*>(e) = v;
+                e += down;
             }
-            continue;
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t r = 8 * i + lane / 4, p = lane % 4, col = mcol + c0 + p * (W / 4);
-            union {
-                T t[W / 4];
-                uint4 u;
-            } o;
-            o.u = *reinterpret_cast<const uint4*>(stage + r * 64 + ((p ^ (r >> 1)) & 3) * 16);
-            if (row0 + r >= row1) continue;
-            T* d = (T*)g.c + (uint64_t)(row0 + r) * g.ldc + col;
-            if (col + W / 4 <= g.m) {
-                *reinterpret_cast<uint4*>(d) = o.u;
-            } else {
-#pragma unroll
-                for (uint32_t j = 0; j < W / 4; ++j)
-                    if (col + j < g.m) d[j] = o.t[j];
+        } else {
+            // rows at any pitch, or the last columns: an element a lane, so that a store covers whole
+            // runs all the same
+#pragma unroll 8
+            for (uint32_t r0 = 0; r0 < W; ++r0) {               // 32 / W rows at a time
+                const uint32_t r = r0 * (32 / W) + lane / W, e = lane % W;
+                const T v = *reinterpret_cast<const T*>(stage + r * 64 + ((e / P ^ (r >> 1)) & 3u) * 16 + e % P * sizeof(T));
+                if (r < rows && mcol + c0 + e < g.m) ((T*)g.c)[(uint64_t)(row0 + r) * g.ldc + mcol + c0 + e] = v;
             }
         }
     }
@@ -638,6 +664,7 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
             uint32_t buf = 0, bphase = 0, slot = 0;
             bool ok = true;
             for (uint32_t t = cid; t < total; t += ncl) {
+                const TileF8 tc = decode_tile<C>(g, first, ends, t);
                 float acc[128];
 #pragma unroll
                 for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
@@ -681,7 +708,6 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                     if (!ok) break;
                 }
                 if (!ok) break;
-                const TileF8 tc = decode_tile<C>(g, first, ends, t);
                 uint8_t* stage = (uint8_t*)bars + 512 + C::TABLES + (warp - 4) * 2048;
                 const uint32_t row0 = tc.row0 + rank * 128 + quarter * 32, mcol = tc.m0 + half * C::COLS;
                 switch (g.c_type) {
