@@ -11,8 +11,10 @@
 // (With 16 lanes a block and 8 values each, 8192 x 4096 bf16 took 30.9 us instead of 20.3.)
 // Values stay in their own type until they are needed, fp32 works on pairs, and the next rows'
 // loads are issued before the current rows are worked on.
-// Rows whose pitch or base is not a multiple of the vector sizes run the same kernel with
-// one-element accesses, column l + 4 * j of the block.
+// Rows whose base or pitch is not a multiple of the vector sizes keep this layout: a chunk is cut out
+// of the two (fp32: three) aligned 16-byte words that hold it, and 8-bit and 16-bit results leave as
+// aligned 32-bit words put together from neighbouring lanes' (8192 x 1001 bf16, one element an access:
+// 26.9 us quantised and 55.7 us normed; this way UNALIGNED_US).
 #include <algorithm>
 #include <cmath>
 
@@ -26,12 +28,9 @@ constexpr uint32_t kVals = kFp8Block / kLanes;       // values of a lane
 constexpr uint32_t kChunks = kVals / 8;
 
 // column of a lane's value j
-template <bool VEC>
-__device__ __forceinline__ uint32_t column(uint32_t col0, uint32_t l, uint32_t j) {
-    return VEC ? col0 + 8 * (kLanes * (j / 8) + l) + j % 8 : col0 + l + kLanes * j;
-}
+__device__ __forceinline__ uint32_t column(uint32_t col0, uint32_t l, uint32_t j) { return col0 + 8 * (kLanes * (j / 8) + l) + j % 8; }
 
-// A lane's 32 values as they lie in memory; 0 past the row's end.
+// A lane's 32 values as they lie in memory; 0 past the row's end, once trimmed.
 template <typename T>
 struct Raw {
     static constexpr uint32_t W = sizeof(T) / 2;     // 16-byte words of a chunk
@@ -41,31 +40,54 @@ struct Raw {
 #pragma unroll
         for (uint32_t i = 0; i < kChunks * W; ++i) w[i] = make_uint4(0, 0, 0, 0);
     }
+    // VEC: rows start on 16-byte boundaries
     template <bool VEC>
     __device__ __forceinline__ void load(const T* row, uint32_t col0, uint32_t l, uint32_t cols) {
-        if (VEC && col0 + kFp8Block <= cols) {
+        // Aligned words around each chunk; one that holds none of its values is not read, and one that
+        // holds any lies in the row's own memory page.
+        constexpr uint32_t N = VEC ? W : W + 1;
+        const uint32_t skip = VEC ? 0u : (uint32_t)((uintptr_t)(row + col0 + 8 * l) & 15u);    // the same for all chunks of a row
+        uint4 v[kChunks][N];
 #pragma unroll
-            for (uint32_t i = 0; i < kChunks * W; ++i) w[i] = reinterpret_cast<const uint4*>(row + column<VEC>(col0, l, 8 * (i / W)))[i % W];
-            return;
+        for (uint32_t i = 0; i < kChunks; ++i) {
+            const uint32_t c = column(col0, l, 8 * i);
+            const uint32_t bytes = c < cols ? min(8u, cols - c) * (uint32_t)sizeof(T) : 0u;
+            const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(row + c) - skip);
+#pragma unroll
+            for (uint32_t k = 0; k < N; ++k) v[i][k] = bytes && 16 * k < skip + bytes ? p[k] : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (uint32_t i = 0; i < kChunks; ++i) {
-            if (VEC && column<VEC>(col0, l, 8 * i) + 8 <= cols) {      // a whole chunk of the last, partial block
+            uint32_t x[4 * N];
 #pragma unroll
-                for (uint32_t k = 0; k < W; ++k) w[i * W + k] = reinterpret_cast<const uint4*>(row + column<VEC>(col0, l, 8 * i))[k];
-                continue;
+            for (uint32_t k = 0; k < N; ++k) { x[4 * k] = v[i][k].x; x[4 * k + 1] = v[i][k].y; x[4 * k + 2] = v[i][k].z; x[4 * k + 3] = v[i][k].w; }
+            if (!VEC) {
+#pragma unroll
+                for (uint32_t j = 0; j + 2 < 4 * N; ++j) x[j] = skip & 8u ? x[j + 2] : x[j];
+#pragma unroll
+                for (uint32_t j = 0; j + 3 < 4 * N; ++j) x[j] = skip & 4u ? x[j + 1] : x[j];
+                if (sizeof(T) == 2) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4 * W; ++j) x[j] = __funnelshift_r(x[j], x[j + 1], skip & 2u ? 16u : 0u);
+                }
             }
-            union {
-                T t[8];
-                uint4 u[W];
-            } c;
 #pragma unroll
-            for (uint32_t k = 0; k < W; ++k) c.u[k] = make_uint4(0, 0, 0, 0);
+            for (uint32_t k = 0; k < W; ++k) w[i * W + k] = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+        }
+    }
+    // Clears what `load` took from behind the row's end in the last words.  Apart from it, so that
+    // nothing waits for the values between their load and their use.
+    __device__ __forceinline__ void trim(uint32_t col0, uint32_t l, uint32_t cols) {
+        if (col0 + kFp8Block <= cols || cols % 8 == 0) return;
 #pragma unroll
-            for (uint32_t j = 0; j < 8; ++j)
-                if (column<VEC>(col0, l, 8 * i + j) < cols) c.t[j] = row[column<VEC>(col0, l, 8 * i + j)];
+        for (uint32_t i = 0; i < kChunks; ++i) {
+            const uint32_t c = column(col0, l, 8 * i), n = c < cols ? min(8u, cols - c) : 0u;
 #pragma unroll
-            for (uint32_t k = 0; k < W; ++k) w[i * W + k] = c.u[k];
+            for (uint32_t j = 0; j < 4 * W; ++j) {
+                uint32_t& x = reinterpret_cast<uint32_t*>(w)[4 * W * i + j];
+                if (sizeof(T) == 4) x = j < n ? x : 0u;
+                else x = 2 * j + 1 < n ? x : 2 * j < n ? x & 0xffffu : 0u;
+            }
         }
     }
     __device__ __forceinline__ uint32_t word(uint32_t i) const {
@@ -138,7 +160,7 @@ template <> __device__ __forceinline__ float Raw<int16_t>::max_abs() const {
     return m;
 }
 
-// a lane's 32 values in fp32 pairs -> row of T
+// fp32 pairs -> 32-bit words of T
 template <typename T>
 __device__ __forceinline__ uint32_t to_word(uint64_t v);
 template <> __device__ __forceinline__ uint32_t to_word<__nv_bfloat16>(uint64_t v) {
@@ -154,35 +176,106 @@ template <> __device__ __forceinline__ uint32_t to_word<__half>(uint64_t v) {
     return *reinterpret_cast<const uint32_t*>(&b);
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store32(T* row, uint32_t col0, uint32_t l, uint32_t cols, const uint64_t (&v)[kVals / 2]) {
+// Stores the words of a lane's chunks (N of 32 bits each, from `chunk(i, x)`) to elements of S bytes at
+// any alignment.  VEC: as one access a chunk.  Else a chunk starts `odd` bytes (0 to 3, the same for a whole row) behind a 32-bit
+// boundary; its words are shifted up by them, and the chunk before it -- the lane before, or lane 3's
+// last one -- gives the bytes that the first word lacks.  What has no neighbour in the block (its
+// first bytes, its last, and the last ones of a row) is stored by elements.  The four lanes of a block
+// arrive together.
+template <uint32_t S, uint32_t N, bool VEC, typename F>
+__device__ __forceinline__ void store_words(uint8_t* row, uint32_t col0, uint32_t l, uint32_t cols, F chunk) {
+    const uint32_t odd = (uint32_t)((uintptr_t)row + (uintptr_t)col0 * S) & 3u;      // 8 elements are a multiple of 4 bytes
+    const uint32_t lanes = 0xfu << (threadIdx.x & 28u);
+    auto bytes = [&](uint8_t* p, uint32_t word, uint32_t from, uint32_t to) {           // bytes from .. to - 1 of a word, at p + from
+        for (uint32_t k = from; k < to; k += S) {
+            if (S == 1) p[k] = (uint8_t)(word >> (8 * k));
+            else *reinterpret_cast<uint16_t*>(p + k) = (uint16_t)(word >> (8 * k));
+        }
+    };
+    uint32_t x[N], before = 0;                 // before: the last word of this lane's chunk before
 #pragma unroll
     for (uint32_t i = 0; i < kChunks; ++i) {
-        if (VEC && column<VEC>(col0, l, 8 * i) + 8 <= cols) {
-            uint4* d = reinterpret_cast<uint4*>(row + column<VEC>(col0, l, 8 * i));
-            if constexpr (sizeof(T) == 4) {
-                reinterpret_cast<ulonglong2*>(d)[0] = make_ulonglong2(v[4 * i], v[4 * i + 1]);
-                reinterpret_cast<ulonglong2*>(d)[1] = make_ulonglong2(v[4 * i + 2], v[4 * i + 3]);
-            } else {
-                *d = make_uint4(to_word<T>(v[4 * i]), to_word<T>(v[4 * i + 1]), to_word<T>(v[4 * i + 2]), to_word<T>(v[4 * i + 3]));
-            }
-            continue;
+        chunk(i, x);
+        const uint32_t c = column(col0, l, 8 * i), n = c < cols ? min(8u, cols - c) : 0u, at = kLanes * i + l;
+        uint8_t* p = row + (uint64_t)c * S;
+        uint32_t last = 0;
+        if (!VEC) {
+            last = __shfl_sync(lanes, l == kLanes - 1 ? before : x[N - 1], (l + kLanes - 1) % kLanes, kLanes);
+            before = x[N - 1];
         }
+        if (VEC && n == 8) {
+            if constexpr (N == 4) *reinterpret_cast<uint4*>(p) = make_uint4(x[0], x[1], x[2], x[3]);
+            else *reinterpret_cast<uint2*>(p) = make_uint2(x[0], x[1]);
+        } else if (n == 8) {
+            uint32_t* a = reinterpret_cast<uint32_t*>(p - odd);
+            if (odd == 0 || at > 0) a[0] = __funnelshift_l(last, x[0], 8 * odd);
+            else bytes(p, x[0], 0, 4 - odd);
 #pragma unroll
-        for (uint32_t j = 8 * i; j < 8 * i + 8; j += 2) {
-            float lo, hi;
-            unpack2(v[j / 2], lo, hi);
-            if (column<VEC>(col0, l, j) < cols) from_f32(lo, row[column<VEC>(col0, l, j)]);
-            if (column<VEC>(col0, l, j + 1) < cols) from_f32(hi, row[column<VEC>(col0, l, j + 1)]);
+            for (uint32_t j = 1; j < N; ++j) a[j] = __funnelshift_l(x[j - 1], x[j], 8 * odd);
+            if (odd && (at == kLanes * kChunks - 1 || c + 16 > cols)) bytes(p + 4 * (N - 1), x[N - 1], 4 - odd, 4);
+        } else if (n) {
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j)
+                if (4 * j < n * S) bytes(p + 4 * j, x[j], 0, min(4u, n * S - 4 * j));
         }
     }
 }
 
+// a lane's 32 values in fp32 pairs -> row of T
+template <typename T, bool VEC>
+__device__ __forceinline__ void store32(T* row, uint32_t col0, uint32_t l, uint32_t cols, const uint64_t (&v)[kVals / 2]) {
+    if constexpr (sizeof(T) == 2) {
+        store_words<2, 4, VEC>(reinterpret_cast<uint8_t*>(row), col0, l, cols, [&](uint32_t i, uint32_t (&x)[4]) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) x[j] = to_word<T>(v[4 * i + j]);
+        });
+    } else {
+        // As store_words does it, in 16-byte words: a chunk starts `odd` values behind a boundary.
+        const uint32_t odd = VEC ? 0u : (uint32_t)((uintptr_t)(row + col0) / 4) & 3u, lanes = 0xfu << (threadIdx.x & 28u);
+        float before[3] = {};
+#pragma unroll
+        for (uint32_t i = 0; i < kChunks; ++i) {
+            const uint32_t c = column(col0, l, 8 * i), n = c < cols ? min(8u, cols - c) : 0u, at = kLanes * i + l;
+            float x[11];                 // the chunk, behind the last three values of the one before it
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) unpack2(v[4 * i + j], x[3 + 2 * j], x[4 + 2 * j]);
+            T* p = row + c;
+            if (!VEC) {
+#pragma unroll
+                for (uint32_t j = 0; j < 3; ++j) {
+                    x[j] = __shfl_sync(lanes, l == kLanes - 1 ? before[j] : x[8 + j], (l + kLanes - 1) % kLanes, kLanes);
+                    before[j] = x[8 + j];
+                }
+            }
+            if (n < 8 || (!VEC && at == 0)) {
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j)
+                    if (j < n) p[j] = x[3 + j];
+                continue;
+            }
+            const bool end = !VEC && (at == kLanes * kChunks - 1 || c + 16 > cols);
+#pragma unroll
+            for (uint32_t j = 0; j < 3; ++j)
+                if (end && 3 - j <= odd) p[5 + j] = x[8 + j];
+            if (!VEC) {
+#pragma unroll
+                for (uint32_t j = 0; j + 2 < 11; ++j) x[j] = odd & 2u ? x[j] : x[j + 2];
+#pragma unroll
+                for (uint32_t j = 0; j + 3 < 11; ++j) x[j] = odd & 1u ? x[j] : x[j + 1];
+            }
+            constexpr uint32_t f = VEC ? 3 : 0;
+            float4* a = reinterpret_cast<float4*>(p - odd);
+            a[0] = make_float4(x[f], x[f + 1], x[f + 2], x[f + 3]);
+            a[1] = make_float4(x[f + 4], x[f + 5], x[f + 6], x[f + 7]);
+        }
+    }
+}
+
+// the 8-bit values of a lane's 32 (`value(p)`: pair p), times inv
 template <bool VEC, typename V>
 __device__ __forceinline__ void store_q32(uint8_t* row, uint32_t col0, uint32_t l, uint32_t cols, uint32_t format, float inv, V value) {
     const uint64_t inv2 = pack2(inv, inv);
-#pragma unroll
-    for (uint32_t i = 0; i < kChunks; ++i) {
+    auto chunk = [&](uint32_t i, uint32_t (&x)[2]) {
         uint32_t p[4];
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
@@ -190,16 +283,10 @@ __device__ __forceinline__ void store_q32(uint8_t* row, uint32_t col0, uint32_t 
             unpack2(mul2(value(4 * i + j), inv2), lo, hi);
             p[j] = cvt_fp8x2(format, lo, hi);
         }
-        if (VEC && column<VEC>(col0, l, 8 * i) + 8 <= cols) {
-            *reinterpret_cast<uint2*>(row + column<VEC>(col0, l, 8 * i)) = make_uint2(p[0] | (p[1] << 16), p[2] | (p[3] << 16));
-            continue;
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) {
-            const uint32_t c = column<VEC>(col0, l, 8 * i + j);
-            if (c < cols) row[c] = (uint8_t)(p[j / 2] >> (8 * (j & 1)));
-        }
-    }
+        x[0] = p[0] | (p[1] << 16);
+        x[1] = p[2] | (p[3] << 16);
+    };
+    store_words<1, 2, VEC>(row, col0, l, cols, chunk);
 }
 
 constexpr float kTiny = 7.888609052210118e-31f;   // 2^-100
@@ -231,10 +318,10 @@ struct QuantArgs {
 constexpr uint32_t kQRows = 8, kQCols = 8;
 
 template <typename T>
-constexpr uint32_t quant_ctas() { return sizeof(T) == 4 ? 2 : 4; }     // resident an SM: two tiles' values are in registers
+constexpr uint32_t quant_ctas(bool vec) { return sizeof(T) == 4 ? 2 : vec ? 4 : 3; }     // resident an SM: two tiles' values are in registers
 
 template <typename T, bool VEC, uint32_t FMT>
-__global__ void __launch_bounds__(256, quant_ctas<T>()) quant_rows_kernel(const QuantArgs g) {
+__global__ void __launch_bounds__(256, quant_ctas<T>(VEC)) quant_rows_kernel(const QuantArgs g) {
     griddep_wait();
     const uint32_t rt0 = g.fd_col.div(blockIdx.x), ct = blockIdx.x - rt0 * g.col_tiles;
     const uint32_t lane = threadIdx.x % 32, l = lane % kLanes;
@@ -251,9 +338,10 @@ __global__ void __launch_bounds__(256, quant_ctas<T>()) quant_rows_kernel(const 
     uint32_t nz, nrow;
     fetch(rt0, next, nz, nrow);
     for (uint32_t t = rt0; t < g.tiles; t += g.step) {
-        const Raw<T> v = next;
+        Raw<T> v = next;
         const uint32_t z = nz, row = nrow;
         if (t + g.step < g.tiles) fetch(t + g.step, next, nz, nrow);
+        v.trim(col0, l, g.cols);
         float scale;
         const float inv = block_scale(v.max_abs(), l, F, scale);
         if (row < g.rows) {
@@ -276,6 +364,7 @@ __global__ void __launch_bounds__(512) quant_blocks_kernel(const QuantArgs g) {
     Raw<T> v;
     if (live) v.template load<VEC>((const T*)g.x + (uint64_t)z * g.x_bs + row * g.ldx, col0, l, g.cols);
     else v.clear();
+    v.trim(col0, l, g.cols);
     float m = v.max_abs();
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -302,30 +391,30 @@ struct NormArgs {
     void* y;
     uint8_t* q;
     float* scale;
-    uint32_t rows, cols, format, weight_type;
+    uint32_t rows, cols, format, weight_type, per_row;
     uint64_t ldx, ldr, ldo, ldy, ldq, lds;
     float eps;
 };
 
-// G threads share a row, which stays in their registers, a block to 4 of them, and then take the
-// row gridDim rows on.  The weight's values of a thread stay in its registers for all its rows: in
-// the tensors' own type where that is the weight's (WT = T), else in fp32.  Rows of more than 256
-// threads have no registers to spare for either: they are loaded, and so is the weight, row by row.
-template <typename T, typename WT>
-constexpr uint32_t norm_ctas(uint32_t g) {     // resident an SM
-    return g > 256 ? 1 : g == 256 ? 2 : sizeof(T) + sizeof(WT) == 4 ? 4 : 4 - sizeof(T) / 4;
-}
+// per_row threads share a row, which stays in their registers, a block to 4 of them, and then take
+// the row gridDim rows on: a part of a warp, or all warps of the CTA.  16-bit weights stay in the
+// threads' registers for all their rows; others (WT = float: the weight is fp32, or of the other
+// 16-bit type) are read again for each row.  BIG: rows of so many threads that there are registers for
+// neither the weight nor the next row's loads.
+template <typename T>
+constexpr uint32_t norm_threads() { return sizeof(T) == 4 ? 384 : 512; }     // an SM's, at 168 and 128 registers each
 
-template <typename T, typename WT, uint32_t G, bool VEC>
-__global__ void __launch_bounds__(G < 128 ? 128 : G, norm_ctas<T, WT>(G)) rmsnorm_kernel(const NormArgs g) {
+template <typename T, typename WT, bool VEC, uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS, 1) rmsnorm_kernel(const NormArgs g) {
     griddep_wait();
-    constexpr bool AHEAD = G <= 256;
-    constexpr uint32_t ROWS = G < 128 ? 128 / G : 1;
+    constexpr bool BIG = THREADS > norm_threads<T>(), KEEP = sizeof(WT) == 2 && !BIG;
     __shared__ float part[2][32];
-    const uint32_t t = threadIdx.x % G, l = t % kLanes, blk = t / kLanes, col0 = blk * kFp8Block;
+    const bool whole = g.per_row > 32;           // all warps of the CTA on one row
+    const uint32_t t = whole ? threadIdx.x : threadIdx.x & (g.per_row - 1), l = t % kLanes, blk = t / kLanes, col0 = blk * kFp8Block;
+    const uint32_t per_cta = whole ? 1u : blockDim.x / g.per_row, warps = blockDim.x / 32;
     const bool mine = col0 < g.cols;
-    uint32_t row = blockIdx.x * ROWS + threadIdx.x / G;
-    const uint32_t step = gridDim.x * ROWS;
+    uint32_t row = blockIdx.x * per_cta + (whole ? 0u : threadIdx.x / g.per_row);
+    const uint32_t step = gridDim.x * per_cta;
     Raw<T> x, r;
     x.clear();
     r.clear();
@@ -334,33 +423,21 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, norm_ctas<T, WT>(G)) rmsnor
         x.template load<VEC>((const T*)g.x + i * g.ldx, col0, l, g.cols);
         if (g.resid) r.template load<VEC>((const T*)g.resid + i * g.ldr, col0, l, g.cols);
     };
-    if (AHEAD) fetch(row);
+    if (!BIG) fetch(row);
     Raw<WT> w;
-    w.clear();
-    auto fetch_weight = [&]() {
-        if (!mine || !g.weight) return;
-        if constexpr (sizeof(WT) == sizeof(T)) {
-            w.template load<VEC>((const WT*)g.weight, col0, l, g.cols);
-        } else if (g.weight_type == CM_T_F32) {
-            w.template load<VEC>((const WT*)g.weight, col0, l, g.cols);
-        } else {
-            // the other 16-bit type: element by element, once a thread
-#pragma unroll
-            for (uint32_t j = 0; j < kVals; ++j) {
-                const uint32_t c = column<VEC>(col0, l, j);
-                if (c < g.cols)
-                    reinterpret_cast<float*>(w.w)[j] = g.weight_type == CM_T_F16 ? to_f32(((const __half*)g.weight)[c])
-                                                                                 : to_f32(((const __nv_bfloat16*)g.weight)[c]);
-            }
-        }
-    };
-    if (AHEAD) fetch_weight();
+    if (KEEP) {
+        w.clear();
+        if (mine && g.weight) w.template load<VEC>((const WT*)g.weight, col0, l, g.cols);
+        w.trim(col0, l, g.cols);
+    }
     const float F = fp8_largest(g.format), inv_cols = 1.0f / (float)g.cols;
     // every thread of a CTA makes the same number of passes: the barrier below is the CTA's
-    for (uint32_t first = blockIdx.x * ROWS, pass = 0; first < g.rows; first += step, row += step, pass ^= 1) {
+    for (uint32_t first = blockIdx.x * per_cta, pass = 0; first < g.rows; first += step, row += step, pass ^= 1) {
         const bool in = mine && row < g.rows;
         uint64_t h[kVals / 2];
-        if (!AHEAD) fetch(row);
+        if (BIG) fetch(row);
+        x.trim(col0, l, g.cols);
+        r.trim(col0, l, g.cols);
         if (g.resid) {
 #pragma unroll
             for (uint32_t p = 0; p < kVals / 2; ++p) h[p] = add2(x.pair(p), r.pair(p));
@@ -368,20 +445,19 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, norm_ctas<T, WT>(G)) rmsnor
 #pragma unroll
             for (uint32_t p = 0; p < kVals / 2; ++p) h[p] = x.pair(p);
         }
-        if (AHEAD) fetch((uint64_t)row + step);
+        if (!BIG) fetch((uint64_t)row + step);
         uint64_t s2[4] = {};
 #pragma unroll
         for (uint32_t p = 0; p < kVals / 2; ++p) s2[p % 4] = fma2(h[p], h[p], s2[p % 4]);
         float ss, other;
         unpack2(add2(add2(s2[0], s2[1]), add2(s2[2], s2[3])), ss, other);
         ss += other;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (G > 32) {
+        for (uint32_t o = min(g.per_row, 32u) / 2; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (whole) {
             // two sets of partial sums in turn: one barrier a row is enough
             if (threadIdx.x % 32 == 0) part[pass][threadIdx.x / 32] = ss;
             __syncthreads();
-            ss = threadIdx.x % 32 < G / 32 ? part[pass][threadIdx.x % 32] : 0.0f;
+            ss = threadIdx.x % 32 < warps ? part[pass][threadIdx.x % 32] : 0.0f;
 #pragma unroll
             for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         }
@@ -390,19 +466,33 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, norm_ctas<T, WT>(G)) rmsnor
         if (in && g.resid_out) store32<T, VEC>((T*)g.resid_out + (uint64_t)row * g.ldo, col0, l, g.cols, h);
 #pragma unroll
         for (uint32_t p = 0; p < kVals / 2; ++p) h[p] = mul2(h[p], rms2);
-        if (g.weight) {
-            if (!AHEAD) fetch_weight();
+        auto times = [&](const auto& v) {
 #pragma unroll
-            for (uint32_t p = 0; p < kVals / 2; ++p) h[p] = mul2(h[p], w.pair(p));
+            for (uint32_t p = 0; p < kVals / 2; ++p) h[p] = mul2(h[p], v.pair(p));
+        };
+        auto times_read = [&](auto type) {
+            using U = decltype(type);
+            Raw<U> v;
+            v.clear();
+            if (mine) v.template load<VEC>((const U*)g.weight, col0, l, g.cols);
+            v.trim(col0, l, g.cols);
+            times(v);
+        };
+        if (g.weight) {
+            if constexpr (KEEP) times(w);
+            else if constexpr (sizeof(WT) == 2) times_read(WT{});
+            else if (g.weight_type == CM_T_F32) times_read(float{});
+            else if (g.weight_type == CM_T_F16) times_read(__half{});
+            else times_read(__nv_bfloat16{});
         }
         if (in && g.y) store32<T, VEC>((T*)g.y + (uint64_t)row * g.ldy, col0, l, g.cols, h);
         if (!g.q) continue;
-        if (col0 + kFp8Block > g.cols) {   // columns past the row's end hold no value (an infinite rms would make 0 * inf of them)
+        if (col0 + kFp8Block > g.cols && rms > 3.4028234663852886e38f) {   // columns past the row's end hold no value: 0 * inf would be one
 #pragma unroll
             for (uint32_t j = 0; j < kVals; j += 2) {
                 float lo, hi;
                 unpack2(h[j / 2], lo, hi);
-                h[j / 2] = pack2(column<VEC>(col0, l, j) < g.cols ? lo : 0.0f, column<VEC>(col0, l, j + 1) < g.cols ? hi : 0.0f);
+                h[j / 2] = pack2(column(col0, l, j) < g.cols ? lo : 0.0f, column(col0, l, j + 1) < g.cols ? hi : 0.0f);
             }
         }
         float m = 0.0f, scale;
@@ -441,14 +531,17 @@ void launch_quant_type(const QuantArgs& g, bool blocks, bool vec, unsigned forma
 }
 
 template <typename T, typename WT, bool VEC>
-void launch_norm(const Context* cx, const NormArgs& g, cudaStream_t s) {
-    // threads a row: the fewest that hold it (32 values each); CTAs: what the SMs hold at once
-    auto ctas = [&](unsigned threads, uint32_t rows) { return std::min(rows, (uint32_t)cx->sm_count * norm_ctas<T, WT>(threads)); };
-    if (g.cols <= 32 * kVals) launch_k(rmsnorm_kernel<T, WT, 32, VEC>, ctas(128, (g.rows + 3) / 4), 128, 0, s, g);
-    else if (g.cols <= 128 * kVals) launch_k(rmsnorm_kernel<T, WT, 128, VEC>, ctas(128, g.rows), 128, 0, s, g);
-    else if (g.cols <= 256 * kVals) launch_k(rmsnorm_kernel<T, WT, 256, VEC>, ctas(256, g.rows), 256, 0, s, g);
-    else if (g.cols <= 512 * kVals) launch_k(rmsnorm_kernel<T, WT, 512, VEC>, ctas(512, g.rows), 512, 0, s, g);
-    else launch_k(rmsnorm_kernel<T, WT, 1024, VEC>, ctas(1024, g.rows), 1024, 0, s, g);
+void launch_norm(const Context* cx, NormArgs g, cudaStream_t s) {
+    // threads a row: four a block; below a warp a power of two, then whole warps
+    const uint32_t need = (g.cols + kFp8Block - 1) / kFp8Block * kLanes;
+    g.per_row = need > 32 ? (need + 31) / 32 * 32 : 4;
+    while (g.per_row < need) g.per_row *= 2;
+    const uint32_t threads = need > 32 ? g.per_row : 128, rows = threads / g.per_row;
+    const uint32_t hold = (uint32_t)cx->sm_count * std::max(1u, norm_threads<T>() / threads);
+    const uint32_t grid = std::min((g.rows + rows - 1) / rows, hold);
+    if (threads <= norm_threads<T>()) launch_k(rmsnorm_kernel<T, WT, VEC, norm_threads<T>()>, grid, threads, 0, s, g);
+    else if (threads <= 512) launch_k(rmsnorm_kernel<T, WT, VEC, 512>, grid, threads, 0, s, g);
+    else launch_k(rmsnorm_kernel<T, WT, VEC, 1024>, grid, threads, 0, s, g);
 }
 
 template <typename T>
@@ -499,14 +592,14 @@ extern "C" int cm_quant_fp8_async(const void* x, unsigned x_type, uint8_t* q, fl
     if (tiles >= (1u << 30) || tiles * g.col_tiles >= (1u << 31)) return set_error(CM_EUNSUPPORTED, "cm_quant_fp8: more than 2^31 tiles");
     g.tiles = (uint32_t)tiles;
     // blocks: one CTA each; rows: as many CTAs as the SMs hold, each walking down its column tile
-    const uint32_t hold = (x_type == CM_T_F32 ? quant_ctas<float>() : quant_ctas<__half>()) * cx->sm_count;
+    const bool vec = aligned(x, ldx * size, 16) && aligned(q, ldq, 8) &&
+                     (batch == 1 || (x_batch_stride * size % 16 == 0 && q_batch_stride % 8 == 0));
+    const uint32_t hold = (x_type == CM_T_F32 ? quant_ctas<float>(vec) : quant_ctas<__half>(vec)) * cx->sm_count;
     g.step = blocks ? g.tiles : std::min(g.tiles, std::max(1u, hold / g.col_tiles));
     g.fd_row = FastDiv(g.row_tiles);
     g.fd_col = FastDiv(g.col_tiles);
     const unsigned grid = g.step * g.col_tiles;
     const cudaStream_t s = (cudaStream_t)stream;
-    const bool vec = aligned(x, ldx * size, 16) && aligned(q, ldq, 8) &&
-                     (batch == 1 || (x_batch_stride * size % 16 == 0 && q_batch_stride % 8 == 0));
     {
         ProfScope ps_(PK_FP8_QUANT, s);
         switch (x_type) {
@@ -560,7 +653,7 @@ extern "C" int cm_rmsnorm_fp8_async(const void* x, const void* resid, const void
     int rc = enter(&cx);
     if (rc) return rc;
     if (rows == 0 || cols == 0) return CM_OK;
-    NormArgs g{x, resid, weight, resid_out, y, q, scale, rows, cols, format, weight_type, ldx, ldr, ldo, ldy, ldq, lds, eps};
+    NormArgs g{x, resid, weight, resid_out, y, q, scale, rows, cols, format, weight_type, 0, ldx, ldr, ldo, ldy, ldq, lds, eps};
     const cudaStream_t s = (cudaStream_t)stream;
     const bool vec = aligned(x, ldx * size, 16) && (!resid || aligned(resid, ldr * size, 16)) &&
                      (!resid_out || aligned(resid_out, ldo * size, 16)) && (!y || aligned(y, ldy * size, 16)) &&
