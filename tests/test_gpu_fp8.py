@@ -236,6 +236,66 @@ def test_rmsnorm_nan_stays_in_its_row(cm):
     assert torch.isfinite(q.float().cpu()[~bad]).all()
 
 
+def ring(rows, cols, t, pitch, offset):
+    """A byte buffer of 0xA5 and the view of [rows][cols] elements of t inside it."""
+    size = t.itemsize
+    b = torch.full(((offset + rows * pitch + 64) * size,), 0xA5, dtype=torch.uint8, device="cuda")
+    return b, b.view(t)[offset: offset + rows * pitch].view(rows, pitch)[:, :cols]
+
+
+# The layout of the rows changes neither the formula nor the order of a sum: every offset gives the
+# bits of the aligned call (which the tests above hold to 64 bits), and writes nothing beside its rows.
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("cols", [1, 7, 8, 9, 100, 127, 128, 130, 257, 384, 500, 1001, 1023, 1100])
+def test_rows_at_every_offset(cm, t, cols):
+    rows = 37
+    aligned = -(-cols // 16) * 16
+    x, r = pitched(values(cols, rows, cols).to(t), aligned), pitched(values(cols + 1, rows, cols).to(t), aligned)
+    w = (1 + 0.2 * values(cols, cols)).to(t).cuda()
+    make = lambda: [ring(rows, cols, d, aligned, 0)[1] for d in (t, t, torch.uint8, torch.uint8)] + [torch.empty(up(cols), rows, device="cuda") for _ in "12"]  # noqa: E731
+    want = make()
+    cm.RmsNormKernelFp8(x, w, want[2].view(E4), want[4], rows, cols, resid=r, resid_out=want[0], y=want[1])
+    cm.QuantKernelFp8(x, want[3].view(E5), want[5], rows, cols)
+    for i, off in enumerate([0, 1, 2, 3, 4, 5, 7, 8, 11, 15]):
+        pitch = cols + (0, 1, 3, 8)[i % 4]
+        xs, rs, ws = ring(rows, cols, t, pitch, off)[1].copy_(x), ring(rows, cols, t, pitch, (off * 3) % 8)[1].copy_(r), ring(1, cols, t, cols, off)[1][0].copy_(w)
+        bufs = [ring(rows, cols, d, pitch, (off * k) % 16) for d, k in ((t, 1), (t, 5), (torch.uint8, 1), (torch.uint8, 3))]
+        s1, s2 = torch.empty(up(cols), rows, device="cuda"), torch.empty(up(cols), rows, device="cuda")
+        cm.RmsNormKernelFp8(xs, ws, bufs[2][1].view(E4), s1, rows, cols, resid=rs, resid_out=bufs[0][1], y=bufs[1][1])
+        cm.QuantKernelFp8(xs, bufs[3][1].view(E5), s2, rows, cols)
+        assert torch.equal(s1, want[4]) and torch.equal(s2, want[5]), off
+        for (b, v), u in zip(bufs, want):
+            assert torch.equal(v.contiguous().view(torch.uint8), u.contiguous().view(torch.uint8)), off
+            v.view(torch.uint8).fill_(0xA5)
+            assert (b == 0xA5).all(), off
+
+
+@pytest.mark.parametrize("rows,cols", [(3000, 1), (5000, 120), (2500, 250), (1300, 640), (1200, 1500), (300, 9000)])
+def test_rmsnorm_more_rows_than_a_pass(cm, rows, cols):
+    x, w = values(rows, rows, cols).to(BF16), (1 + 0.2 * values(cols, cols)).to(BF16)
+    y = torch.empty(rows, cols, dtype=BF16, device="cuda")
+    q, s = torch.empty(rows, cols, dtype=E4, device="cuda"), torch.empty(up(cols), rows, device="cuda")
+    cm.RmsNormKernelFp8(x.cuda(), w.cuda(), q, s, rows, cols, eps=1e-6, y=y)
+    h = x.double()
+    want = h / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-6) * w.double()
+    assert ((y.double().cpu() - want).abs() <= (24 * U + half(BF16)) * want.abs()).all()
+    sc = expand(s, rows, cols, 1)
+    err = (q.double().cpu() * sc - want).abs()
+    assert (err <= torch.maximum(HALF_STEP[E4] * want.abs(), HALF_SUBNORMAL[E4] * sc) + 32 * U * want.abs()).all()
+
+
+def test_rmsnorm_in_place_unaligned(cm):
+    rows, cols = 700, 1001
+    x, r, w = values(1, rows, cols).to(F16).cuda(), values(2, rows, cols).to(F16).cuda(), values(3, cols).to(F16).cuda()
+    q1, q2 = (torch.empty(rows, cols, dtype=E5, device="cuda") for _ in range(2))
+    s1, s2 = (torch.empty(up(cols), rows, device="cuda") for _ in range(2))
+    ro, y = torch.empty_like(x), torch.empty_like(x)
+    cm.RmsNormKernelFp8(x, w, q1, s1, rows, cols, resid=r, resid_out=ro, y=y)
+    cm.RmsNormKernelFp8(x, w, q2, s2, rows, cols, resid=r, resid_out=r, y=x)
+    assert torch.equal(r, ro) and torch.equal(x, y) and torch.equal(s1, s2)
+    assert torch.equal(q1.view(torch.uint8), q2.view(torch.uint8))
+
+
 # ---- products ---------------------------------------------------------------------------------------
 def operands(seed, n, k, m, af=E4, bf=E4, groups=0):
     """(a, a_scale, b, b_scale) on the CPU: 8-bit values and scales as the quantising entries store them."""
