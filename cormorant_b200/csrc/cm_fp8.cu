@@ -8,13 +8,16 @@
 // Chunk i of lane l is the 8 columns from 8 * (4 * i + l): the 4 lanes of a block read 64
 // neighbouring bytes of a 2-byte type with one load and write one 32-byte sector with one store;
 // the maximum is two shuffles, and of the two quotients lane 0 takes A / F and the others F / A.
-// (With 16 lanes a block and 8 values each, 8192 x 4096 bf16 took 30.9 us instead of 20.3.)
+// (With 16 lanes a block and 8 values each, 8192 x 4096 bf16 took 30.9 us instead of 20.3; 17.7 us,
+// 5.7 TB/s, by now, and 39 us, 6.0 TB/s, normed with the residual's addition.)
 // Values stay in their own type until they are needed, fp32 works on pairs, and the next rows'
 // loads are issued before the current rows are worked on.
 // Rows whose base or pitch is not a multiple of the vector sizes keep this layout: a chunk is cut out
 // of the two (fp32: three) aligned 16-byte words that hold it, and 8-bit and 16-bit results leave as
 // aligned 32-bit words put together from neighbouring lanes' (8192 x 1001 bf16, one element an access:
-// 26.9 us quantised and 55.7 us normed; this way UNALIGNED_US).
+// 26.9 us quantised and 55.7 us normed; this way 10.6 and 27).  What lies behind a row's end in its
+// last words is cleared where the values are used: done at the load, or by blocks that take another
+// path than whole ones, it cost 8192 x 2000 bf16 normed 31 us instead of 22..
 #include <algorithm>
 #include <cmath>
 
@@ -309,13 +312,15 @@ struct QuantArgs {
     uint32_t rows, cols;
     uint64_t ldx, ldq, lds, x_bs, q_bs, s_bs;
     uint32_t row_tiles, col_tiles, tiles, step;   // row tiles a matrix, column tiles, row tiles of the batch, row tiles a pass
+    uint32_t wide;                                // log2 of the column blocks of a CTA's tile
     FastDiv fd_row, fd_col;
 };
 
 // A warp takes 8 rows of a column block -- their scales lie side by side and fill one 32-byte
 // sector --, a CTA 8 rows x 8 column blocks, 2 KB of a row of a 2-byte type, and then the rows
-// `step` tiles on.
-constexpr uint32_t kQRows = 8, kQCols = 8;
+// `step` tiles on.  Where that many column blocks would leave warps idle in a narrow matrix or in the
+// last column tile, the tile is 4, 2 or 1 blocks wide and 2, 4 or 8 times as high (8192 x 100 bf16: 6.5 -> 4.1 us).
+constexpr uint32_t kQRows = 8, kQWarps = 8;
 
 template <typename T>
 constexpr uint32_t quant_ctas(bool vec) { return sizeof(T) == 4 ? 2 : vec ? 4 : 3; }     // resident an SM: two tiles' values are in registers
@@ -325,12 +330,13 @@ __global__ void __launch_bounds__(256, quant_ctas<T>(VEC)) quant_rows_kernel(con
     griddep_wait();
     const uint32_t rt0 = g.fd_col.div(blockIdx.x), ct = blockIdx.x - rt0 * g.col_tiles;
     const uint32_t lane = threadIdx.x % 32, l = lane % kLanes;
-    const uint32_t cb = ct * kQCols + threadIdx.x / 32, col0 = cb * kFp8Block;
+    const uint32_t warp = threadIdx.x / 32, first = (warp >> g.wide) * kQRows + lane / kLanes, tile_rows = (kQWarps >> g.wide) * kQRows;
+    const uint32_t cb = (ct << g.wide) + (warp & ((1u << g.wide) - 1)), col0 = cb * kFp8Block;
     if (col0 >= g.cols) return;                        // the whole warp
     const float F = fp8_largest(FMT);
     auto fetch = [&](uint32_t t, Raw<T>& v, uint32_t& z, uint32_t& row) {
         z = g.fd_row.div(t);
-        row = (t - z * g.row_tiles) * kQRows + lane / kLanes;
+        row = (t - z * g.row_tiles) * tile_rows + first;
         if (row < g.rows) v.template load<VEC>((const T*)g.x + (uint64_t)z * g.x_bs + row * g.ldx, col0, l, g.cols);
         else v.clear();
     };
@@ -586,8 +592,10 @@ extern "C" int cm_quant_fp8_async(const void* x, unsigned x_type, uint8_t* q, fl
     if (rc) return rc;
     if (rows == 0 || cols == 0 || batch == 0) return CM_OK;
     QuantArgs g{x, q, scale, rows, cols, ldx, ldq, lds, x_batch_stride, q_batch_stride, scale_batch_stride};
-    g.row_tiles = (uint32_t)(blocks ? rb : (rows + (uint64_t)kQRows - 1) / kQRows);
-    g.col_tiles = (uint32_t)(blocks ? cb : (cb + kQCols - 1) / kQCols);
+    for (g.wide = 3; g.wide && ((cb - 1) >> g.wide) + 1 > (cb + cb / 8) >> g.wide; --g.wide) {}     // at most an eighth of the warps idle
+    const uint64_t tile_rows = (kQWarps >> g.wide) * kQRows;
+    g.row_tiles = (uint32_t)(blocks ? rb : (rows + tile_rows - 1) / tile_rows);
+    g.col_tiles = (uint32_t)(blocks ? cb : ((cb - 1) >> g.wide) + 1);
     const uint64_t tiles = (uint64_t)g.row_tiles * batch;
     if (tiles >= (1u << 30) || tiles * g.col_tiles >= (1u << 31)) return set_error(CM_EUNSUPPORTED, "cm_quant_fp8: more than 2^31 tiles");
     g.tiles = (uint32_t)tiles;
