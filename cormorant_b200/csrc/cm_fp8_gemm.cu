@@ -3,13 +3,24 @@
 // dense (cm_matmul_fp8) and grouped by expert (cm_matmul_fp8_grouped: rows offsets[g] ..
 // offsets[g+1] - 1 of a and c use b[g]).
 //
-// The weights are the tensor cores' 128-row operand and the tokens their N operand:
-//   D[128 weight rows (TMEM lanes)][TN tokens (TMEM columns)] = one 128-deep block of K
-// so a tile's weight scale is one number a block (a tile is one weight-scale block high), a single
-// token costs a 16-column tile instead of a 128-row one, and an output column is 32 neighbouring
-// lanes: its stores are whole sectors.  A block's product is a fresh accumulator (4 MMAs, 32 deep);
-// epilogue warps take it out of TMEM and add it, times token scale * weight scale, to fp32 sums in
-// registers while the next blocks' MMAs run into other TMEM buffers.
+// A block's product is a fresh accumulator (4 MMAs, 32 deep); epilogue warps take it out of TMEM and
+// add it, times token scale * weight scale, to fp32 sums in registers while the next blocks' MMAs run
+// into other TMEM buffers.  There are two layouts:
+//   few tokens   The weights are the tensor cores' 128-row operand and TN = 16, 32 or 64 tokens their
+//                N operand: D[128 weight rows (TMEM lanes)][TN tokens (TMEM columns)].  A single token
+//                costs a 16-column tile instead of a 128-row one, the weight scale is one number a
+//                block, and an output column is 32 neighbouring lanes: its stores are whole sectors.
+//   many (TOK)   Two SMs share a tile of 256 tokens (the M operand) and TN = 128 or 256 weight rows:
+//                D[128 tokens a CTA][TN weight rows].  A thread's columns are of one weight block, so a
+//                block's scale is one number a thread, and each SM stages half of the N operand.
+//                (128 x 128 tiles of one SM, which stage both operands whole and read a scale a
+//                column, took 19.8 us at 300 x 4096 x 4096, and 256 x 128 tiles of two 14.7.)
+// What bounds it: one token is the weights' HBM read and the launch (4096 x 4096: 7.4 us); ragged and
+// middle sizes are the pace at which one SM takes its operands from L2, some 100 KB a microsecond,
+// times the waves; 8192 x 4096 x 11008 (335 us, 2.2 PFLOP/s) is the exchange of the two accumulators
+// that TMEM holds between MMAs and additions: a block of 0.28 us of MMAs (measured alone) takes 0.38
+// to 0.42 us.  Accumulators handed over in halves (353 us) and blocks fetched into a second set of
+// registers while the one before is added (256 x 128 tiles: 396 -> 489 us) were slower.
 //
 // Warps: 0 TMA producer, 1 MMA issuer (of the pair's leader), 2-3 token scales (global memory ->
 // times the weight scale -> a ring in shared memory), 4.. epilogue.  Every mbarrier wait is bounded
@@ -50,30 +61,32 @@ struct KArgs {
 
 template <int TN, int CG, bool TOK>
 struct F8Cfg {
-    // eight epilogue warps: from 128 columns on, four for each half of the columns; narrower tiles'
-    // K blocks go to the two fours in turn, which add their sums at the end of a tile (a block costs a
-    // warp some 500 cycles of waiting whatever its width)
+    // Eight epilogue warps.  TOK: four for each half of the columns.  Else the K blocks go to the two
+    // fours in turn, which add their sums at the end of a tile (a block costs a warp some 500 cycles of
+    // waiting whatever its width).
     static constexpr int EPI_WARPS = 8;
-    static constexpr int TURNS = TN >= 128 ? 1 : 2;
-    static constexpr int COLS = TURNS == 1 ? TN / 2 : TN;    // accumulator columns of an epilogue warp
+    static constexpr int TURNS = TOK ? 1 : 2;
+    static constexpr int COLS = TN / 2 * TURNS;              // accumulator columns of an epilogue warp
     static constexpr int THREADS = 128 + 32 * EPI_WARPS;
     static constexpr uint32_t TOKENS = TOK ? 128 * CG : TN;  // token rows of a tile
     static constexpr uint32_t WEIGHTS = TOK ? TN : 128 * CG; // weight rows of a tile
     static constexpr bool SPLIT_REGS = TN == 256;            // 128 sums a thread: registers move to the epilogue warps
     static constexpr int A_TILE = 128 * 128, B_TILE = TN / CG * 128;
     static constexpr int STAGE = A_TILE + B_TILE;
-    static constexpr int STAGES = TN >= 128 ? 6 : TN == 64 ? 7 : TN == 32 ? 9 : 10;
+    static constexpr int STAGES = TN == 256 ? 6 : TN == 128 ? 8 : TN == 64 ? 7 : TN == 32 ? 9 : 10;
     static constexpr int NBUF = TN == 256 ? 2 : 4;           // accumulators in TMEM
-    static constexpr int SLOTS = 8;                          // scale ring: K blocks, in groups of 4 with a barrier each way
+    // scale ring: K blocks (not TOK: in groups of 4 with a barrier each way)
+    static constexpr int SLOTS = TOK ? 2 * NBUF + 4 : 8;
     static constexpr int GROUPS = SLOTS / 4;
     static constexpr uint32_t TMEM_COLS = NBUF * TN;
     static constexpr int TABLES = (2 * (kMaxGroups + 1) * 4 + 15) / 16 * 16;
     static_assert((STAGES * STAGE + SLOTS * TN * 4) % 16 == 0, "what follows the ring is 16-byte aligned");
     // output staging, 32 rows x 64 bytes a warp; or the sums that the two fours exchange
-    static constexpr int OUT = TOK ? EPI_WARPS * 2048 : TURNS == 2 ? TN * 128 * 4 : 0;
+    static constexpr int OUT = TOK ? EPI_WARPS * 2048 : TN * 128 * 4;
     static constexpr int SMEM = 1024 + STAGES * STAGE + SLOTS * TN * 4 + 512 + TABLES + OUT;
     static_assert(SMEM <= 232448 && 2 * SMEM > 232448, "one CTA an SM");
-    static_assert(TN * 512 <= STAGES * STAGE, "partial sums of a split tile fit the stages");
+    static_assert(TOK == (CG == 2) && TOK == (TN >= 128), "token rows are the M operand of the wide tiles, which take a pair of SMs");
+    static_assert(TOK || TN * 512 <= STAGES * STAGE, "partial sums of a split tile fit the stages");
 };
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
@@ -291,9 +304,9 @@ __device__ __forceinline__ uint4 pack16<int16_t>(const float* v) {
 // at a time (16-byte pieces XOR-swizzled over the bank groups), so that a store covers whole
 // 64-byte runs of eight rows instead of 16 bytes of 32.  The code is passed through once a tile, at
 // the pace of instruction fetches, so what counts is its length.
-template <typename T>
+template <typename T, int COLS>
 __device__ __forceinline__ void store_rows(const KArgs& g, uint32_t row0, uint32_t row1, uint32_t mcol, uint8_t* stage, uint32_t lane,
-                                           const float (&acc)[128]) {
+                                           const float (&acc)[COLS]) {
     constexpr uint32_t W = 64 / sizeof(T), P = W / 4;          // columns of a pass and of a piece
     const bool vec = (uintptr_t)g.c % 16 == 0 && g.ldc * sizeof(T) % 16 == 0;
     const uint32_t rows = row1 > row0 ? row1 - row0 : 0u, sw = (lane >> 1) & 3u, rsw = (lane >> 3) & 3u;
@@ -302,7 +315,7 @@ __device__ __forceinline__ void store_rows(const KArgs& g, uint32_t row0, uint32
     T* d = (T*)g.c + (uint64_t)(row0 + lane / 4) * g.ldc + mcol + lane % 4 * P;
     const uint64_t down = 8 * g.ldc;
 #pragma unroll
-    for (uint32_t c0 = 0; c0 < 128; c0 += W) {
+    for (uint32_t c0 = 0; c0 < COLS; c0 += W) {
         if (mcol + c0 >= g.m) break;                            // the whole warp
         __syncwarp();
 #pragma unroll
@@ -478,7 +491,7 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                             if (leader) mbar_expect_tx(smem_u32(&full_b[s]), 2 * C::STAGE);
                             // each CTA its 128 rows of the M operand and its half of the N operand
                             tma_load_2d_pair(st, &tmT, full, (int)(kb * 128), (int)(tc.row0 + rank * 128));
-                            tma_load_3d_pair(st + C::A_TILE, &tmW, full, (int)(kb * 128), (int)(tc.m0 + rank * 128), (int)(tc.group * g.group_step));
+                            tma_load_3d_pair(st + C::A_TILE, &tmW, full, (int)(kb * 128), (int)(tc.m0 + rank * (TN / CG)), (int)(tc.group * g.group_step));
                         } else {
                             const uint32_t full = smem_u32(&full_b[s]);
                             mbar_expect_tx(full, C::STAGE);
@@ -538,12 +551,12 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
             }
         } else {
             if constexpr (TOK) {
-                // Scale warps: K blocks are counted over all tiles of this CTA; warp 2 has the even ones and
-                // with them accumulator 0, warp 3 the odd ones and accumulator 1.  A block's barrier
+                // Scale warps: K blocks are counted over all tiles of this CTA; warp 2 has the even ones,
+                // warp 3 the odd ones.  A block's barrier
                 // completes with its MMAs and with its scales' arrival here, so the epilogue waits once.
-                // When block i - 2 is complete, its MMAs were issued, so every epilogue warp has given back
-                // the accumulator of block i - 4 and has read that block's scales: block i + 4 may take
-                // their place in the ring of eight.
+                // When block i - NBUF is complete, its MMAs were issued, so every epilogue warp has given
+                // back the accumulator of block i - 2 NBUF and has read that block's scales: block i + 4
+                // may take their place in the ring.
                 const uint32_t par = warp - 2;
                 uint32_t t = cid, kb = 0, wblocks = 0;       // the next block to load
                 TileF8 tc{};
@@ -564,34 +577,40 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                         fresh = false;
                     }
                     b2[0] = __ldg(sbp + kb);
-                    b2[1] = wblocks > 1 ? __ldg(sbp + g.b_lds + kb) : 0.0f;
+                    b2[1] = TN == 256 && wblocks > 1 ? __ldg(sbp + g.b_lds + kb) : 0.0f;
                     const float* a = g.as + (uint64_t)kb * g.a_lds + tc.row0;
 #pragma unroll
                     for (uint32_t q = 0; q < 4; ++q) a4[q] = tc.row0 + lane + 32 * q < tc.row1 ? __ldg(a + lane + 32 * q) : 0.0f;
                     step(2);
                 };
-                auto store = [&](uint64_t i, const float (&a4)[4], const float (&b2)[2]) {
-                    float* dst = ring + (uint32_t)(i % C::SLOTS) * TN;
+                uint32_t place = par;                        // in the ring, of the next block stored
+                auto store = [&](const float (&a4)[4], const float (&b2)[2]) {
+                    float* dst = ring + place * TN;
+                    place += 2;
+                    if (place >= C::SLOTS) place -= C::SLOTS;
 #pragma unroll
                     for (uint32_t q = 0; q < 4; ++q) {
                         dst[lane + 32 * q] = a4[q] * b2[0];
-                        dst[128 + lane + 32 * q] = a4[q] * b2[1];
+                        if (TN == 256) dst[128 + lane + 32 * q] = a4[q] * b2[1];
                     }
                 };
                 const uint64_t items = (uint64_t)(cid < total ? (total - cid + ncl - 1) / ncl : 0u) * g.kb;
-                const uint32_t accf = smem_u32(&accf_b[par]);
+                uint32_t buf = par, phase = 1;               // of block i - NBUF; there is none before the first
                 step(par);
                 load(sa[0], sb[0]);
                 load(sa[1], sb[1]);
-                if (par < items) store(par, sa[0], sb[0]);
+                if (par < items) store(sa[0], sb[0]);
                 load(sa[0], sb[0]);
-                if (par + 2 < items) store(par + 2, sa[1], sb[1]);
+                if (par + 2 < items) store(sa[1], sb[1]);
                 for (uint64_t i = par; i < items; i += 2) {
-                    if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(accf, (uint32_t)(i / 2 - 1) & 1u, wc))) break;
+                    const uint32_t accf = smem_u32(&accf_b[buf]);
+                    if (i >= C::NBUF && !__all_sync(0xffffffffu, mbar_wait(accf, phase, wc))) break;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(accf);
-                    if (i + 4 < items) store(i + 4, sa[0], sb[0]);
+                    if (i + 4 < items) store(sa[0], sb[0]);
                     load(sa[0], sb[0]);
+                    buf += 2;
+                    if (buf >= C::NBUF) { buf -= C::NBUF; phase ^= 1; }
                 }
             } else {
                 // Scale warps: of a tile's K blocks, in groups of four, 2 takes the even ones and 3 the odd
@@ -651,28 +670,26 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
             // A lane is a token row and the warp's 128 columns are one weight block, so a block's scale is
             // one number a thread.
             //
-            // 128 sums leave registers for half of a block's columns.  The second half is fetched as the
-            // first is added, the accumulator is given back when it is here, and the next block's first
-            // half is fetched while it is added.  Everything in shared memory answers
-            // slowly while the tensor cores read their operands there (a barrier test takes some 200
-            // cycles), so the next block's accumulator and scale are asked for at the top of this one.
+            // 128 sums leave registers for half of a block's columns: the second half is fetched as the
+            // first is added, and the accumulator is given back when it is here, before it is added.
+            // 64 sums take a block's columns at once.
             constexpr int CW = 32;
             const uint32_t quarter = warp & 3u, half = (warp - 4) / 4;
             const uint32_t acce0 = CG == 2 ? map_to_rank(smem_u32(&acce_b[0]), 0) : smem_u32(&acce_b[0]), accf0 = smem_u32(&accf_b[0]);
-            const uint32_t d0 = tmem + half * 128 + (quarter << 21);
-            const float* sc = ring + half * 128 + quarter * 32 + lane;
+            const uint32_t d0 = tmem + half * C::COLS + (quarter << 21);
+            const float* sc = ring + half * (TN / 256 * 128) + quarter * 32 + lane;
             uint32_t buf = 0, bphase = 0, slot = 0;
             bool ok = true;
             for (uint32_t t = cid; t < total; t += ncl) {
                 const TileF8 tc = decode_tile<C>(g, first, ends, t);
-                float acc[128];
+                float acc[C::COLS];
 #pragma unroll
-                for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+                for (int j = 0; j < C::COLS; ++j) acc[j] = 0.0f;
                 uint32_t r0[CW], r1[CW];
-                // Between a load and its wait there are only additions and barrier tests: nothing that makes
-                // the compiler move a register that the load still writes.
+                // Between a load and its wait there are only additions: nothing that makes the compiler move
+                // a register that the load still writes.
                 float one = 0.0f;
-                auto begin = [&]() {                 // the block's accumulator and scales are there: fetch its first half
+                auto begin = [&]() {                 // the block's accumulator and scales are there: fetch its first 64 columns
                     ok = __all_sync(0xffffffffu, mbar_wait(accf0 + 8 * buf, bphase, wc));
                     if (!ok) return;
                     tc_fence_after();
@@ -690,19 +707,21 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                     const uint32_t d = d0 + buf * TN, acce = acce0 + 8 * buf;
                     tmem_ld_done(r0);
                     tmem_ld_done(r1);
-                    add(0, r0);
-                    tmem_ld(d + 2 * CW, r0);
-                    add(1, r1);
-                    tmem_ld(d + 3 * CW, r1);
-                    tmem_ld_done(r0);
-                    tmem_ld_done(r1);
+                    if constexpr (TN == 256) {
+                        add(0, r0);
+                        tmem_ld(d + 2 * CW, r0);
+                        add(1, r1);
+                        tmem_ld(d + 3 * CW, r1);
+                        tmem_ld_done(r0);
+                        tmem_ld_done(r1);
+                    }
                     tc_fence_before();
                     __syncwarp();
                     arrive_cluster_if(lane == 0, acce);      // the accumulator's columns are in registers
-                    add(2, r0);
-                    add(3, r1);
-                    buf ^= 1u;
-                    bphase ^= buf ^ 1u;
+                    add(TN == 256 ? 2 : 0, r0);
+                    add(TN == 256 ? 3 : 1, r1);
+                    buf = (buf + 1u) % C::NBUF;
+                    if (buf == 0) bphase ^= 1u;
                     slot = (slot + 1u) % C::SLOTS;
                     if (left > 1) begin();
                     if (!ok) break;
@@ -711,15 +730,14 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                 uint8_t* stage = (uint8_t*)bars + 512 + C::TABLES + (warp - 4) * 2048;
                 const uint32_t row0 = tc.row0 + rank * 128 + quarter * 32, mcol = tc.m0 + half * C::COLS;
                 switch (g.c_type) {
-                    case CM_T_Q88: store_rows<int16_t>(g, row0, tc.row1, mcol, stage, lane, acc); break;
-                    case CM_T_F32: store_rows<float>(g, row0, tc.row1, mcol, stage, lane, acc); break;
-                    case CM_T_F16: store_rows<__half>(g, row0, tc.row1, mcol, stage, lane, acc); break;
-                    default: store_rows<__nv_bfloat16>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                    case CM_T_Q88: store_rows<int16_t, C::COLS>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                    case CM_T_F32: store_rows<float, C::COLS>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                    case CM_T_F16: store_rows<__half, C::COLS>(g, row0, tc.row1, mcol, stage, lane, acc); break;
+                    default: store_rows<__nv_bfloat16, C::COLS>(g, row0, tc.row1, mcol, stage, lane, acc); break;
                 }
             }
         } else {
-            const uint32_t quarter = warp & 3u, four = (warp - 4) / 4;
-            const uint32_t col0 = C::TURNS == 1 ? four * C::COLS : 0u, turn = C::TURNS == 1 ? 0u : four;
+            const uint32_t quarter = warp & 3u, turn = (warp - 4) / 4;
             const uint32_t nkb = kb1 - kb0;
             uint32_t item = 0, grp = 0;          // K blocks and groups of scales before this tile
             bool ok = true;
@@ -739,7 +757,7 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&accf_b[buf]), (it / C::NBUF) & 1u, wc));
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t d = tmem + buf * TN + col0 + (quarter << 21);
+                        const uint32_t d = tmem + buf * TN + (quarter << 21);
                         tmem_ld(d, r0);
                         if (NC > 1) tmem_ld(d + CW, r1);
                         tmem_ld_done(r0);
@@ -747,7 +765,7 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                         tc_fence_before();
                         __syncwarp();
                         arrive_if(lane == 0, smem_u32(&acce_b[buf]));
-                        const float* sc = ring + (gs * 4 + q) * TN + col0;      // a scale a column
+                        const float* sc = ring + (gs * 4 + q) * TN;      // a scale a column
 #pragma unroll
                         for (int j = 0; j < C::COLS; j += 4) {
                             const float4 s4 = *reinterpret_cast<const float4*>(sc + j);
@@ -761,32 +779,29 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                     __syncwarp();
                     arrive_if(lane == 0, smem_u32(&sempty_b[gs]));
                 }
-                if (C::TURNS == 2) {
-                    // each four finishes half of the columns, adding what the other one summed of them
-                    constexpr int H = C::COLS / 2;
-                    float* mine = (float*)((uint8_t*)bars + 512 + C::TABLES) + quarter * 32 + lane;
+                // each four finishes half of the columns, adding what the other one summed of them
+                constexpr int H = TN / 2;
+                float* mine = (float*)((uint8_t*)bars + 512 + C::TABLES) + quarter * 32 + lane;
 #pragma unroll
-                    for (int j = 0; j < H; ++j) mine[(turn * H + j) * 128] = turn ? acc[j] : acc[H + j];
-                    epilogue_sync<C::EPI_WARPS * 32>();
+                for (int j = 0; j < H; ++j) mine[(turn * H + j) * 128] = turn ? acc[j] : acc[H + j];
+                epilogue_sync<C::EPI_WARPS * 32>();
 #pragma unroll
-                    for (int j = 0; j < H; ++j) acc[j] = (turn ? acc[H + j] : acc[j]) + mine[((turn ^ 1u) * H + j) * 128];
-                    if (t + ncl < total) epilogue_sync<C::EPI_WARPS * 32>();      // read before the next tile writes
-                }
-                constexpr int OWN = C::COLS / C::TURNS;
-                const uint32_t own0 = C::TURNS == 1 ? col0 : turn * OWN;
+                for (int j = 0; j < H; ++j) acc[j] = (turn ? acc[H + j] : acc[j]) + mine[((turn ^ 1u) * H + j) * 128];
+                if (t + ncl < total) epilogue_sync<C::EPI_WARPS * 32>();      // read before the next tile writes
+                const uint32_t own0 = turn * H;
                 if (KS) {
                     // this CTA's part, [column][weight row], over the stages: their copies have landed and
                     // the MMAs that read them are complete (this tile is the CTA's only one)
                     float* part = (float*)smem + quarter * 32 + lane;
 #pragma unroll
-                    for (int j = 0; j < OWN; ++j) part[(own0 + j) * 128] = acc[j];
+                    for (int j = 0; j < H; ++j) part[(own0 + j) * 128] = acc[j];
                 } else if (ok) {
                     const uint32_t mrow = tc.m0 + quarter * 32 + lane;
                     switch (g.c_type) {
-                        case CM_T_Q88: store_cols<int16_t, OWN>(g, tc, own0, mrow, acc); break;
-                        case CM_T_F32: store_cols<float, OWN>(g, tc, own0, mrow, acc); break;
-                        case CM_T_F16: store_cols<__half, OWN>(g, tc, own0, mrow, acc); break;
-                        default: store_cols<__nv_bfloat16, OWN>(g, tc, own0, mrow, acc); break;
+                        case CM_T_Q88: store_cols<int16_t, H>(g, tc, own0, mrow, acc); break;
+                        case CM_T_F32: store_cols<float, H>(g, tc, own0, mrow, acc); break;
+                        case CM_T_F16: store_cols<__half, H>(g, tc, own0, mrow, acc); break;
+                        default: store_cols<__nv_bfloat16, H>(g, tc, own0, mrow, acc); break;
                     }
                 }
             }
@@ -987,10 +1002,11 @@ int run_tiles(const Context* cx, const uint8_t* a, uint64_t lda, const uint8_t* 
     if (!rc) rc = make_map(&tt, a, f.k, lda, f.n, 1, 0, C::TOKENS / CG, 2);
     if (rc) return rc;
     if constexpr (TN == 16) {
-        // Few tiles (wider ones are taken only where narrow ones fill the SMs): a cluster of CTAs to a tile, as many as are resident at once, where the blocks that
-        // a CTA is spared cost more than the cluster's launch, barriers and additions.  (Hundredths of a
+        // Few tiles (wider ones are taken only where narrow ones fill the SMs): a cluster of CTAs to a
+        // tile, as many as are resident at once, where the blocks that a CTA is spared cost more than
+        // the cluster's launch, barriers and additions.  (Hundredths of a
         // microsecond: one token, m = k = 4096, 32 blocks of 0.18 us: 9.7 us on one CTA a tile, 8.3 on
-        // two, 7.6 on four; m = k = 1024, 8 blocks: 4.3, 5.0 and 4.8.)
+        // two, 7.4 on four; m = k = 1024, 8 blocks: 4.3, 5.0 and 4.8.)
         constexpr uint32_t block = 18, extra = 180;
         uint32_t best = 1, least = g.kb * block;
         for (uint32_t size = 2; size <= 8 && size <= g.kb && most * size <= (uint64_t)cx->sm_count; size *= 2) {
@@ -1006,26 +1022,28 @@ int run_tiles(const Context* cx, const uint8_t* a, uint64_t lda, const uint8_t* 
     return launch_tiles<TN, CG, TOK, false>(cx, tw, tt, g, CG, most, s);
 }
 
-// The tile, by its token rows: 16 to 128 tokens x 128 weight rows on one SM, or 256 x 256 on two.  A
-// wider tile reads the weights less often and does more a block, but a block takes it longer and
-// there are fewer tiles to spread over the SMs.  The one is taken whose whole waves cost least:
-// waves x (K blocks x time of a block + time of a tile's output), in hundredths of a microsecond as
-// measured at k = 4096 and 1024 (16 to 256 tokens: 0.18, 0.20, 0.24, 0.42, 0.48 a block).  With m = k
-// = 4096, for instance, 128 tokens take 10.6 us in tiles of 32 and 17.6 in one of 128; 512 tokens
-// 18.5 in tiles of 128, 21.4 of 64 and 20.5 of 256; 1024 tokens 21.1 of 256 and 33.0 of 128.
-uint32_t pick_tokens(const Context* cx, const Fp8Args& f, uint32_t kb) {
+// The tile: 16 to 64 tokens x 128 weight rows on one SM, or 256 x 128 or 256 x 256 on two.  A wider
+// tile reads the operands less often and does more a block, but a block takes it longer and there are
+// fewer tiles to spread over the SMs.  The one is taken whose whole waves cost least: waves x (K
+// blocks x time of a block + time of a tile's output), in hundredths of a microsecond, fitted to 127
+// measured sizes from 1 x 512 x 512 to 8192 x 4096 x 11008 and groups of 1 to 512 rows; the choice is
+// within a tenth of the best of the five at each of them.  m = k = 4096, in tiles of 16, 32, 64, 256 x
+// 128 and 256 x 256: 100 tokens 16.6, 10.5, 11.9, 12.5 and 18.0 us; 200: 23.1, 17.7, 11.9, 12.9 and
+// 18.3; 512: 49.7, 32.3, 21.4, 13.6 and 18.3; 1000: 96, 54, 39.5, 22.5 and 19.7.
+uint32_t pick_tile(const Context* cx, const Fp8Args& f, uint32_t kb) {
     static const struct { uint32_t tokens, weights, sms, block, out; } kinds[] = {
-        {16, 128, 1, 18, 30}, {32, 128, 1, 20, 30}, {64, 128, 1, 24, 60}, {128, 128, 1, 42, 80}, {256, 256, 2, 48, 200}};
-    uint32_t best = 16;
+        {16, 128, 1, 19, 30}, {32, 128, 1, 22, 70}, {64, 128, 1, 25, 80}, {256, 128, 2, 30, 100}, {256, 256, 2, 47, 220}};
+    uint32_t best = 0;
     uint64_t least = ~0ull;
-    for (const auto& t : kinds) {
+    for (uint32_t kind = 0; kind < 5; ++kind) {
+        const auto& t = kinds[kind];
         // groups: their sizes are on the device; on average half a tile of each is not filled
         uint64_t token_tiles = (f.n + (uint64_t)t.tokens - 1) / t.tokens;
         if (f.offsets) token_tiles = std::min<uint64_t>(f.n, f.n / t.tokens + (f.groups + 1) / 2 + 1);
         const uint64_t tiles = token_tiles * ((f.m + (uint64_t)t.weights - 1) / t.weights);
         const uint64_t at_once = (uint64_t)cx->sm_count / t.sms;
         const uint64_t cost = (tiles + at_once - 1) / at_once * ((uint64_t)kb * t.block + t.out);
-        if (cost < least) { least = cost; best = t.tokens; }
+        if (cost < least) { least = cost; best = kind; }
     }
     return best;
 }
@@ -1066,11 +1084,11 @@ int fp8_launch(const char* who, const Context* cx, const Fp8Args& f, cudaStream_
     const uint8_t* a = a_bytes ? scratch : f.a;
     const uint8_t* b = b_bytes ? scratch + a_bytes : f.b;
     const uint64_t pa = a_bytes ? k16 : lda, pb = b_bytes ? k16 : ldb, gsb = one ? 0 : b_bytes ? f.m * k16 : f.b_gs;
-    switch (pick_tokens(cx, f, g.kb)) {
-        case 16: rc = run_tiles<16, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
-        case 32: rc = run_tiles<32, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
-        case 64: rc = run_tiles<64, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
-        case 128: rc = run_tiles<128, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
+    switch (pick_tile(cx, f, g.kb)) {
+        case 0: rc = run_tiles<16, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
+        case 1: rc = run_tiles<32, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
+        case 2: rc = run_tiles<64, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
+        case 3: rc = run_tiles<128, 2, true>(cx, a, pa, b, pb, gsb, f, g, s); break;
         default: rc = run_tiles<256, 2, true>(cx, a, pa, b, pb, gsb, f, g, s); break;
     }
     scratch_free(scratch, s);
