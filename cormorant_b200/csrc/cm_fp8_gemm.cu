@@ -15,12 +15,13 @@
 //                block's scale is one number a thread, and each SM stages half of the N operand.
 //                (128 x 128 tiles of one SM, which stage both operands whole and read a scale a
 //                column, took 19.8 us at 300 x 4096 x 4096, and 256 x 128 tiles of two 14.7.)
-// What bounds it: one token is the weights' HBM read and the launch (4096 x 4096: 7.4 us); ragged and
-// middle sizes are the pace at which one SM takes its operands from L2, some 100 KB a microsecond,
-// times the waves; 8192 x 4096 x 11008 (335 us, 2.2 PFLOP/s) is the exchange of the two accumulators
-// that TMEM holds between MMAs and additions: a block of 0.28 us of MMAs (measured alone) takes 0.38
-// to 0.42 us.  Accumulators handed over in halves (353 us) and blocks fetched into a second set of
-// registers while the one before is added (256 x 128 tiles: 396 -> 489 us) were slower.
+// What bounds it: one token is the weights' HBM read and the launch (4096 x 4096: 7.4 us).  Middle
+// sizes are whole waves of tiles whose blocks take 0.19 to 0.3 us against 0.12 to 0.15 us of MMAs
+// measured alone: accumulators change hands, and an SM takes its operands from L2 at up to 100 KB a
+// microsecond.  8192 x 4096 x 11008 (335 us, 2.2 PFLOP/s; 390 us in a long run, at the clocks of the
+// power limit) is the exchange of the two accumulators that TMEM holds: a block of 0.28 us of MMAs
+// takes 0.38 to 0.42 us.  Accumulators handed over in halves (353 us) and blocks fetched into a second
+// set of registers while the one before is added (in 256 x 128 tiles: 396 -> 489 us) were slower.
 //
 // Warps: 0 TMA producer, 1 MMA issuer (of the pair's leader), 2-3 token scales (global memory ->
 // times the weight scale -> a ring in shared memory), 4.. epilogue.  Every mbarrier wait is bounded
