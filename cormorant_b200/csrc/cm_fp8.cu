@@ -215,7 +215,7 @@ __device__ __forceinline__ void store_words(uint8_t* row, uint32_t col0, uint32_
             else bytes(p, x[0], 0, 4 - odd);
 #pragma unroll
             for (uint32_t j = 1; j < N; ++j) a[j] = __funnelshift_l(x[j - 1], x[j], 8 * odd);
-            if (odd && (at == kLanes * kChunks - 1 || c + 16 > cols)) bytes(p + 4 * (N - 1), x[N - 1], 4 - odd, 4);
+            if (odd && (at == kLanes * kChunks - 1 || cols - c < 16)) bytes(p + 4 * (N - 1), x[N - 1], 4 - odd, 4);
         } else if (n) {
 #pragma unroll
             for (uint32_t j = 0; j < N; ++j)
@@ -256,7 +256,7 @@ __device__ __forceinline__ void store32(T* row, uint32_t col0, uint32_t l, uint3
                     if (j < n) p[j] = x[3 + j];
                 continue;
             }
-            const bool end = !VEC && (at == kLanes * kChunks - 1 || c + 16 > cols);
+            const bool end = !VEC && (at == kLanes * kChunks - 1 || cols - c < 16);
 #pragma unroll
             for (uint32_t j = 0; j < 3; ++j)
                 if (end && 3 - j <= odd) p[5 + j] = x[8 + j];

@@ -270,6 +270,28 @@ def test_rows_at_every_offset(cm, t, cols):
             assert (b == 0xA5).all(), off
 
 
+@pytest.mark.parametrize("cols", [2 ** 32 - 1, 2 ** 32 - 8])
+def test_quant_longest_row(cm, cols):
+    """The columns of a 32-bit size's end, at odd addresses: offsets past 32 bits, no index that wraps."""
+    tail = 1000 + cols % 128
+    x = torch.zeros(cols, dtype=BF16, device="cuda")
+    x[-tail:] = values(5, tail).to(BF16).cuda()
+    x[:256] = values(6, 256).to(BF16).cuda()
+    b = torch.full((cols + 8,), 0xA5, dtype=torch.uint8, device="cuda")
+    s = torch.empty(up(cols), 1, device="cuda")
+    for off in (1, 2, 3):
+        q = b[off: off + cols]
+        cm.QuantKernelFp8(x, q, s, 1, cols, fmt=0)
+        first = (cols - tail) // 128 * 128
+        for lo, hi in ((0, 256), (first, cols)):
+            want_q, want_s = plain_quant(x[lo:hi].float().cpu()[None], E4, 1)
+            assert torch.equal(q[lo:hi].view(E4).float().cpu()[None], want_q), off
+            assert torch.equal(s[lo // 128: up(hi), 0].cpu(), want_s[0]), off
+        assert (b[:off] == 0xA5).all() and (b[off + cols:] == 0xA5).all()
+        b[-16:] = 0xA5
+        b[:16] = 0xA5
+
+
 @pytest.mark.parametrize("rows,cols", [(3000, 1), (5000, 120), (2500, 250), (1300, 640), (1200, 1500), (300, 9000)])
 def test_rmsnorm_more_rows_than_a_pass(cm, rows, cols):
     x, w = values(rows, rows, cols).to(BF16), (1 + 0.2 * values(cols, cols)).to(BF16)
