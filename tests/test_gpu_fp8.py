@@ -382,6 +382,26 @@ def test_matmul(cm, n, k, m, t, af, bf):
     assert torch.equal(c, c2)
 
 
+# 256 x 128 tiles on pairs of SMs: one tile a pair and several, 1 to 9 blocks of K through four
+# accumulators, an odd and an even number of weight blocks, every output type
+PAIRS = [(300, 1000, 4001, BF16, E5, E4), (513, 300, 2100, F16, E4, E4), (700, 520, 1990, Q88, E4, E5), (4043, 69, 1162, F32, E4, E4),
+         (3697, 143, 1717, BF16, E4, E4), (5000, 384, 900, F32, E4, E5), (3257, 543, 1987, F16, E5, E4), (4028, 836, 1040, F32, E4, E4)]
+
+
+@pytest.mark.parametrize("n,k,m,t,af,bf", PAIRS)
+def test_matmul_pairs(cm, n, k, m, t, af, bf):
+    test_matmul(cm, n, k, m, t, af, bf)
+
+
+PAIRS_GROUPED = [([700, 0, 1300, 2254], 3, 0, 190, 988, F32, E4, E4), ([1000, 1, 256, 1058], 0, 4, 307, 2234, BF16, E4, E5),
+                 ([500, 700, 0, 300, 3, 335], 0, 0, 1096, 1890, F16, E4, E4)]
+
+
+@pytest.mark.parametrize("sizes,before,behind,k,m,t,af,bf", PAIRS_GROUPED)
+def test_grouped_pairs(cm, sizes, before, behind, k, m, t, af, bf):
+    test_grouped(cm, sizes, before, behind, k, m, t, af, bf)
+
+
 @pytest.mark.parametrize("n,k,m,off_a,off_b,off_c", [(5, 256, 130, 1, 0, 1), (130, 300, 200, 0, 3, 1), (300, 512, 256, 8, 8, 3)])
 def test_matmul_unaligned_bases(cm, n, k, m, off_a, off_b, off_c):
     a, sa, b, sb = operands(n, n, k, m)
