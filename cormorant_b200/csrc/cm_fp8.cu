@@ -17,7 +17,7 @@
 // aligned 32-bit words put together from neighbouring lanes' (8192 x 1001 bf16, one element an access:
 // 26.9 us quantised and 55.7 us normed; this way 10.6 and 27).  What lies behind a row's end in its
 // last words is cleared where the values are used: done at the load, or by blocks that take another
-// path than whole ones, it cost 8192 x 2000 bf16 normed 31 us instead of 22..
+// path than whole ones, it cost 8192 x 2000 bf16 normed 31 us instead of 22.
 #include <algorithm>
 #include <cmath>
 
