@@ -81,7 +81,8 @@ struct Raw {
     // Clears what `load` took from behind the row's end in the last words.  Apart from it, so that
     // nothing waits for the values between their load and their use.
     __device__ __forceinline__ void trim(uint32_t col0, uint32_t l, uint32_t cols) {
-        if (col0 + kFp8Block <= cols || cols % 8 == 0) return;
+        // no sum that wraps: rows end within 128 columns of 2^32 too (a lane behind the row holds zeros already)
+        if (cols - col0 >= kFp8Block || cols % 8 == 0) return;
 #pragma unroll
         for (uint32_t i = 0; i < kChunks; ++i) {
             const uint32_t c = column(col0, l, 8 * i), n = c < cols ? min(8u, cols - c) : 0u;

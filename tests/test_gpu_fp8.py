@@ -292,6 +292,24 @@ def test_quant_longest_row(cm, cols):
         b[:16] = 0xA5
 
 
+@pytest.mark.parametrize("br", [1, 128])
+@pytest.mark.parametrize("cols", [2 ** 32 - 1, 2 ** 32 - 5, 2 ** 32 - 127])
+@pytest.mark.parametrize("behind", [float("nan"), 2.0 ** 100])
+def test_quant_longest_row_takes_nothing_from_behind_it(cm, cols, br, behind):
+    """The last block of a row that ends within 128 columns of 2^32: what follows the row in its last words stays out."""
+    tail = 1000 + cols % 128
+    b = torch.zeros(cols + 8, dtype=BF16, device="cuda")
+    x = b[:cols]
+    x[-tail:] = values(7, tail).to(BF16).cuda()
+    b[cols:] = behind
+    q, s = torch.empty(cols, dtype=E4, device="cuda"), torch.full((up(cols), 1) if br == 1 else (1, up(cols)), -7.0, device="cuda")
+    cm.QuantKernelFp8(x, q, s, 1, cols, block_rows=br)
+    first = (cols - tail) // 128 * 128
+    want_q, want_s = plain_quant(x[first:].float().cpu()[None], E4, br)
+    assert torch.equal(s.flatten()[first // 128:].cpu(), want_s.flatten())
+    assert torch.equal(q[first:].float().cpu()[None], want_q)
+
+
 @pytest.mark.parametrize("rows,cols", [(3000, 1), (5000, 120), (2500, 250), (1300, 640), (1200, 1500), (300, 9000)])
 def test_rmsnorm_more_rows_than_a_pass(cm, rows, cols):
     x, w = values(rows, rows, cols).to(BF16), (1 + 0.2 * values(cols, cols)).to(BF16)
