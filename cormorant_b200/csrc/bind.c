@@ -110,8 +110,9 @@ static int room_of(PyObject* t, int dtype, uint64_t* room) {
 
 /* The [batch][rows][cols] operand t: None, a raw address, or a CUDA tensor of the kind's types on
  * the library's device with contiguous rows.  A tensor of two or more dimensions has its own pitch
- * (and, of three, batch stride) unless they are given; a flat one and a raw address are dense unless
- * they are given.  A tensor has to be large enough. */
+ * unless the pitch is given, one of three or more its own batch stride unless the batch stride is
+ * given (the dimensions before the last two are one batch as far as their matrices lie an even stride
+ * apart); what is missing is dense.  A tensor has to be large enough. */
 static int matrix(PyObject* t, uint64_t rows, uint64_t cols, PyObject* ld, int kind, const char* what, uint64_t batch, PyObject* bs, Mat* m) {
     m->p = NULL; m->ld = m->bs = 0; m->code = ANY; m->given = t != Py_None;
     if (!m->given) return 0;
@@ -179,22 +180,29 @@ static int matrix(PyObject* t, uint64_t rows, uint64_t cols, PyObject* ld, int k
         }
         m->ld = item(stride, nd - 2);
         if (rows <= 1 && m->ld < cols) m->ld = cols;
-        if (batch <= 1 || (nd == 3 && !has_bs)) {
-            if (nd == 3) {
-                if (item(shape, 0) < batch) {
-                    PyErr_Format(PyExc_ValueError, "%s: %R holds fewer than %llu matrices", what, shape, (unsigned long long)batch);
-                    goto done;
-                }
-                if (!has_bs) m->bs = item(stride, 0);
-            } else if (!has_bs) {
-                m->bs = rows * m->ld;
-            }
-            rc = 0;
-            goto done;
-        }
     }
     if (!has_ld && nd < 2) m->ld = cols;
-    if (!has_bs) m->bs = rows * m->ld;
+    if (!has_bs) {
+        m->bs = rows * m->ld;
+        if (nd >= 3) {                       /* its own, whether or not the pitch is given */
+            uint64_t have = item(shape, nd - 3);
+            m->bs = item(stride, nd - 3);
+            for (Py_ssize_t i = nd - 4; i >= 0; --i) {
+                if (item(shape, i) == 1) continue;
+                if (have == 1) m->bs = item(stride, i);
+                else if (item(stride, i) != have * m->bs) break;
+                have *= item(shape, i);
+            }
+            if (have < batch) {
+                PyErr_Format(PyExc_ValueError, "%s: %R holds fewer than %llu matrices an even stride apart", what, shape, (unsigned long long)batch);
+                goto done;
+            }
+        }
+    }
+    if (nd >= 2 && !has_ld && (batch <= 1 || (nd >= 3 && !has_bs))) {        /* its shape has said that it is large enough */
+        rc = 0;
+        goto done;
+    }
     if (rows && cols && batch) {
         uint64_t room;
         if (nd == 1) room = item(shape, 0);

@@ -373,8 +373,8 @@ _native_module = None
 def _native():
     """The native side of the entries below (csrc/bind.c), given the C ABI's addresses.  An operand is
     None, a raw device address or a CUDA tensor: a tensor of two or more dimensions has its own row
-    pitch (and batch stride) unless they are given, a flat one and a raw address are dense unless they
-    are given; raw addresses need their type.  TypeError / ValueError for tensors of the wrong type or
+    pitch unless the pitch is given, one of three or more its own batch stride unless the batch stride
+    is given; what is missing is dense; raw addresses need their type.  TypeError / ValueError for tensors of the wrong type or
     device, too small, or with rows that are not contiguous."""
     global _native_module
     if _native_module is None:
