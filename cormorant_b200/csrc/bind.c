@@ -28,13 +28,12 @@ static struct {
 /* ---- element types --------------------------------------------------------------------------- */
 enum { D_I16, D_F32, D_F16, D_BF16, D_E4M3, D_E5M2, D_U8, D_I32, D_COUNT };
 static const char* const kDtypeNames[D_COUNT] = {"int16", "float32", "float16", "bfloat16", "float8_e4m3fn", "float8_e5m2", "uint8", "int32"};
-static const uint64_t kDtypeSize[D_COUNT] = {2, 4, 2, 2, 1, 1, 1, 4};
 static PyObject* dtypes[D_COUNT];
 
 enum { K_TYPE, K_FORMAT, K_SCALE, K_OFFSETS };   /* what an operand may hold */
 #define ANY (-1)                                   /* a raw address, or bytes of either format */
 
-static PyObject *s_data_ptr, *s_stride, *s_shape, *s_dtype, *s_get_device, *s_cuda_stream, *s_untyped_storage, *s_nbytes, *s_storage_offset;
+static PyObject *s_data_ptr, *s_stride, *s_shape, *s_dtype, *s_get_device, *s_cuda_stream;
 
 static int find_dtypes(void) {
     PyObject* torch = PyImport_ImportModule("torch");      /* a tensor is at hand: it is loaded */
@@ -96,23 +95,21 @@ typedef struct {
     int given;            /* not None */
 } Mat;
 
-/* Elements of t's storage from its first one on. */
-static int room_of(PyObject* t, int dtype, uint64_t* room) {
-    PyObject* st = PyObject_CallMethodNoArgs(t, s_untyped_storage);
-    if (!st) return -1;
-    uint64_t bytes = 0, off = 0;
-    int rc = call_u64(st, s_nbytes, &bytes);
-    Py_DECREF(st);
-    if (!rc) rc = call_u64(t, s_storage_offset, &off);
-    *room = bytes / kDtypeSize[dtype] - off;
-    return rc;
+/* Elements from t's first one to its last. */
+static uint64_t room_of(PyObject* shape, PyObject* stride) {
+    uint64_t last = 0;
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(shape); ++i) {
+        if (!item(shape, i)) return 0;
+        last += (item(shape, i) - 1) * item(stride, i);
+    }
+    return last + 1;
 }
 
 /* The [batch][rows][cols] operand t: None, a raw address, or a CUDA tensor of the kind's types on
  * the library's device with contiguous rows.  A tensor of two or more dimensions has its own pitch
  * unless the pitch is given, one of three or more its own batch stride unless the batch stride is
  * given (the dimensions before the last two are one batch as far as their matrices lie an even stride
- * apart); what is missing is dense.  A tensor has to be large enough. */
+ * apart); what is missing is dense.  Nothing beyond a tensor's own last element is reached. */
 static int matrix(PyObject* t, uint64_t rows, uint64_t cols, PyObject* ld, int kind, const char* what, uint64_t batch, PyObject* bs, Mat* m) {
     m->p = NULL; m->ld = m->bs = 0; m->code = ANY; m->given = t != Py_None;
     if (!m->given) return 0;
@@ -204,9 +201,7 @@ static int matrix(PyObject* t, uint64_t rows, uint64_t cols, PyObject* ld, int k
         goto done;
     }
     if (rows && cols && batch) {
-        uint64_t room;
-        if (nd == 1) room = item(shape, 0);
-        else if (room_of(t, dtype, &room)) goto done;
+        const uint64_t room = room_of(shape, stride);
         if ((unsigned __int128)(batch - 1) * m->bs + (unsigned __int128)(rows - 1) * m->ld + cols > room) {
             PyErr_Format(PyExc_ValueError, "%s: the buffer is too short for %llu x %llu x %llu at pitch %llu", what, (unsigned long long)batch,
                          (unsigned long long)rows, (unsigned long long)cols, (unsigned long long)m->ld);
@@ -374,9 +369,8 @@ static PyMethodDef methods[] = {
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", NULL, -1, methods, NULL, NULL, NULL, NULL};
 
 PyMODINIT_FUNC PyInit__bind(void) {
-    static PyObject** const names[] = {&s_data_ptr, &s_stride, &s_shape, &s_dtype, &s_get_device, &s_cuda_stream, &s_untyped_storage, &s_nbytes,
-                                       &s_storage_offset};
-    static const char* const text[] = {"data_ptr", "stride", "shape", "dtype", "get_device", "cuda_stream", "untyped_storage", "nbytes", "storage_offset"};
+    static PyObject** const names[] = {&s_data_ptr, &s_stride, &s_shape, &s_dtype, &s_get_device, &s_cuda_stream};
+    static const char* const text[] = {"data_ptr", "stride", "shape", "dtype", "get_device", "cuda_stream"};
     for (size_t i = 0; i < sizeof(names) / sizeof(*names); ++i)
         if (!(*names[i] = PyUnicode_InternFromString(text[i]))) return NULL;
     return PyModule_Create(&module);

@@ -122,3 +122,38 @@ def test_leading_dimensions_that_lie_evenly_are_one_batch(call):
 def test_too_few_matrices_are_refused(call, given):
     with pytest.raises(ValueError):
         call(cm.QuantKernelFp8, zeros(3, 8, 128)[:2, :4], bytes_(3, 4, 128), floats(3, 1, 4), 4, 128, 3, **given)
+
+
+# ---- a call stays inside the tensors that it is given ----------------------------------------------------
+def quant(x, q, s, rows, cols, batch=1, **given):
+    return cm.QuantKernelFp8, (x, q, s, rows, cols, batch), given
+
+
+BEYOND = {   # views whose storage goes on behind them
+    "batch of a matrix": quant(zeros(3 * 4, 128)[:4], bytes_(3, 4, 128), floats(3, 1, 4), 4, 128, 3),
+    "output batch of a matrix": quant(zeros(3, 4, 128), bytes_(3 * 4, 128)[:8], floats(3, 1, 4), 4, 128, 3),
+    "scales of a matrix": quant(zeros(3, 4, 128), bytes_(3, 4, 128), floats(3, 4)[:2], 4, 128, 3),
+    "rows at a given pitch": quant(zeros(8, 128)[:4], bytes_(8, 128), floats(1, 8), 8, 128, ldx=128),
+    "output rows at a given pitch": quant(zeros(8, 128), bytes_(8, 128)[:7], floats(1, 8), 8, 128, ldq=128),
+    "a wider pitch than its own": quant(zeros(8, 256)[:, :128], bytes_(8, 128), floats(1, 8), 8, 128, ldx=257),
+    "a given batch stride": quant(zeros(4, 4, 128)[:3], bytes_(3, 4, 128), floats(3, 1, 4), 4, 128, 3, x_batch_stride=600),
+    "weights of the groups": (cm.MatmulKernelFp8Grouped, (bytes_(5, 128), floats(1, 5), bytes_(4 * 64, 128)[:64], floats(4, 1, 1), zeros(5, 64),
+                                                         zeros(5, dtype=torch.int32), 4, 5, 128, 64), {}),
+    "a number": (cm.MatmulKernelFp8, (bytes_(2, 128), floats(2)[0], bytes_(1, 128), floats(1), zeros(2, 1), 2, 128, 1), {}),
+}
+
+
+@pytest.mark.parametrize("which", BEYOND)
+def test_nothing_beyond_a_tensor_is_reached(call, which):
+    entry, args, given = BEYOND[which]
+    with pytest.raises(ValueError):
+        call(entry, *args, **given)
+
+
+def test_all_of_a_tensor_may_be_reached(call):
+    wide = zeros(8, 256)[:, :128]
+    assert call(cm.QuantKernelFp8, wide, bytes_(8, 128), floats(1, 8), 8, 128, ldx=256).ldx == 256
+    assert call(cm.QuantKernelFp8, wide, bytes_(8, 128), floats(4, 2), 2, 128, 4).x_bs == 512
+    assert call(cm.QuantKernelFp8, zeros(4, 4, 128)[:3], bytes_(3, 4, 128), floats(3, 1, 4), 4, 128, 3, x_batch_stride=512).x_bs == 512
+    assert call(cm.MatmulKernelFp8, bytes_(1, 128), floats(2)[0], bytes_(1, 128), floats(1), zeros(1, 1), 1, 128, 1).n == 1
+    assert call(cm.QuantKernelFp8, zeros(0, 128), bytes_(0, 128), floats(1, 0), 0, 128).rows == 0
