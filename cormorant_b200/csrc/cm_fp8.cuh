@@ -4,8 +4,11 @@
 // A block of 128 values x (1 x 128 for activations, 128 x 128 for weights) is held as
 //   A = max(max|x|, 2^-100),  scale = A / F,  q = round(x * (F / A)) in e4m3 (F = 448) or e5m2
 //   (F = 57344), to nearest even; x ~ q * scale.
-// The floor of A keeps an all-zero block away from 0 / 0; 2^-100 leaves F / A and the products of
-// two such scales with any accumulated value exact enough that nothing above 2^-149 is lost.
+// The floor of A keeps an all-zero block away from 0 / 0; at 2^-100 F / A is finite in both formats.
+// The products round a_scale * b_scale to fp32 before it meets a block's sum: from 2^-126 on that is
+// one rounding like the others, below it a subnormal number, a multiple of 2^-149, and up to 2^-150
+// times the block's unscaled sum is lost (the sum is at most 128 F_a F_b: an error below 2^-125
+// for e4m3 by e4m3, 2^-118 for the mixed formats, 2^-111 for e5m2 by e5m2).
 #pragma once
 
 #include <cuda_bf16.h>

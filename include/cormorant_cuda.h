@@ -425,7 +425,10 @@ int cm_rmsnorm_fp8_async(const void* x, const void* resid, const void* weight, v
  *                                       * (sum of a[i][.] * b[j][.] over the block's columns),
  * i < n, j < m: a [n][k] activations, b [m][k] weights (k contiguous in both: a . b transposed),
  * each in its own format, c of c_type.  Sums are fp32 and are rounded once to c_type (CM_T_Q88:
- * floor to 1/256, saturating, NaN = 0).  The product of a block's two scales has to be finite.
+ * floor to 1/256, saturating, NaN = 0).  The product of a block's two scales has to be finite, and
+ * 2^-126 or more to be as exact as the rest: it is rounded to fp32 first, so that below 2^-126 a
+ * block may be off by 2^-150 times its unscaled sum (less than 2^-125 for e4m3 by e4m3, 2^-118 for
+ * mixed formats, 2^-111 for e5m2 by e5m2).
  * k = 0 gives zeros.  Results do not depend on the stream or on other calls in flight. */
 int cm_matmul_fp8(const uint8_t* a, const float* a_scale, const uint8_t* b, const float* b_scale, void* c, unsigned n,
                   unsigned k, unsigned m, uint64_t lda, uint64_t a_scale_ld, uint64_t ldb, uint64_t b_scale_ld,

@@ -462,6 +462,25 @@ def test_matmul_nan_and_infinity_stay_in_their_row_and_column(cm, n):
     assert (err <= (264 + 2 * up(k)) * U * mag + half(F32) * want.abs())[clean].all()
 
 
+@pytest.mark.parametrize("n", [3, 40, 300, 1300])
+@pytest.mark.parametrize("af,bf", [(E4, E4), (E5, E4), (E5, E5)])
+@pytest.mark.parametrize("exponent", [-125, -127, -140, -149, -170])
+def test_matmul_small_scales(cm, n, af, bf, exponent):
+    """Scales whose products are just normal, subnormal and zero in fp32.  A scale of 2^-126 or more is one rounding (u,
+    counted above), one below is off by 2^-150 at most, which the block's sum multiplies; results and their kb additions
+    are multiples of 2^-149, off by half of it each."""
+    k, m = 300, 1500 if n > 1000 else 130
+    a, sa, b, sb = operands(n + 1, n, k, m, af, bf)
+    sa, sb = (1 + 0.4 * torch.rand(sa.shape, generator=torch.Generator().manual_seed(1))) * 2.0 ** -64, \
+             (1 + 0.4 * torch.rand(sb.shape, generator=torch.Generator().manual_seed(2))) * 2.0 ** (exponent + 64)
+    want, mag = product64(a, sa, b, sb)
+    lost = a.double().abs() @ b.double().abs().t() * 2.0 ** -150 if exponent < -126 else 0
+    c = torch.empty(n, m, device="cuda")
+    cm.MatmulKernelFp8(a.cuda(), sa.cuda(), b.cuda(), sb.cuda(), c, n, k, m)
+    err = (c.double().cpu() - want).abs()
+    assert (err <= (264 + 2 * up(k)) * U * mag + half(F32) * want.abs() + lost + (up(k) + 9) * 2.0 ** -150).all()
+
+
 def test_matmul_pitch_past_32_bits(cm):
     """Rows of a and c that lie more than 2^32 bytes apart."""
     n, k, m = 3, 256, 136
