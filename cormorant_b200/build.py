@@ -1,4 +1,4 @@
-"""Build libcormorant_cuda.so (and its CPython binding _bind.so) in-tree for sm_100a (nvcc cross-compiles; no GPU needed).
+"""Build libcormorant_cuda.so (and its CPython binding _bind.*.so) in-tree for sm_100a (nvcc cross-compiles; no GPU needed).
 
     python -m cormorant_b200.build [--force] [--ptxas-info]
 """
@@ -6,6 +6,8 @@ from __future__ import annotations
 
 import argparse
 import os
+import shlex
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -16,7 +18,9 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libcormorant_cuda.so"
-BIND = PKG / "_bind.so"              # the CPython side of the 8-bit floating-point entries (csrc/bind.c)
+# The CPython side of the 8-bit floating-point entries (csrc/bind.c).  Its name carries the interpreter's
+# ABI tag: another Python neither finds it nor takes it for its own.
+BIND = PKG / ("_bind" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 INCLUDE = ROOT / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -36,6 +40,27 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def build_binding(force: bool = False, quiet: bool = True) -> Path | None:
+    """The CPython binding, or None (and a line on stderr) where Python's headers or a C compiler ($CC,
+    else gcc) are missing: the library and its C users need neither, the 8-bit Python entries then
+    raise ImportError."""
+    src, include, cc = CSRC / "bind.c", Path(sysconfig.get_paths()["include"]), shlex.split(os.environ.get("CC") or "gcc")
+    old = BIND.with_name("_bind.so")         # without a tag, which every Python would load
+    if old != BIND:
+        old.unlink(missing_ok=True)
+    for what, there in ((include / "Python.h", (include / "Python.h").exists()), (cc[0], shutil.which(cc[0]))):
+        if not there:
+            print(f"{BIND.name} is not built: no {what}", file=sys.stderr)
+            return None
+    if force or _stale(BIND, [src, INCLUDE / "cormorant_cuda.h", Path(__file__)]):
+        cmd = [*cc, "-O2", "-Wall", "-Wextra", "-Werror", "-std=gnu11", "-shared", "-fPIC", "-fvisibility=hidden",
+               "-I", str(include), "-I", str(INCLUDE), "-o", str(BIND), str(src)]
+        if not quiet:
+            print(" ".join(cmd), file=sys.stderr)
+        subprocess.run(cmd, check=True)
+    return BIND
+
+
 def build(force: bool = False, ptxas_info: bool = False, quiet: bool = True) -> Path:
     BUILD.mkdir(exist_ok=True)
     headers = sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
@@ -53,13 +78,7 @@ def build(force: bool = False, ptxas_info: bool = False, quiet: bool = True) -> 
     if force or _stale(LIB, objs):
         cmd = [_nvcc(), *ARCH, "-shared", "--cudart", "static", "-o", str(LIB), *map(str, objs), "-lrt", "-ldl", "-lpthread"]
         subprocess.run(cmd, check=True)
-    src = CSRC / "bind.c"
-    if force or _stale(BIND, [src, INCLUDE / "cormorant_cuda.h", Path(__file__)]):
-        cmd = ["gcc", "-O2", "-Wall", "-Wextra", "-Werror", "-std=gnu11", "-shared", "-fPIC", "-fvisibility=hidden",
-               "-I", sysconfig.get_paths()["include"], "-I", str(INCLUDE), "-o", str(BIND), str(src)]
-        if not quiet:
-            print(" ".join(cmd), file=sys.stderr)
-        subprocess.run(cmd, check=True)
+    build_binding(force, quiet)
     return LIB
 
 

@@ -380,7 +380,10 @@ def _native():
     if _native_module is None:
         import ctypes as C
 
-        from . import _bind                    # ImportError if it is not built: there is no other path
+        try:
+            from . import _bind
+        except ImportError as e:               # there is no other path
+            raise ImportError("cormorant_b200._bind is not built for this Python: python -m cormorant_b200.build") from e
         L = lib()
         names = ["cm_device"] + [n + t for n in ("cm_quant_fp8", "cm_rmsnorm_fp8", "cm_matmul_fp8", "cm_matmul_fp8_grouped")
                                  for t in ("", "_async")]
