@@ -660,6 +660,39 @@ def test_two_blocks_on_two_streams_and_captured(cm):
             b.check()
 
 
+@pytest.mark.parametrize("n,d,h,groups", [(5, 512, 264, 3), (90, 1000, 520, 6), (1100, 640, 384, 4)])
+def test_a_feed_forward_block_of_experts(cm, n, d, h, groups):
+    """norm + quantise, grouped product, activation (in Q8.8, by the framework's own kernel), quantise, grouped product, on
+    one stream; each step is checked from the inputs that it was given."""
+    e = lambda *s, t: torch.empty(*s, dtype=t, device="cuda")  # noqa: E731
+    x, r, w = values(n, n, d).to(BF16).cuda(), values(n + 1, n, d).to(BF16).cuda(), (1 + 0.1 * values(n + 2, d)).to(BF16).cuda()
+    gen = torch.Generator().manual_seed(n + 3)
+    up_w, down_w = (torch.randn(groups, h, d, generator=gen) * 0.05).cuda(), (torch.randn(groups, d, h, generator=gen) * 0.05).cuda()
+    u, us, v, vs = e(groups, h, d, t=E4), e(groups, up(h), up(d), t=F32), e(groups, d, h, t=E4), e(groups, up(d), up(h), t=F32)
+    cm.QuantKernelFp8(up_w, u, us, h, d, groups, block_rows=128)
+    cm.QuantKernelFp8(down_w, v, vs, d, h, groups, block_rows=128)
+    ends = [0, *sorted((torch.rand(groups - 1, generator=gen) * n).int().tolist()), n]
+    off = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    q, s, h1, out, r1 = e(n, d, t=E4), e(up(d), n, t=F32), e(n, h, t=Q88), e(n, d, t=BF16), e(n, d, t=BF16)
+    h2, hq, hs = e(n, h, t=Q88), e(n, h, t=E4), e(up(h), n, t=F32)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    cm.RmsNormKernelFp8(x, w, q, s, n, d, resid=r, resid_out=r1, stream=stream)
+    cm.MatmulKernelFp8Grouped(q, s, u, us, h1, off, groups, n, d, h, stream=stream)
+    cm.VectorOPKernel(h1, h1, h2, n * h, cm.OP_RELU, stream=stream)
+    cm.QuantKernelFp8(h2, hq, hs, n, h, stream=stream)
+    cm.MatmulKernelFp8Grouped(hq, hs, v, vs, out, off, groups, n, h, d, stream=stream)
+    stream.synchronize()
+    c = lambda t: t.cpu()  # noqa: E731
+    want, mag = grouped_want(c(q), c(s), c(u), c(us), ends, 0.0)
+    check_product(c(h1), want, mag, d, Q88)
+    assert torch.equal(h2, h1.clamp_min(0)) and (h2 > 0).any()
+    want_q, want_s = plain_quant(real(c(h2)).float(), E4, 1)
+    assert torch.equal(c(hq).float(), want_q) and torch.equal(c(hs), want_s.t())
+    want, mag = grouped_want(c(hq), c(hs), c(v), c(vs), ends, 0.0)
+    check_product(c(out), want, mag, h, BF16)
+
+
 def test_synchronous_entries_report(cm):
     """The entries without a stream return after the work, and refuse tensors that are too small."""
     a, sa, b, sb = (t.cuda() for t in operands(33, 5, 256, 130))
