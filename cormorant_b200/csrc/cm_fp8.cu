@@ -453,26 +453,47 @@ __global__ void __launch_bounds__(THREADS, 1) rmsnorm_kernel(const NormArgs g) {
             for (uint32_t p = 0; p < kVals / 2; ++p) h[p] = x.pair(p);
         }
         if (!BIG) fetch((uint64_t)row + step);
-        uint64_t s2[4] = {};
+        // sum over the row of a thread's v^2; `set`: the partial sums' place
+        auto squares = [&](auto v, uint32_t set) {
+            uint64_t s2[4] = {};
 #pragma unroll
-        for (uint32_t p = 0; p < kVals / 2; ++p) s2[p % 4] = fma2(h[p], h[p], s2[p % 4]);
-        float ss, other;
-        unpack2(add2(add2(s2[0], s2[1]), add2(s2[2], s2[3])), ss, other);
-        ss += other;
-        for (uint32_t o = min(g.per_row, 32u) / 2; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (whole) {
-            // two sets of partial sums in turn: one barrier a row is enough
-            if (threadIdx.x % 32 == 0) part[pass][threadIdx.x / 32] = ss;
-            __syncthreads();
-            ss = threadIdx.x % 32 < warps ? part[pass][threadIdx.x % 32] : 0.0f;
+            for (uint32_t p = 0; p < kVals / 2; ++p) s2[p % 4] = fma2(v(p), v(p), s2[p % 4]);
+            float ss, other;
+            unpack2(add2(add2(s2[0], s2[1]), add2(s2[2], s2[3])), ss, other);
+            ss += other;
+            for (uint32_t o = min(g.per_row, 32u) / 2; o; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (whole) {
+                // two sets of partial sums in turn: one barrier a row is enough
+                if (threadIdx.x % 32 == 0) part[set][threadIdx.x / 32] = ss;
+                __syncthreads();
+                ss = threadIdx.x % 32 < warps ? part[set][threadIdx.x % 32] : 0.0f;
 #pragma unroll
-            for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            }
+            return ss;
+        };
+        float ms = fmaf(squares([&](uint32_t p) { return h[p]; }, pass), inv_cols, g.eps), rms = 1.0f, after = 1.0f;
+        // Squares that leave fp32 (|h| from 2^64 / sqrt(cols) on, or mean and eps both below 2^-90, where squares
+        // lose bits): the row is summed again times 2^-100 or 2^100, which the output takes back, where it is 2^100 in two
+        // steps.  The branch is a warp's, and where a row has all warps of the CTA, the same for each of them.
+        constexpr uint32_t kInf = 0x7f800000u, kSmall = (127u - 90u) << 23;
+        const bool again = __any_sync(0xffffffffu, __float_as_uint(ms) - kSmall >= kInf - kSmall);
+        if (again) {
+            const bool large = isinf(ms), small = ms < __uint_as_float(kSmall);
+            const float by = large ? 7.888609052210118e-31f : small ? 1.2676506002282294e30f : 1.0f;      // 2^-100, 2^100
+            ms = fmaf(squares([&](uint32_t p) { return mul2(h[p], pack2(by, by)); }, pass ^ 1u), inv_cols, g.eps * by * by);
+            if (whole) __syncthreads();                                           // the next row's sums go to the same place
+            rms = small ? 1.180591620717411303424e21f : 1.0f;                        // 2^70
+            after = small ? 1073741824.0f : by;                                     // 2^30
         }
-        const float rms = 1.0f / sqrtf(fmaf(ss, inv_cols, g.eps));
-        const uint64_t rms2 = pack2(rms, rms);
+        rms /= sqrtf(ms);
         if (in && g.resid_out) store32<T, VEC>((T*)g.resid_out + (uint64_t)row * g.ldo, col0, l, g.cols, h);
+        auto by_factor = [&](float f) {
 #pragma unroll
-        for (uint32_t p = 0; p < kVals / 2; ++p) h[p] = mul2(h[p], rms2);
+            for (uint32_t p = 0; p < kVals / 2; ++p) h[p] = mul2(h[p], pack2(f, f));
+        };
+        by_factor(rms);
+        if (again) by_factor(after);
         auto times = [&](const auto& v) {
 #pragma unroll
             for (uint32_t p = 0; p < kVals / 2; ++p) h[p] = mul2(h[p], v.pair(p));

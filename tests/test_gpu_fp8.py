@@ -211,6 +211,31 @@ def test_rmsnorm(cm, rows, cols, t, wt, fmt, with_r, with_o, with_y, with_q, pit
                 assert (o.as_strided((rows - 1, ld - cols), (ld, 1), o.storage_offset() + cols) == v).all()
 
 
+# Squares that leave fp32: rows of one block, of a part of a warp, of several warps, and of the widest CTA, each with
+# ordinary rows beside the ones whose squares overflow or vanish.
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("rows,cols", [(9, 1), (70, 100), (41, 777), (13, 1024), (700, 2056), (5, 20000)])
+@pytest.mark.parametrize("eps", [0.0, 1e-5, 2.0 ** -130])
+def test_rmsnorm_large_and_small_rows(cm, t, rows, cols, eps):
+    x, w = values(rows, rows, cols), (1 + 0.2 * values(cols, cols)).to(t)
+    x[x == 0] = 1.0
+    exponents = torch.tensor([0, 62, -70, 100, -110, 123, -125, 64, -40])[torch.arange(rows) % 9]
+    x = (x.clamp(-8, 8).double() * (2.0 ** exponents.double())[:, None]).to(t)
+    r = torch.zeros_like(x)
+    ro, y = torch.empty(rows, cols, dtype=t, device="cuda"), torch.empty(rows, cols, dtype=t, device="cuda")
+    q, s = torch.empty(rows, cols, dtype=E4, device="cuda"), torch.empty(up(cols), rows, device="cuda")
+    cm.RmsNormKernelFp8(x.cuda(), w.cuda(), q, s, rows, cols, eps=eps, resid=r.cuda(), resid_out=ro, y=y)
+    assert torch.equal(ro.cpu(), x)
+    h = x.double()
+    want = h / torch.sqrt((h * h).mean(1, keepdim=True) + float(torch.tensor(eps))) * w.double()
+    # 24u and the output's rounding as above; results below 2^-126 (rows far below eps) are multiples of 2^-149, three roundings
+    err = (y.double().cpu() - want).abs()
+    assert (err <= (24 * U + half(t)) * want.abs() + (3 * 2.0 ** -150 if t == F32 else 2.0 ** -134 + 2 * 2.0 ** -150)).all()
+    sc = expand(s, rows, cols, 1)
+    err = (q.double().cpu() * sc - want).abs()
+    assert (err <= torch.maximum(HALF_STEP[E4] * want.abs(), HALF_SUBNORMAL[E4] * sc) + 32 * U * want.abs() + 4 * 2.0 ** -150).all()
+
+
 @pytest.mark.parametrize("rows,cols", [(5, 4096), (700, 1000)])
 def test_rmsnorm_in_place(cm, rows, cols):
     x, r, w = values(1, rows, cols).to(BF16).cuda(), values(2, rows, cols).to(BF16).cuda(), values(3, cols).to(BF16).cuda()
