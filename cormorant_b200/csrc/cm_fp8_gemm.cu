@@ -134,35 +134,82 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a, uint64_t b,
             : "memory");
 }
 
-// 16 or 32 accumulator columns of this warp's 32 lanes; they are there after tmem_ld_done, which
-// carries the registers, so that nothing that reads them can move above it.
+// 16, 32 or 2 x 32 accumulator columns of this warp's 32 lanes.  A load writes its registers until its
+// wait, so the two are one statement: nothing that the compiler makes of the code around it -- a copy, a
+// spill -- can come between them and read a register too early.
 #define CM_O(i) "=r"(r[i])
-#define CM_IO(i) "+r"(r[i])
+#define CM_O0(i) "=&r"(r0[i])
+#define CM_O1(i) "=r"(r1[i])
+#define CM_IO1(i) "+&r"(r1[i])
+#define CM_ACC(i) "+&f"(acc[i])
 #define CM_8(X, o) X(o), X(o + 1), X(o + 2), X(o + 3), X(o + 4), X(o + 5), X(o + 6), X(o + 7)
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
+#define CM_32(X) CM_8(X, 0), CM_8(X, 8), CM_8(X, 16), CM_8(X, 24)
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
         : CM_8(CM_O, 0), CM_8(CM_O, 8)
-        : "r"(taddr));
+        : "r"(taddr)
+        : "memory");
 }
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : CM_8(CM_O, 0), CM_8(CM_O, 8), CM_8(CM_O, 16), CM_8(CM_O, 24)
-        : "r"(taddr));
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : CM_32(CM_O)
+        : "r"(taddr)
+        : "memory");
 }
-__device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : CM_8(CM_IO, 0), CM_8(CM_IO, 8)::"memory");
+__device__ __forceinline__ void tmem_get(uint32_t taddr0, uint32_t taddr1, uint32_t (&r0)[32], uint32_t (&r1)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : CM_32(CM_O0), CM_32(CM_O1)
+        : "r"(taddr0), "r"(taddr1)
+        : "memory");
 }
-__device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : CM_8(CM_IO, 0), CM_8(CM_IO, 8), CM_8(CM_IO, 16), CM_8(CM_IO, 24)::"memory");
+// acc += r1 * one between the load of r0 and the load of the next r1
+__device__ __forceinline__ void tmem_get_adding(uint32_t taddr0, uint32_t taddr1, uint32_t (&r0)[32], uint32_t (&r1)[32], float* acc, float one) {
+#define CM_FMA(a, r) "fma.rn.f32 %" #a ", %" #r ", %98, %" #a ";\n\t"
+#define CM_FMA4(a, b, c, d, p, q, r, s) CM_FMA(a, p) CM_FMA(b, q) CM_FMA(c, r) CM_FMA(d, s)
+    asm volatile(
+        "{\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%96];\n\t"
+        CM_FMA4(64, 65, 66, 67, 32, 33, 34, 35)
+        CM_FMA4(68, 69, 70, 71, 36, 37, 38, 39)
+        CM_FMA4(72, 73, 74, 75, 40, 41, 42, 43)
+        CM_FMA4(76, 77, 78, 79, 44, 45, 46, 47)
+        CM_FMA4(80, 81, 82, 83, 48, 49, 50, 51)
+        CM_FMA4(84, 85, 86, 87, 52, 53, 54, 55)
+        CM_FMA4(88, 89, 90, 91, 56, 57, 58, 59)
+        CM_FMA4(92, 93, 94, 95, 60, 61, 62, 63)
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%97];\n\t"
+        "tcgen05.wait::ld.sync.aligned;\n\t}"
+        : CM_32(CM_O0), CM_32(CM_IO1), CM_32(CM_ACC)
+        : "r"(taddr0), "r"(taddr1), "f"(one)
+        : "memory");
+#undef CM_FMA
+#undef CM_FMA4
 }
 #undef CM_O
-#undef CM_IO
+#undef CM_O0
+#undef CM_O1
+#undef CM_IO1
+#undef CM_ACC
 #undef CM_8
+#undef CM_32
 
 // One thread of a converged warp.  The compiler knows that a branch on it holds one thread and keeps
 // the operands of the MMA and copy instructions in uniform registers; behind `lane == 0` it moves
@@ -687,16 +734,13 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
 #pragma unroll
                 for (int j = 0; j < C::COLS; ++j) acc[j] = 0.0f;
                 uint32_t r0[CW], r1[CW];
-                // Between a load and its wait there are only additions: nothing that makes the compiler move
-                // a register that the load still writes.
                 float one = 0.0f;
                 auto begin = [&]() {                 // the block's accumulator and scales are there: fetch its first 64 columns
                     ok = __all_sync(0xffffffffu, mbar_wait(accf0 + 8 * buf, bphase, wc));
                     if (!ok) return;
                     tc_fence_after();
                     one = sc[slot * TN];
-                    tmem_ld(d0 + buf * TN, r0);
-                    tmem_ld(d0 + buf * TN + CW, r1);
+                    tmem_get(d0 + buf * TN, d0 + buf * TN + CW, r0, r1);
                 };
                 begin();
                 if (!ok) break;
@@ -706,15 +750,9 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                 };
                 for (uint32_t left = g.kb; left; --left) {
                     const uint32_t d = d0 + buf * TN, acce = acce0 + 8 * buf;
-                    tmem_ld_done(r0);
-                    tmem_ld_done(r1);
                     if constexpr (TN == 256) {
                         add(0, r0);
-                        tmem_ld(d + 2 * CW, r0);
-                        add(1, r1);
-                        tmem_ld(d + 3 * CW, r1);
-                        tmem_ld_done(r0);
-                        tmem_ld_done(r1);
+                        tmem_get_adding(d + 2 * CW, d + 3 * CW, r0, r1, acc + CW, one);
                     }
                     tc_fence_before();
                     __syncwarp();
@@ -759,10 +797,8 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                         if (!ok) break;
                         tc_fence_after();
                         const uint32_t d = tmem + buf * TN + (quarter << 21);
-                        tmem_ld(d, r0);
-                        if (NC > 1) tmem_ld(d + CW, r1);
-                        tmem_ld_done(r0);
-                        if (NC > 1) tmem_ld_done(r1);
+                        if constexpr (NC > 1) tmem_get(d, d + CW, r0, r1);
+                        else tmem_get(d, r0);
                         tc_fence_before();
                         __syncwarp();
                         arrive_if(lane == 0, smem_u32(&acce_b[buf]));
