@@ -60,8 +60,10 @@ struct KArgs {
     uint64_t timeout_ns;
 };
 
-template <int TN, int CG, bool TOK>
+template <int TN>
 struct F8Cfg {
+    static constexpr bool TOK = TN >= 128;                    // token rows are the M operand; such tiles take a pair of SMs
+    static constexpr int CG = TOK ? 2 : 1;
     // Eight epilogue warps.  TOK: four for each half of the columns.  Else the K blocks go to the two
     // fours in turn, which add their sums at the end of a tile (a block costs a warp some 500 cycles of
     // waiting whatever its width).
@@ -86,7 +88,6 @@ struct F8Cfg {
     static constexpr int OUT = TOK ? EPI_WARPS * 2048 : TN * 128 * 4;
     static constexpr int SMEM = 1024 + STAGES * STAGE + SLOTS * TN * 4 + 512 + TABLES + OUT;
     static_assert(SMEM <= 232448 && 2 * SMEM > 232448, "one CTA an SM");
-    static_assert(TOK == (CG == 2) && TOK == (TN >= 128), "token rows are the M operand of the wide tiles, which take a pair of SMs");
     static_assert(TOK || TN * 512 <= STAGES * STAGE, "partial sums of a split tile fit the stages");
 };
 
@@ -409,10 +410,12 @@ struct ScaleRegs {
 
 // KS: the CTAs of a cluster share one tile, each a contiguous part of its K blocks, and add their
 // sums through distributed shared memory, in the order of their ranks.
-template <int TN, int CG, bool TOK, bool KS>
-__global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
+template <int TN, bool KS>
+__global__ void __launch_bounds__(F8Cfg<TN>::THREADS, 1)
     gemm_f8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT, const KArgs g) {
-    using C = F8Cfg<TN, CG, TOK>;
+    using C = F8Cfg<TN>;
+    constexpr bool TOK = C::TOK;
+    constexpr int CG = C::CG;
     static_assert(TN == 16 || !KS, "only the narrowest tiles split K");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -543,8 +546,8 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
                         } else {
                             const uint32_t full = smem_u32(&full_b[s]);
                             mbar_expect_tx(full, C::STAGE);
-                            tma_load_3d(st + (TOK ? C::A_TILE : 0), &tmW, full, (int)(kb * 128), (int)tc.m0, (int)(tc.group * g.group_step));
-                            tma_load_2d(st + (TOK ? 0 : C::A_TILE), &tmT, full, (int)(kb * 128), (int)tc.row0);
+                            tma_load_3d(st, &tmW, full, (int)(kb * 128), (int)tc.m0, (int)(tc.group * g.group_step));
+                            tma_load_2d(st + C::A_TILE, &tmT, full, (int)(kb * 128), (int)tc.row0);
                         }
                         if (++s == C::STAGES) { s = 0; phase ^= 1; }
                     }
@@ -723,7 +726,7 @@ __global__ void __launch_bounds__(F8Cfg<TN, CG, TOK>::THREADS, 1)
             // 64 sums take a block's columns at once.
             constexpr int CW = 32;
             const uint32_t quarter = warp & 3u, half = (warp - 4) / 4;
-            const uint32_t acce0 = CG == 2 ? map_to_rank(smem_u32(&acce_b[0]), 0) : smem_u32(&acce_b[0]), accf0 = smem_u32(&accf_b[0]);
+            const uint32_t acce0 = map_to_rank(smem_u32(&acce_b[0]), 0), accf0 = smem_u32(&accf_b[0]);
             const uint32_t d0 = tmem + half * C::COLS + (quarter << 21);
             const float* sc = ring + half * (TN / 256 * 128) + quarter * 32 + lane;
             uint32_t buf = 0, bphase = 0, slot = 0;
@@ -962,20 +965,20 @@ int make_map(CUtensorMap* map, const uint8_t* base, uint32_t k, uint64_t ld, uin
 }
 
 // Clusters of `size` CTAs of this kernel that the GPU holds at once.
-template <int TN, int CG, bool TOK, bool KS>
+template <int TN, bool KS>
 int resident_clusters(const Context* cx, uint32_t size, int* out) {
     static int known[16][9] = {};        // by device and size (function attributes are a device's own)
     const int dev = cx->device < 16 ? cx->device : 15;
     if (!known[dev][size] || dev == 15) {
-        const auto kern = gemm_f8_kernel<TN, CG, TOK, KS>;
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F8Cfg<TN, CG, TOK>::SMEM);
+        const auto kern = gemm_f8_kernel<TN, KS>;
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F8Cfg<TN>::SMEM);
         if (e != cudaSuccess) return cuda_error(e, "cudaFuncSetAttribute(gemm_f8)");
         int n = cx->sm_count / (int)size;
         if (size > 1) {
             cudaLaunchConfig_t q{};
             q.gridDim = dim3(size * n);
-            q.blockDim = dim3(F8Cfg<TN, CG, TOK>::THREADS);
-            q.dynamicSmemBytes = F8Cfg<TN, CG, TOK>::SMEM;
+            q.blockDim = dim3(F8Cfg<TN>::THREADS);
+            q.dynamicSmemBytes = F8Cfg<TN>::SMEM;
             cudaLaunchAttribute at{};
             at.id = cudaLaunchAttributeClusterDimension;
             at.val.clusterDim.x = size; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
@@ -990,16 +993,16 @@ int resident_clusters(const Context* cx, uint32_t size, int* out) {
     return CM_OK;
 }
 
-template <int TN, int CG, bool TOK, bool KS>
+template <int TN, bool KS>
 int launch_tiles(const Context* cx, const CUtensorMap& tw, const CUtensorMap& tt, const KArgs& g, uint32_t size, uint64_t most, cudaStream_t s) {
     int resident = 0;
-    int rc = resident_clusters<TN, CG, TOK, KS>(cx, size, &resident);
+    int rc = resident_clusters<TN, KS>(cx, size, &resident);
     if (rc) return rc;
     const unsigned clusters = (unsigned)std::min<uint64_t>(most, KS ? most : (uint64_t)resident);
     cudaLaunchConfig_t q{};
     q.gridDim = dim3(size * clusters);
-    q.blockDim = dim3(F8Cfg<TN, CG, TOK>::THREADS);
-    q.dynamicSmemBytes = F8Cfg<TN, CG, TOK>::SMEM;
+    q.blockDim = dim3(F8Cfg<TN>::THREADS);
+    q.dynamicSmemBytes = F8Cfg<TN>::SMEM;
     q.stream = s;
     cudaLaunchAttribute at[2]{};
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1010,16 +1013,18 @@ int launch_tiles(const Context* cx, const CUtensorMap& tw, const CUtensorMap& tt
     cudaError_t e;
     {
         ProfScope ps_(PK_FP8_GEMM, s);
-        e = cudaLaunchKernelEx(&q, gemm_f8_kernel<TN, CG, TOK, KS>, tw, tt, g);
+        e = cudaLaunchKernelEx(&q, gemm_f8_kernel<TN, KS>, tw, tt, g);
     }
     count_launch();
     return e == cudaSuccess ? CM_OK : cuda_error(e, "gemm_f8 launch");
 }
 
-template <int TN, int CG, bool TOK>
+template <int TN>
 int run_tiles(const Context* cx, const uint8_t* a, uint64_t lda, const uint8_t* b, uint64_t ldb, uint64_t b_gs, const Fp8Args& f, KArgs g,
               cudaStream_t s) {
-    using C = F8Cfg<TN, CG, TOK>;
+    using C = F8Cfg<TN>;
+    constexpr bool TOK = C::TOK;
+    constexpr int CG = C::CG;
     g.tiles_m = (f.m + C::WEIGHTS - 1) / C::WEIGHTS;
     g.tiles_t = (f.n + C::TOKENS - 1) / C::TOKENS;
     // a group's last tile may be partial, so grouped rows make at most n / TOKENS + groups tiles
@@ -1050,13 +1055,13 @@ int run_tiles(const Context* cx, const uint8_t* a, uint64_t lda, const uint8_t* 
             const uint32_t cost = (g.kb + size - 1) / size * block + extra;
             int resident = 0;
             if (cost >= least) continue;
-            rc = resident_clusters<TN, CG, TOK, true>(cx, size, &resident);
+            rc = resident_clusters<TN, true>(cx, size, &resident);
             if (rc) return rc;
             if (most <= (uint64_t)resident) { best = size; least = cost; }
         }
-        if (best > 1) return launch_tiles<TN, CG, TOK, true>(cx, tw, tt, g, best, most, s);
+        if (best > 1) return launch_tiles<TN, true>(cx, tw, tt, g, best, most, s);
     }
-    return launch_tiles<TN, CG, TOK, false>(cx, tw, tt, g, CG, most, s);
+    return launch_tiles<TN, false>(cx, tw, tt, g, CG, most, s);
 }
 
 // The tile: 16 to 64 tokens x 128 weight rows on one SM, or 256 x 128 or 256 x 256 on two.  A wider
@@ -1122,11 +1127,11 @@ int fp8_launch(const char* who, const Context* cx, const Fp8Args& f, cudaStream_
     const uint8_t* b = b_bytes ? scratch + a_bytes : f.b;
     const uint64_t pa = a_bytes ? k16 : lda, pb = b_bytes ? k16 : ldb, gsb = one ? 0 : b_bytes ? f.m * k16 : f.b_gs;
     switch (pick_tile(cx, f, g.kb)) {
-        case 0: rc = run_tiles<16, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
-        case 1: rc = run_tiles<32, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
-        case 2: rc = run_tiles<64, 1, false>(cx, a, pa, b, pb, gsb, f, g, s); break;
-        case 3: rc = run_tiles<128, 2, true>(cx, a, pa, b, pb, gsb, f, g, s); break;
-        default: rc = run_tiles<256, 2, true>(cx, a, pa, b, pb, gsb, f, g, s); break;
+        case 0: rc = run_tiles<16>(cx, a, pa, b, pb, gsb, f, g, s); break;
+        case 1: rc = run_tiles<32>(cx, a, pa, b, pb, gsb, f, g, s); break;
+        case 2: rc = run_tiles<64>(cx, a, pa, b, pb, gsb, f, g, s); break;
+        case 3: rc = run_tiles<128>(cx, a, pa, b, pb, gsb, f, g, s); break;
+        default: rc = run_tiles<256>(cx, a, pa, b, pb, gsb, f, g, s); break;
     }
     scratch_free(scratch, s);
     if (rc) return rc;
