@@ -37,10 +37,15 @@ int cuda_error(cudaError_t e, const char* what) {
 
 int enter(const Context** out) {
     if (!g_ready) return set_error(CM_ENOINIT, "cm_init has not been called");
+    // A thread that has not touched the device yet reports it as its current one (0 is the default) but has no
+    // context, which the runtime's calls make up for and the driver's do not (cuTensorMapEncodeTiled answers
+    // CUDA_ERROR_INVALID_CONTEXT): cudaSetDevice binds it.
+    static thread_local int t_bound = -1;
     int cur = -1;
-    if (cudaGetDevice(&cur) != cudaSuccess || cur != g_ctx.device) {
+    if (t_bound != g_ctx.device || cudaGetDevice(&cur) != cudaSuccess || cur != g_ctx.device) {
         cudaError_t e = cudaSetDevice(g_ctx.device);
         if (e != cudaSuccess) return cuda_error(e, "cudaSetDevice");
+        t_bound = g_ctx.device;
     }
     *out = &g_ctx;
     return CM_OK;

@@ -737,3 +737,24 @@ def test_synchronous_entries_report(cm):
         cm.MatmulKernelFp8(a, sa, b, sb, c, 5, 256, 130, a_fmt=cm.F8_E5M2)
     with pytest.raises(cm.CormorantError):
         cm.QuantKernelFp8(c, a, sa, 5, 130, block_rows=64)
+
+
+@pytest.mark.parametrize("n,k,m", [(1, 4096, 256), (300, 512, 256)])
+def test_first_call_of_a_new_thread(cm, n, k, m):
+    """A thread that has not used the GPU yet may begin with a product."""
+    import threading
+    a, sa, b, sb = (t.cuda() for t in operands(n, n, k, m))
+    want, c, failed = torch.empty(n, m, device="cuda"), torch.empty(n, m, device="cuda"), []
+    cm.MatmulKernelFp8(a, sa, b, sb, want, n, k, m)
+
+    def first():
+        try:
+            cm.MatmulKernelFp8(a, sa, b, sb, c, n, k, m)
+        except BaseException as e:
+            failed.append(e)
+
+    t = threading.Thread(target=first)
+    t.start()
+    t.join()
+    assert not failed, failed
+    assert torch.equal(c, want)
