@@ -38,7 +38,7 @@ static PyObject *s_data_ptr, *s_stride, *s_shape, *s_dtype, *s_get_device, *s_cu
 static int find_dtypes(void) {
     PyObject* torch = PyImport_ImportModule("torch");      /* a tensor is at hand: it is loaded */
     if (!torch) return -1;
-    for (int i = 0; i < D_COUNT; ++i) {
+    for (int i = D_COUNT - 1; i >= 0; --i) {               /* the first one, which says that all are there, last */
         dtypes[i] = PyObject_GetAttrString(torch, kDtypeNames[i]);
         if (!dtypes[i]) { Py_DECREF(torch); return -1; }
     }

@@ -27,6 +27,7 @@
 // times the weight scale -> a ring in shared memory), 4.. epilogue.  Every mbarrier wait is bounded
 // by %globaltimer, as in cm_gemm.cu.
 #include <algorithm>
+#include <atomic>
 
 #include "cm_fp8.cuh"
 #include "cm_tcgen05.cuh"
@@ -967,13 +968,14 @@ int make_map(CUtensorMap* map, const uint8_t* base, uint32_t k, uint64_t ld, uin
 // Clusters of `size` CTAs of this kernel that the GPU holds at once.
 template <int TN, bool KS>
 int resident_clusters(const Context* cx, uint32_t size, int* out) {
-    static int known[16][9] = {};        // by device and size (function attributes are a device's own)
+    static std::atomic<int> known[16][9] = {};      // by device and size (function attributes are a device's own); first calls may come from several threads
     const int dev = cx->device < 16 ? cx->device : 15;
-    if (!known[dev][size] || dev == 15) {
+    int n = dev == 15 ? 0 : known[dev][size].load();
+    if (!n) {
         const auto kern = gemm_f8_kernel<TN, KS>;
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F8Cfg<TN>::SMEM);
         if (e != cudaSuccess) return cuda_error(e, "cudaFuncSetAttribute(gemm_f8)");
-        int n = cx->sm_count / (int)size;
+        n = cx->sm_count / (int)size;
         if (size > 1) {
             cudaLaunchConfig_t q{};
             q.gridDim = dim3(size * n);
@@ -987,9 +989,9 @@ int resident_clusters(const Context* cx, uint32_t size, int* out) {
             if (cudaOccupancyMaxActiveClusters(&r, kern, &q) == cudaSuccess && r > 0) n = std::min(n, r);
             cudaGetLastError();
         }
-        known[dev][size] = n;
+        known[dev][size].store(n);
     }
-    *out = known[dev][size];
+    *out = n;
     return CM_OK;
 }
 

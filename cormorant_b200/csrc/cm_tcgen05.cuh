@@ -5,6 +5,8 @@
 
 #include <cuda.h>
 
+#include <atomic>
+
 #include "cm_async.cuh"
 
 namespace cm {
@@ -60,13 +62,14 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 inline EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
+    static std::atomic<EncodeTiledFn> known{nullptr};        // first calls may come from several threads
+    EncodeTiledFn fn = known.load();
     if (!fn) {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
             q == cudaDriverEntryPointSuccess)
-            fn = (EncodeTiledFn)p;
+            known.store(fn = (EncodeTiledFn)p);
     }
     return fn;
 }

@@ -758,3 +758,45 @@ def test_first_call_of_a_new_thread(cm, n, k, m):
     t.join()
     assert not failed, failed
     assert torch.equal(c, want)
+
+
+FIRST_CALLS = """
+import sys, threading
+import torch
+import cormorant_b200 as cm
+sys.path.insert(0, "tests")
+import test_gpu_fp8 as T
+cm.init("0")
+sizes = [(1, 4096, 256), (70, 512, 4096), (300, 1000, 1001), (1100, 512, 1300), (3000, 256, 2304)]
+data = [[v.cuda() for v in T.operands(n, n, k, m)] for n, k, m in sizes]
+out = [[torch.empty(n, m, device="cuda") for n, k, m in sizes] for _ in range(4)]
+torch.cuda.synchronize()
+ready, failed = threading.Barrier(4), []
+def calls(i):
+    stream = torch.cuda.Stream()
+    ready.wait()
+    try:
+        for j in range(len(sizes)):
+            j = (i + j) % len(sizes)
+            cm.MatmulKernelFp8(*data[j], out[i][j], *sizes[j], stream=stream)
+        stream.synchronize()
+    except BaseException as e:
+        failed.append(e)
+threads = [threading.Thread(target=calls, args=(i,)) for i in range(4)]
+for t in threads: t.start()
+for t in threads: t.join()
+assert not failed, failed
+assert all(torch.equal(a, b) for o in out[1:] for a, b in zip(o, out[0]))
+for d, (n, k, m), c in zip(data, sizes, out[0]):
+    T.check_product(c.cpu(), *T.product64(*(v.cpu() for v in d)), k, T.F32)
+print("done")
+"""
+
+
+def test_first_calls_from_several_threads():
+    """A process whose first calls of every tile come from four threads at once."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "done", r.stderr[-2000:]
