@@ -800,3 +800,146 @@ def test_first_calls_from_several_threads():
     from pathlib import Path
     r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip() == "done", r.stderr[-2000:]
+
+
+# ---- every tile ------------------------------------------------------------------------------------------
+# The product's tile is chosen by size; which one a size takes is worked out here from the table in its source, so that
+# a change of the rule shows as a test that no longer reaches the tile it names.
+TILES = ["16", "32", "64", "256x128", "256x256"]
+
+
+def tile_of(n, k, m, groups=0):
+    import re
+    from pathlib import Path
+    source = (Path(__file__).resolve().parent.parent / "cormorant_b200" / "csrc" / "cm_fp8_gemm.cu").read_text()
+    table = re.search(r"kinds\[\] = \{\s*(.*?)\};", source, re.S).group(1)
+    kinds = [tuple(map(int, t.split(","))) for t in re.findall(r"\{([\d, ]+)\}", table)]
+    assert len(kinds) == len(TILES)
+    sms, costs = torch.cuda.get_device_properties(0).multi_processor_count, []
+    for tokens, weights, ctas, block, out in kinds:
+        rows = min(n, n // tokens + (groups + 1) // 2 + 1) if groups else -(-n // tokens)
+        tiles, at_once = rows * -(-m // weights), sms // ctas
+        costs.append(-(-tiles // at_once) * (up(k) * block + out))
+    return TILES[costs.index(min(costs))]
+
+
+@pytest.mark.parametrize("tile,n,k,m", [("16", 40, 640, 300), ("32", 90, 512, 4096), ("64", 200, 1000, 4096), ("256x128", 520, 300, 2050),
+                                        ("256x256", 600, 512, 4224)])
+def test_matmul_nan_and_infinity_stay_where_they_are(cm, tile, n, k, m):
+    assert tile_of(n, k, m) == tile
+    a, sa, b, sb = operands(9, n, k, m)
+    want, mag = product64(a, sa, b, sb)
+    ai, bi, sa = a.view(torch.uint8).clone(), b.view(torch.uint8).clone(), sa.clone()
+    bad_rows, bad_cols = [1, n // 2, n - 1], [0, m // 2 + 1, m - 1]
+    ai[1, 130], sa[1, n // 2], sa[up(k) - 1, n - 1] = 0x7F, float("nan"), float("inf")
+    bi[bad_cols, k - 1] = 0xFF
+    c = torch.empty(n, m, device="cuda")
+    cm.MatmulKernelFp8(ai.view(E4).cuda(), sa.cuda(), bi.view(E4).cuda(), sb.cuda(), c, n, k, m)
+    got = c.cpu()
+    rows, cols = torch.ones(n, dtype=torch.bool), torch.ones(m, dtype=torch.bool)
+    rows[bad_rows], cols[bad_cols] = False, False
+    assert not torch.isfinite(got[~rows]).any() and torch.isnan(got[:, ~cols]).all()
+    err = (got.double() - want).abs()
+    assert (err <= (264 + 2 * up(k)) * U * mag + half(F32) * want.abs())[rows][:, cols].all()
+
+
+# A group's last tile reads the rows behind it, which are another group's or no group's: NaN there stays there.
+@pytest.mark.parametrize("tile,sizes,k,m", [("16", [11, 0, 29, 10], 300, 300), ("32", [50, 0, 50], 300, 3000), ("64", [70, 1, 100, 0, 129], 300, 2000),
+                                            ("256x128", [700, 0, 800], 300, 2600), ("256x256", [300, 257, 0, 543], 300, 2040)])
+def test_grouped_nan_stays_in_its_rows(cm, tile, sizes, k, m):
+    ends = [3]
+    for v in sizes:
+        ends.append(ends[-1] + v)
+    n = ends[-1] + 5
+    assert tile_of(n, k, m, len(sizes)) == tile
+    a, sa, b, sb = operands(k + m, n, k, m, groups=len(sizes))
+    want, mag = grouped_want(a, sa, b, sb, ends, 0.0)
+    bad = torch.zeros(n, dtype=torch.bool)
+    bad[: ends[0]] = bad[ends[-1]:] = True                                # no group's rows
+    for i in ends[1:-1]:
+        bad[i] = True                                                      # the first row of each group but one
+    ai, sa = a.view(torch.uint8).clone(), sa.clone()
+    ai[bad], sa[:, bad] = 0x7F, float("nan")
+    c = torch.full((n, m), -3.0, device="cuda")
+    cm.MatmulKernelFp8Grouped(ai.view(E4).cuda(), sa.cuda(), b.cuda(), sb.cuda(), c, torch.tensor(ends, dtype=torch.int32, device="cuda"), len(sizes), n, k, m)
+    got = c.cpu()
+    assert (got[: ends[0]] == -3).all() and (got[ends[-1]:] == -3).all()
+    inside = torch.zeros(n, dtype=torch.bool)
+    inside[ends[0]: ends[-1]] = True
+    assert torch.isnan(got[inside & bad]).all()
+    err = (got.double() - want).abs()
+    assert (err <= (264 + 2 * up(k)) * U * mag + half(F32) * want.abs())[inside & ~bad].all()
+
+
+# Rows of c that start on 16-byte boundaries leave the wide tiles in whole 16-byte pieces.
+@pytest.mark.parametrize("t", [F32, F16, BF16, Q88])
+@pytest.mark.parametrize("tile,n,k,m", [("256x256", 600, 512, 4232), ("256x256", 1300, 300, 2632), ("256x128", 520, 300, 2056), ("256x128", 1100, 512, 1304)])
+def test_matmul_aligned_output_rows(cm, tile, n, k, m, t):
+    assert tile_of(n, k, m) == tile and m * t.itemsize % 16 == 0
+    a, sa, b, sb = operands(n + m, n, k, m, E5 if t == F16 else E4, E4)
+    want, mag = product64(a, sa, b, sb)
+    c = torch.full((n + 2, m), -3, dtype=t, device="cuda")
+    cm.MatmulKernelFp8(a.cuda(), sa.cuda(), b.cuda(), sb.cuda(), c[1:], n, k, m)
+    check_product(c[1: n + 1].cpu(), want, mag, k, t)
+    assert (c[0] == -3).all() and (c[n + 1] == -3).all()
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16, Q88])
+@pytest.mark.parametrize("tile,sizes,k,m", [("256x256", [300, 257, 0, 543], 300, 2040), ("256x256", [1, 1500, 999], 300, 2600), ("256x128", [700, 0, 800], 300, 2600)])
+def test_grouped_aligned_output_rows(cm, tile, sizes, k, m, t):
+    ends = [0]
+    for v in sizes:
+        ends.append(ends[-1] + v)
+    n = ends[-1]
+    assert tile_of(n, k, m, len(sizes)) == tile and m * t.itemsize % 16 == 0
+    a, sa, b, sb = operands(k + m, n, k, m, groups=len(sizes))
+    want, mag = grouped_want(a, sa, b, sb, ends, 0.0)
+    c = torch.full((n + 1, m), -3, dtype=t, device="cuda")
+    cm.MatmulKernelFp8Grouped(a.cuda(), sa.cuda(), b.cuda(), sb.cuda(), c, torch.tensor(ends, dtype=torch.int32, device="cuda"), len(sizes), n, k, m)
+    check_product(c[:n].cpu(), want, mag, k, t)
+    assert (c[n] == -3).all()
+
+
+@pytest.mark.parametrize("pair", [("16", "256x256"), ("256x128", "64"), ("256x256", "256x128"), ("32", "16")])
+def test_every_tile_captured_on_two_streams(cm, pair):
+    """Two graphs of a dense and a grouped product each, replayed side by side with changed inputs."""
+    sizes = {"16": (40, 640, 300), "32": (90, 512, 4096), "64": (200, 1000, 4096), "256x128": (520, 300, 2050), "256x256": (600, 512, 4224)}
+    grouped = {"16": ([11, 0, 29, 10], 300, 300), "32": ([50, 0, 50], 300, 3000), "64": ([70, 1, 100, 0, 129], 300, 2000),
+               "256x128": ([700, 0, 800], 300, 2600), "256x256": ([300, 257, 0, 543], 300, 2040)}
+    work = []
+    for tile in pair:
+        n, k, m = sizes[tile]
+        gs, gk, gm = grouped[tile]
+        ends = np.cumsum([0, *gs]).tolist()
+        assert tile_of(n, k, m) == tile and tile_of(ends[-1], gk, gm, len(gs)) == tile
+        dev = lambda ops: [v.cuda() for v in ops]  # noqa: E731
+        d, g = dev(operands(n, n, k, m)), dev(operands(gm, ends[-1], gk, gm, groups=len(gs)))
+        off = torch.tensor(ends, dtype=torch.int32, device="cuda")
+        c, gc, s = torch.empty(n, m, dtype=BF16, device="cuda"), torch.empty(ends[-1], gm, device="cuda"), torch.cuda.Stream()
+
+        def run(d=d, g=g, c=c, gc=gc, off=off, s=s, n=n, k=k, m=m, gs=gs, gk=gk, gm=gm, ends=ends):
+            cm.MatmulKernelFp8(*d, c, n, k, m, stream=s)
+            cm.MatmulKernelFp8Grouped(*g, gc, off, len(gs), ends[-1], gk, gm, stream=s)
+
+        torch.cuda.synchronize()
+        run()
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            run()
+        work.append((graph, s, d, g, c, gc, k, gk, ends))
+    for change in range(2):
+        for _, _, d, g, c, gc, *_ in work:
+            d[1].mul_(1 + change)
+            g[3].mul_(1 + change)
+            c.fill_(float("nan"))
+            gc.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for graph, s, *_ in work:
+                with torch.cuda.stream(s):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for _, _, d, g, c, gc, k, gk, ends in work:
+            check_product(c.cpu(), *product64(*(v.cpu() for v in d)), k, BF16)
+            check_product(gc.cpu(), *grouped_want(*(v.cpu() for v in g), ends, 0.0), gk, F32)
