@@ -943,3 +943,34 @@ def test_every_tile_captured_on_two_streams(cm, pair):
         for _, _, d, g, c, gc, k, gk, ends in work:
             check_product(c.cpu(), *product64(*(v.cpu() for v in d)), k, BF16)
             check_product(gc.cpu(), *grouped_want(*(v.cpu() for v in g), ends, 0.0), gk, F32)
+
+
+@pytest.mark.parametrize("n,k,m,groups", [(5, 256, 130, 4), (300, 512, 260, 3), (1100, 300, 2040, 4)])
+@pytest.mark.parametrize("layout", ["rows side by side", "odd gap", "16-byte gap"])
+def test_grouped_weights_at_any_group_stride(cm, n, k, m, groups, layout):
+    """Groups whose rows lie between each other's, and groups that lie no whole number of rows apart."""
+    a, sa, b, sb = operands(n, n, k, m, groups=groups)
+    ends = [n * i // groups for i in range(groups + 1)]
+    want, mag = grouped_want(a, sa, b, sb, ends, 0.0)
+    k16 = (k + 15) // 16 * 16
+    ld, gs = (groups * k16, k16) if layout == "rows side by side" else (k16, m * k16 + (16 if layout == "16-byte gap" else 7))
+    buf = torch.full(((groups - 1) * gs + (m - 1) * ld + k16,), 0x7F, dtype=torch.uint8, device="cuda")
+    view = buf.as_strided((groups, m, k), (gs, ld, 1))
+    view.copy_(b.view(torch.uint8))
+    c = torch.full((n, m), -3.0, device="cuda")
+    cm.MatmulKernelFp8Grouped(a.cuda(), sa.cuda(), view.view(E4), sb.cuda(), c, torch.tensor(ends, dtype=torch.int32, device="cuda"), groups, n, k, m)
+    check_product(c.cpu(), want, mag, k, F32)
+
+
+@pytest.mark.parametrize("n,k,m", [(3, 128, 130), (600, 512, 4224)])
+def test_matmul_q88_of_nan_and_infinity(cm, n, k, m):
+    a, sa, b, sb = operands(n, n, k, m)
+    want, mag = product64(a, sa, b, sb)
+    sa = sa.clone()
+    sa[0, 0], sa[0, 1] = float("nan"), float("inf")
+    c = torch.full((n, m), 77, dtype=Q88, device="cuda")
+    cm.MatmulKernelFp8(a.cuda(), sa.cuda(), b.cuda(), sb.cuda(), c, n, k, m)
+    got, first = c.cpu(), (a[1, :128].double() @ b[:, :128].double().t())
+    assert (got[0] == 0).all()
+    assert torch.equal(got[1], torch.where(first > 0, 32767, torch.where(first < 0, -32768, 0)).to(Q88))
+    check_product(got[2:], want[2:], mag[2:], k, Q88)
