@@ -31,6 +31,7 @@ int set_error(int code, const char* fmt, ...) {
 }
 
 int cuda_error(cudaError_t e, const char* what) {
+    cudaGetLastError();          // it is reported here, and not once more by the next call's launch check
     return set_error(e == cudaErrorMemoryAllocation ? CM_ENOMEM : CM_ECUDA, "%s: %s", what,
                      cudaGetErrorString(e));
 }

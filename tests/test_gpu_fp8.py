@@ -974,3 +974,23 @@ def test_matmul_q88_of_nan_and_infinity(cm, n, k, m):
     assert (got[0] == 0).all()
     assert torch.equal(got[1], torch.where(first > 0, 32767, torch.where(first < 0, -32768, 0)).to(Q88))
     check_product(got[2:], want[2:], mag[2:], k, Q88)
+
+
+def test_a_refused_allocation_is_not_the_next_calls_error(cm):
+    """A product whose aligned copies would take 1 TB is answered with CM_ENOMEM, and the next call is judged by itself."""
+    n, k, m, groups = 1, 1000, 1 << 20, 1024
+    a, sa, b, sb = (t.cuda() for t in operands(3, 40, 256, 130))
+    want, c = torch.empty(40, 130, device="cuda"), torch.empty(40, 130, device="cuda")
+    cm.MatmulKernelFp8(a, sa, b, sb, want, 40, 256, 130)
+    w = torch.zeros(groups - 1 + m * k, dtype=torch.uint8, device="cuda")           # the groups' weights overlap: one byte apart
+    big = (torch.zeros(n, k, dtype=E4, device="cuda"), torch.zeros(up(k), n, device="cuda"), w.view(E4), torch.zeros(up(m), up(k), device="cuda"),
+           torch.zeros(n, m, device="cuda"), torch.zeros(groups + 1, dtype=torch.int32, device="cuda"), groups, n, k, m)
+    with pytest.raises(cm.CormorantError, match="memory"):
+        cm.MatmulKernelFp8Grouped(*big, ldb=k, b_group_stride=1, b_scale_ld=up(k), b_scale_group_stride=0)
+    cm.MatmulKernelFp8(a, sa, b, sb, c, 40, 256, 130)
+    assert torch.equal(c, want)
+    q, s = torch.empty(40, 130, dtype=E4, device="cuda"), torch.empty(2, 40, device="cuda")
+    with pytest.raises(cm.CormorantError, match="memory"):
+        cm.MatmulKernelFp8Grouped(*big, ldb=k, b_group_stride=1, b_scale_ld=up(k), b_scale_group_stride=0)
+    cm.QuantKernelFp8(c, q, s, 40, 130)
+    torch.cuda.synchronize()
