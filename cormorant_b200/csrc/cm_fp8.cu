@@ -544,6 +544,11 @@ __global__ void __launch_bounds__(THREADS, 1) rmsnorm_kernel(const NormArgs g) {
 // ---- host ---------------------------------------------------------------------------------------
 bool aligned(const void* p, uint64_t pitch_bytes, unsigned to) { return ((uintptr_t)p % to) == 0 && pitch_bytes % to == 0; }
 
+// Whether the matrices of a batch do not overlap: each behind the one before, or their rows side by side.
+bool apart(uint64_t rows, uint64_t ld, uint64_t cols, uint64_t batch, uint64_t stride) {
+    return stride >= (rows - 1) * ld + cols || (stride >= cols && ld >= (batch - 1) * stride + cols);
+}
+
 template <typename T, bool VEC, uint32_t FMT>
 void launch_quant(const QuantArgs& g, bool blocks, unsigned grid, cudaStream_t s) {
     if (blocks) launch_k(quant_blocks_kernel<T, VEC, FMT>, grid, 512, 0, s, g);
@@ -606,7 +611,7 @@ extern "C" int cm_quant_fp8_async(const void* x, unsigned x_type, uint8_t* q, fl
         if (!extent_ok(rows, ldx, cols, size) || !extent_ok(rows, ldq, cols, 1) || !extent_ok(s_outer, lds, s_inner, 4) ||
             !extent_ok(batch, x_batch_stride, 0, size) || !extent_ok(batch, q_batch_stride, 0, 1) || !extent_ok(batch, scale_batch_stride, 0, 4))
             return set_error(CM_EINVAL, "cm_quant_fp8: sizes overflow");
-        if (batch > 1 && (q_batch_stride < (rows - 1) * ldq + cols || scale_batch_stride < (s_outer - 1) * lds + s_inner))
+        if (batch > 1 && (!apart(rows, ldq, cols, batch, q_batch_stride) || !apart(s_outer, lds, s_inner, batch, scale_batch_stride)))
             return set_error(CM_EINVAL, "cm_quant_fp8: the outputs of two batch steps overlap");
     }
     const Context* cx;

@@ -398,7 +398,8 @@ int cm_matmul_prepared_async(const cm_matmul_weights_t* w, const int16_t* a, int
 #define CM_F8_E4M3  0u
 #define CM_F8_E5M2  1u
 /* x [batch][rows][cols] -> q and its scales; block_rows 1 (activations) or 128 (weights).
- * scale pitch lds >= rows (block_rows 1) or >= ceil(cols/128) (128).  x_batch_stride may be 0. */
+ * scale pitch lds >= rows (block_rows 1) or >= ceil(cols/128) (128).  x_batch_stride may be 0; the
+ * outputs of batch steps lie behind each other or, row by row, side by side. */
 int cm_quant_fp8(const void* x, unsigned x_type, uint8_t* q, float* scale, unsigned rows, unsigned cols,
                  unsigned batch, uint64_t ldx, uint64_t ldq, uint64_t lds, uint64_t x_batch_stride,
                  uint64_t q_batch_stride, uint64_t scale_batch_stride, unsigned format, unsigned block_rows);

@@ -91,6 +91,18 @@ def test_bad_arguments_are_refused(L, which, change):
     assert CALLS[which][0].encode() in L.cm_last_error()
 
 
+# Outputs of batch steps may lie behind each other or, row by row, side by side; not in each other.
+SIDE_BY_SIDE = [(dict(batch=2, q_bs=300, ldq=600), ENOINIT), (dict(batch=3, s_bs=5, lds=15), ENOINIT), (dict(batch=2, rows=1, q_bs=300, s_bs=1, lds=2), ENOINIT),
+                (dict(batch=2, block_rows=128, rows=200, q_bs=300, ldq=700, s_bs=3, lds=6), ENOINIT), (dict(batch=2, q_bs=299, ldq=600), EINVAL),
+                (dict(batch=2, q_bs=300, ldq=599), EINVAL), (dict(batch=3, s_bs=4, lds=15), EINVAL), (dict(batch=3, s_bs=5, lds=14), EINVAL),
+                (dict(batch=2, q_bs=0, ldq=600), EINVAL), (dict(batch=2, cols=128, s_bs=4), EINVAL)]
+
+
+@pytest.mark.parametrize("change,want", SIDE_BY_SIDE, ids=lambda v: "-".join(f"{k}{x}" for k, x in v.items()) if isinstance(v, dict) else str(v))
+def test_outputs_of_batch_steps(L, change, want):
+    assert call(L, "quant", **change) == want, L.cm_last_error()
+
+
 @pytest.mark.parametrize("which,change", [
     ("norm", dict(type=0)), ("norm", dict(weight_type=0)),
     ("norm", dict(cols=32769, ldx=32769, ldr=32769, ldo=32769, ldy=32769, ldq=32769)),

@@ -140,6 +140,21 @@ def test_quant_batch_and_broadcast(cm, br):
     assert torch.equal(q[2].view(torch.uint8), q[0].view(torch.uint8)) and torch.equal(scale[2], scale[0])
 
 
+@pytest.mark.parametrize("br", [1, 128])
+@pytest.mark.parametrize("batch,rows,cols", [(3, 130, 200), (4, 1, 300), (2, 70, 1024)])
+def test_quant_batch_side_by_side(cm, br, batch, rows, cols):
+    """Batch steps whose output rows lie between each other's: one operand of all steps' columns, scales of all steps' rows."""
+    x = values(8, batch, rows, cols).to(BF16).cuda()
+    q = torch.full((rows, batch, cols), 0x55, dtype=torch.uint8, device="cuda").view(E4)
+    outer, inner = (up(cols), rows) if br == 1 else (up(rows), up(cols))
+    scale = torch.full((outer, batch, inner), -7.0, device="cuda")
+    cm.QuantKernelFp8(x, q.permute(1, 0, 2), scale.permute(1, 0, 2), rows, cols, batch, block_rows=br)
+    for z in range(batch):
+        want_q, want_s = plain_quant(x[z].float().cpu(), E4, br)
+        assert torch.equal(q[:, z].float().cpu(), want_q)
+        assert torch.equal(scale[:, z].cpu(), want_s.t() if br == 1 else want_s)
+
+
 @pytest.mark.parametrize("fmt", [E4, E5])
 @pytest.mark.parametrize("br", [1, 128])
 def test_quant_infinities_nan_and_extremes(cm, fmt, br):
