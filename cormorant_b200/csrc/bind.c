@@ -92,7 +92,6 @@ typedef struct {
     void* p;
     uint64_t ld, bs;      /* row pitch, batch stride, in elements */
     int code;             /* element type or format, or ANY */
-    int given;            /* not None */
 } Mat;
 
 /* Elements from t's first one to its last. */
@@ -111,8 +110,8 @@ static uint64_t room_of(PyObject* shape, PyObject* stride) {
  * given (the dimensions before the last two are one batch as far as their matrices lie an even stride
  * apart); what is missing is dense.  Nothing beyond a tensor's own last element is reached. */
 static int matrix(PyObject* t, uint64_t rows, uint64_t cols, PyObject* ld, int kind, const char* what, uint64_t batch, PyObject* bs, Mat* m) {
-    m->p = NULL; m->ld = m->bs = 0; m->code = ANY; m->given = t != Py_None;
-    if (!m->given) return 0;
+    m->p = NULL; m->ld = m->bs = 0; m->code = ANY;
+    if (t == Py_None) return 0;
     const int has_ld = ld && ld != Py_None, has_bs = bs && bs != Py_None;
     if (has_ld && as_u64(ld, &m->ld)) return -1;
     if (has_bs && as_u64(bs, &m->bs)) return -1;
