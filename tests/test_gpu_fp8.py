@@ -1009,3 +1009,42 @@ def test_a_refused_allocation_is_not_the_next_calls_error(cm):
         cm.MatmulKernelFp8Grouped(*big, ldb=k, b_group_stride=1, b_scale_ld=up(k), b_scale_group_stride=0)
     cm.QuantKernelFp8(c, q, s, 40, 130)
     torch.cuda.synchronize()
+
+
+FIRST_CAPTURED = """
+import sys
+import torch
+import cormorant_b200 as cm
+sys.path.insert(0, "tests")
+import test_gpu_fp8 as T
+cm.init("0")
+sizes = [(1, 4096, 256), (70, 512, 4096), (300, 1000, 1001), (1100, 512, 1300), (3000, 250, 2304)]
+data = [[v.cuda() for v in T.operands(n, n, k, m)] for n, k, m in sizes]
+out = [torch.empty(n, m, device="cuda") for n, k, m in sizes]
+x, q, s = T.values(1, 37, 1000).cuda(), torch.empty(37, 1000, dtype=T.E4, device="cuda"), torch.empty(8, 37, device="cuda")
+torch.cuda.synchronize()
+graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+with torch.cuda.graph(graph, stream=stream):
+    for d, size, c in zip(data, sizes, out):
+        cm.MatmulKernelFp8(*d, c, *size, stream=stream)
+    cm.QuantKernelFp8(x, q, s, 37, 1000, stream=stream)
+for _ in range(2):
+    for c in out:
+        c.fill_(float("nan"))
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    for d, (n, k, m), c in zip(data, sizes, out):
+        T.check_product(c.cpu(), *T.product64(*(v.cpu() for v in d)), k, T.F32)
+    assert torch.equal(q.float().cpu(), T.plain_quant(x.cpu(), T.E4, 1)[0])
+print("done")
+"""
+
+
+def test_first_calls_captured():
+    """A process whose first calls are recorded into a graph, one with operands that are copied into aligned rows."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", FIRST_CAPTURED], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "done", r.stderr[-2000:]
