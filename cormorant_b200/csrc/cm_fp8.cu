@@ -15,7 +15,7 @@
 // Rows whose base or pitch is not a multiple of the vector sizes keep this layout: a chunk is cut out
 // of the two (fp32: three) aligned 16-byte words that hold it, and 8-bit and 16-bit results leave as
 // aligned 32-bit words put together from neighbouring lanes' (8192 x 1001 bf16, one element an access:
-// 26.9 us quantised and 55.7 us normed; this way 10.6 and 27).  What lies behind a row's end in its
+// 26.9 us quantised and 55.7 us normed; this way 9.7 and 24).  What lies behind a row's end in its
 // last words is cleared where the values are used: done at the load, or by blocks that take another
 // path than whole ones, it cost 8192 x 2000 bf16 normed 31 us instead of 22.
 #include <algorithm>
