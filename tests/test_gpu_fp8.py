@@ -992,7 +992,7 @@ def test_matmul_q88_of_nan_and_infinity(cm, n, k, m):
 
 
 def test_a_refused_allocation_is_not_the_next_calls_error(cm):
-    """A product whose aligned copies would take 1 TB is answered with CM_ENOMEM, and the next call is judged by itself."""
+    """A product whose aligned copies would take 1 TB is answered with CM_ENOMEM, and the next call has a result of its own."""
     n, k, m, groups = 1, 1000, 1 << 20, 1024
     a, sa, b, sb = (t.cuda() for t in operands(3, 40, 256, 130))
     want, c = torch.empty(40, 130, device="cuda"), torch.empty(40, 130, device="cuda")
